@@ -31,6 +31,11 @@ extern "C" {
 #define FLUXB_F32 0
 #define FLUXB_BF16 1
 
+/* Element types of position ids (fluxb_rope_axes). */
+#define FLUXB_ID_F32 0
+#define FLUXB_ID_I32 1
+#define FLUXB_ID_I64 2
+
 /* GEMM epilogues (fluxb_linear). */
 #define FLUXB_EPI_NONE 0       /* y = acc + bias */
 #define FLUXB_EPI_GELU 1       /* y = gelu_tanh(acc + bias) */
@@ -285,6 +290,76 @@ int fluxb_linear_qkv_grouped_scatter(const fluxb_linear_problem* problems, const
                                      void* const* group_bases, int n_groups, int64_t k_off, int64_t v_off,
                                      int64_t o_sb, int64_t o_sh, int64_t o_sl, float eps, int64_t N2, int epi2,
                                      int round_before_act, fluxb_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Operators next to the block path that the reference has no counterpart for: LayerNorm with a
+ * learned scale and offset, the backward pass of both LayerNorm forms, rotary positions from
+ * position ids, and per-request low-rank adapters.
+ * ------------------------------------------------------------------------------------- */
+
+/*
+ * fluxb_layer_norm_modulation (same kernels, same y) that also stores each row's mean and
+ * 1/sqrt(var + eps), fp32, for fluxb_layer_norm_bwd.
+ */
+int fluxb_layer_norm_modulation_stats(const void* x, const void* scale, const void* shift, void* y, float* mean,
+                                      float* rstd, int64_t rows, int64_t cols, int64_t rows_per_batch, int64_t x_ld,
+                                      int64_t y_ld, int64_t mod_stride, float eps, int dtype, fluxb_stream_t stream);
+
+/*
+ * y = (x - mean) * rstd * (unit + factor[g]) + offset[g], g = row / rows_per_group.  unit = 0 is
+ * LayerNorm with a learned scale (one group: rows_per_group = rows), unit = 1 the modulated form.
+ * Any width and alignment; x rows x_ld apart, y rows y_ld apart, factor and offset vec_stride
+ * apart from group to group.  factor NULL: ones in place of unit + factor; offset NULL: zeros.
+ * mean, rstd: fp32 per row, both or neither.  rows must be a multiple of rows_per_group.
+ */
+int fluxb_layer_norm(const void* x, const void* factor, const void* offset, void* y, float* mean, float* rstd,
+                     int64_t rows, int64_t cols, int64_t rows_per_group, int64_t x_ld, int64_t y_ld,
+                     int64_t vec_stride, float unit, float eps, int dtype, fluxb_stream_t stream);
+
+/*
+ * Backward of the above: with h = (x - mean) rstd and g = dy (unit + factor),
+ *   dx = rstd (g - mean(g) - h mean(g h)),  dfactor[grp] = sum dy h,  doffset[grp] = sum dy
+ * over the rows of each group.  mean and rstd are the forward's.  dx, dfactor, doffset may be
+ * NULL (not wanted).  dfactor and doffset are [groups, cols], fp32 if grads_f32 else of `dtype`;
+ * summed in fp32 in a fixed order.  scratch: fluxb_layer_norm_bwd_scratch() floats, needed when
+ * dfactor or doffset is wanted, contents undefined afterwards.  rows = 0 writes nothing.
+ */
+int64_t fluxb_layer_norm_bwd_scratch(int64_t rows, int64_t cols, int64_t rows_per_group);
+int fluxb_layer_norm_bwd(const void* dy, const void* x, const void* factor, const float* mean, const float* rstd,
+                         void* dx, void* dfactor, void* doffset, float* scratch, int64_t rows, int64_t cols,
+                         int64_t rows_per_group, int64_t dy_ld, int64_t x_ld, int64_t dx_ld, int64_t vec_stride,
+                         float unit, int grads_f32, int dtype, fluxb_stream_t stream);
+
+/*
+ * Rotary positions with several axes, from position ids instead of a table: the pairs (2j, 2j+1)
+ * of a head are dealt to the axes in order, axes_dim[i] columns to axis i, and pair j' of an axis
+ * of d columns turns by ids[b, l, axis] * theta^(-2 j'/d).  Columns behind the axes are copied.
+ * The angle is taken in fp64.  backward != 0 turns the other way: the gradient.
+ *   q, k, oq, ok: [B, heads, L, D], each with strides (batch, head, row) in elements, unit stride
+ *   on D; Hq and Hk may differ and either may be 0.  ids: [B, L, n_axes] of id_type
+ *   (FLUXB_ID_*) with its three strides (0 to share).  At most 8 axes and 128 rotated pairs.
+ */
+int fluxb_rope_axes(const void* q, void* oq, const int64_t* q_strides, const int64_t* oq_strides, int64_t Hq,
+                    const void* k, void* ok, const int64_t* k_strides, const int64_t* ok_strides, int64_t Hk,
+                    const void* ids, int id_type, const int64_t* id_strides, int64_t B, int64_t L, int64_t D,
+                    const int64_t* axes_dim, int n_axes, double theta, int backward, int dtype,
+                    fluxb_stream_t stream);
+
+/*
+ * A shared projection plus one low-rank adapter per request:
+ *   y[m] = act(x[m] w^T + bias + scale[a] (x[m] A_a^T) B_a^T),  a = adapter[m / L],  m < B*L
+ * bf16, fp32 accumulation; epi FLUXB_EPI_NONE or FLUXB_EPI_GELU.  x [B*L, K] (ldx), w [N, K] (ldw),
+ * y [B*L, N] (ldy), lora_a [n_adapters, R, K], lora_b [n_adapters, N, R] contiguous, lora_scale
+ * fp32 [n_adapters] or NULL (ones), adapter int32 or int64 [B] on the device.  adapter -1: the
+ * request has none; any other value outside [0, n_adapters) counts as -1 and sets the device
+ * status word (FLUXB_ERR_BAD_ARG, site 81).  K, N and the row strides are multiples of 8, pointers
+ * 16-byte aligned.  scratch: fluxb_linear_lora_scratch_bytes() bytes.
+ */
+int64_t fluxb_linear_lora_scratch_bytes(int64_t M, int64_t N, int64_t K, int64_t R);
+int fluxb_linear_lora(const void* x, const void* w, const void* bias, void* y, const void* lora_a, const void* lora_b,
+                      const float* lora_scale, const void* adapter, int adapter_is64, void* scratch, int64_t B,
+                      int64_t L, int64_t N, int64_t K, int64_t R, int64_t n_adapters, int64_t ldx, int64_t ldw,
+                      int64_t ldy, int epi, fluxb_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------
  * Sequence-parallel (Ulysses) exchange over peer memory.  The reference has no multi-GPU path,

@@ -14,12 +14,22 @@ from triton_kernels_b200.functional import (
     rms_norm_torch,
     rms_norm_torch_compile,
 )
-from triton_kernels_b200.kernels import apply_rope, layer_norm_modulation, linear, rms_norm, scaled_dot_product_attention
-from triton_kernels_b200.modules import DoubleStreamBlock, QKNorm, RMSNorm, SingleStreamBlock
+from triton_kernels_b200.kernels import (
+    apply_rope,
+    apply_rope_axes,
+    layer_norm,
+    layer_norm_modulation,
+    linear,
+    linear_lora,
+    rms_norm,
+    scaled_dot_product_attention,
+)
+from triton_kernels_b200.modules import DoubleStreamBlock, LayerNorm, LinearLoRA, QKNorm, RMSNorm, SingleStreamBlock
 
 __all__ = [
     "apply_rope_torch", "apply_rope_torch_compile", "layer_norm_modulation_torch",
     "layer_norm_modulation_torch_compile", "rms_norm_torch", "rms_norm_torch_compile",
     "apply_rope", "layer_norm_modulation", "linear", "rms_norm", "scaled_dot_product_attention",
     "DoubleStreamBlock", "QKNorm", "RMSNorm", "SingleStreamBlock",
+    "apply_rope_axes", "layer_norm", "linear_lora", "LayerNorm", "LinearLoRA",
 ]

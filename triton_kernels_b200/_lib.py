@@ -7,7 +7,8 @@ PyTorch fallback.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p, POINTER
+from contextlib import nullcontext
+from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_void_p, POINTER
 from pathlib import Path
 
 import torch
@@ -15,6 +16,7 @@ import torch
 LIB_PATH = Path(__file__).resolve().parent / "libfluxb200.so"
 
 F32, BF16 = 0, 1
+ID_F32, ID_I32, ID_I64 = 0, 1, 2
 EPI_NONE, EPI_GELU, EPI_GATE_RESID = 0, 1, 2
 ERR_BAD_ARG, ERR_UNSUPPORTED, ERR_CUDA, ERR_TIMEOUT = -1, -2, -3, -4
 
@@ -62,6 +64,13 @@ SIGNATURES = {
     "fluxb_modulation_scale_shift": (_I, [_P, _P, _P, _L, _L, _L, _L, _I, _I, _P]),
     "fluxb_modulation_gate_proj": (_I, [_P, _P, _P, _P, _L, _L, _L, _L, _I, _I, _P]),
     "fluxb_silu": (_I, [_P, _P, _L, _I, _P]),
+    "fluxb_layer_norm_modulation_stats": (_I, [_P] * 6 + [_L] * 6 + [_F, _I, _P]),
+    "fluxb_layer_norm": (_I, [_P] * 6 + [_L] * 6 + [_F, _F, _I, _P]),
+    "fluxb_layer_norm_bwd_scratch": (_L, [_L, _L, _L]),
+    "fluxb_layer_norm_bwd": (_I, [_P] * 9 + [_L] * 7 + [_F, _I, _I, _P]),
+    "fluxb_rope_axes": (_I, [_P, _P, _P, _P, _L, _P, _P, _P, _P, _L, _P, _I, _P, _L, _L, _L, _P, _I, c_double, _I, _I, _P]),
+    "fluxb_linear_lora_scratch_bytes": (_L, [_L] * 4),
+    "fluxb_linear_lora": (_I, [_P] * 8 + [_I, _P] + [_L] * 9 + [_I, _P]),
     "fluxb_peer_header_bytes": (_I, []),
     "fluxb_peer_alloc": (_I, [_L, POINTER(c_void_p)]),
     "fluxb_peer_free": (_I, [_P]),
@@ -136,6 +145,21 @@ def require_cuda(*tensors: torch.Tensor) -> None:
 
 def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
+
+
+def on_device_of(t: torch.Tensor):
+    """Context that makes t's device current for the launch: a no-op where it is already."""
+    index = t.device.index
+    return _HERE if index is None or index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+_HERE = nullcontext()
+
+
+def require_same_device(first: torch.Tensor, *others: torch.Tensor) -> None:
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise RuntimeError(f"fluxb200 kernels take tensors of one device; got {first.device} and {t.device}")
 
 
 def stream_handle() -> int:

@@ -16,64 +16,9 @@
 
 #include <mutex>
 
-#include "common.cuh"
+#include "vec.cuh"
 
 namespace fluxb {
-
-// ----------------------------------------------------------------------------------------
-// 16-byte vector access for fp32 / bf16 rows, presented to the math as fp32 lanes.
-// ----------------------------------------------------------------------------------------
-template <typename T>
-struct Vec;
-template <>
-struct Vec<float> {
-  static constexpr int N = 4;
-  float v[4];
-  __device__ __forceinline__ void unpack(const uint4& t) {
-    v[0] = __uint_as_float(t.x); v[1] = __uint_as_float(t.y);
-    v[2] = __uint_as_float(t.z); v[3] = __uint_as_float(t.w);
-  }
-  __device__ __forceinline__ void load(const float* p) {
-    float4 t = *reinterpret_cast<const float4*>(p);
-    v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
-  }
-  __device__ __forceinline__ void load_nc(const float* p) {
-    float4 t = __ldg(reinterpret_cast<const float4*>(p));
-    v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
-  }
-  __device__ __forceinline__ void store(float* p) const {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  }
-};
-template <>
-struct Vec<__nv_bfloat16> {
-  static constexpr int N = 8;
-  float v[8];
-  __device__ __forceinline__ void unpack(const uint4& t) {
-    v[0] = bf16_lo(t.x); v[1] = bf16_hi(t.x); v[2] = bf16_lo(t.y); v[3] = bf16_hi(t.y);
-    v[4] = bf16_lo(t.z); v[5] = bf16_hi(t.z); v[6] = bf16_lo(t.w); v[7] = bf16_hi(t.w);
-  }
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) {
-    unpack(*reinterpret_cast<const uint4*>(p));
-  }
-  __device__ __forceinline__ void load_nc(const __nv_bfloat16* p) {
-    unpack(__ldg(reinterpret_cast<const uint4*>(p)));
-  }
-  __device__ __forceinline__ void store(__nv_bfloat16* p) const {
-    uint4 t;
-    t.x = pack_bf16(v[0], v[1]); t.y = pack_bf16(v[2], v[3]);
-    t.z = pack_bf16(v[4], v[5]); t.w = pack_bf16(v[6], v[7]);
-    *reinterpret_cast<uint4*>(p) = t;
-  }
-};
-
-// Makes the compiler forget what it knows about a packed vector, so the fp32 widening is redone
-// at each use instead of being kept live (which doubles the registers of a bf16 row).
-__device__ __forceinline__ void forget(uint4& t) {
-  asm volatile("" : "+r"(t.x), "+r"(t.y), "+r"(t.z), "+r"(t.w));
-}
-
-__device__ __forceinline__ uint4 ld_nc_u4(const void* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 
 template <int G>
 __device__ __forceinline__ float group_sum(float v) {
@@ -108,8 +53,8 @@ struct RowAddr {
 template <typename T, int G, int VPL>
 __global__ void __launch_bounds__(256, (VPL <= 12 ? 3 : (VPL <= 24 ? 2 : 1)))
 ln_mod_rows_kernel(const T* __restrict__ x, const T* __restrict__ scale, const T* __restrict__ shift,
-                   T* __restrict__ y, int64_t rows, int cols, int64_t rows_per_batch, int64_t x_ld,
-                   int64_t y_ld, int64_t mod_stride, float eps) {
+                   T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t rows, int cols,
+                   int64_t rows_per_batch, int64_t x_ld, int64_t y_ld, int64_t mod_stride, float eps) {
   constexpr int VN = Vec<T>::N;
   const int lane_in_group = threadIdx.x % G;
   const int64_t groups_per_block = blockDim.x / G;
@@ -147,6 +92,7 @@ ln_mod_rows_kernel(const T* __restrict__ x, const T* __restrict__ scale, const T
     }
   }
   const float rstd = rsqrtf(group_sum<G>(q) / cols + eps);
+  if (mean_out != nullptr && active && lane_in_group == 0) { mean_out[r] = mean; rstd_out[r] = rstd; }
 
   const int64_t b = r / rows_per_batch;
   const T* sc = scale + b * mod_stride;
@@ -170,9 +116,9 @@ ln_mod_rows_kernel(const T* __restrict__ x, const T* __restrict__ scale, const T
 template <typename T>
 __global__ void __launch_bounds__(256)
 ln_mod_generic_kernel(const T* __restrict__ x, const T* __restrict__ scale,
-                      const T* __restrict__ shift, T* __restrict__ y, int64_t rows, int cols,
-                      int64_t rows_per_batch, int64_t x_ld, int64_t y_ld, int64_t mod_stride,
-                      float eps) {
+                      const T* __restrict__ shift, T* __restrict__ y, float* __restrict__ mean_out,
+                      float* __restrict__ rstd_out, int64_t rows, int cols, int64_t rows_per_batch, int64_t x_ld,
+                      int64_t y_ld, int64_t mod_stride, float eps) {
   constexpr int VN = Vec<T>::N;
   const int lane = threadIdx.x & 31;
   const int64_t row = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
@@ -197,6 +143,7 @@ ln_mod_generic_kernel(const T* __restrict__ x, const T* __restrict__ scale,
     }
   }
   const float rstd = rsqrtf(warp_sum(q) / cols + eps);
+  if (mean_out != nullptr && lane == 0) { mean_out[row] = mean; rstd_out[row] = rstd; }
   const int64_t b = row / rows_per_batch;
   const T* sc = scale + b * mod_stride;
   const T* sh = shift + b * mod_stride;
@@ -252,7 +199,7 @@ constexpr int kBulkHeaderBytes = 256;  // mbarriers: one per warp (up to 16) + o
 template <typename T, bool kLayerNorm, bool kStagedMod, int kVPL>
 __global__ void __launch_bounds__(512, 2)
 norm_rows_bulk_kernel(const T* __restrict__ x, const T* __restrict__ scale, const T* __restrict__ shift,
-                      T* __restrict__ y, float* __restrict__ rstd_out, int64_t rows, int cols,
+                      T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t rows, int cols,
                       int64_t rows_per_batch, RowAddr xaddr, int64_t y_ld, int64_t mod_stride, float eps,
                       DeviceStatus* status) {
   constexpr int VN = Vec<T>::N;
@@ -319,6 +266,7 @@ norm_rows_bulk_kernel(const T* __restrict__ x, const T* __restrict__ scale, cons
     const float ds = warp_sum(s) / cols;
     mean = pivot + ds;
     rstd = rsqrtf(fmaxf(warp_sum(q) / cols - ds * ds, 0.f) + eps);
+    if (mean_out != nullptr && lane == 0) { mean_out[row] = mean; rstd_out[row] = rstd; }
   } else {
     float q = 0.f;
 #pragma unroll(kVPL > 0 ? kVPL : 1)
@@ -390,7 +338,7 @@ static inline bool bulk_rows_ok(int64_t cols, size_t elt, const RowAddr& a) {
 }
 
 template <typename T, bool kLayerNorm, bool kStagedMod>
-static int launch_norm_bulk_as(const T* x, const T* scale, const T* shift, T* y, float* rstd, int64_t rows,
+static int launch_norm_bulk_as(const T* x, const T* scale, const T* shift, T* y, float* mean, float* rstd, int64_t rows,
                                int64_t cols, int64_t rpb, RowAddr xaddr, int64_t y_ld, int64_t mod_stride,
                                float eps, cudaStream_t st) {
   const int warps = kStagedMod ? 16 : 8;
@@ -403,14 +351,14 @@ static int launch_norm_bulk_as(const T* x, const T* scale, const T* shift, T* y,
   if (e != cudaSuccess)
     return set_error(FLUXB_ERR_CUDA, "row norm: cannot set shared memory size: %s", cudaGetErrorString(e));
   kern<<<(unsigned)((rows + warps - 1) / warps), warps * 32, smem, st>>>(
-      x, scale, shift, y, rstd, rows, (int)cols, rpb, xaddr, y_ld, mod_stride, eps, device_status_ptr());
+      x, scale, shift, y, mean, rstd, rows, (int)cols, rpb, xaddr, y_ld, mod_stride, eps, device_status_ptr());
   return FLUXB_OK;
 }
 
 // Rows of up to 6 KB whose blocks of 16 rows each stay inside one batch element, with 16-byte
 // aligned per-column vectors, take the form that stages those vectors in shared memory.
 template <typename T, bool kLayerNorm>
-static int launch_norm_bulk(const T* x, const T* scale, const T* shift, T* y, float* rstd, int64_t rows,
+static int launch_norm_bulk(const T* x, const T* scale, const T* shift, T* y, float* mean, float* rstd, int64_t rows,
                             int64_t cols, int64_t rpb, RowAddr xaddr, int64_t y_ld, int64_t mod_stride, float eps,
                             cudaStream_t st) {
   const bool aligned = (reinterpret_cast<uintptr_t>(scale) & 15) == 0 &&
@@ -418,15 +366,15 @@ static int launch_norm_bulk(const T* x, const T* scale, const T* shift, T* y, fl
                                         (mod_stride * (int64_t)sizeof(T)) % 16 == 0));
   const bool one_batch_per_block = !kLayerNorm || rpb % 16 == 0 || rows <= rpb;
   if (cols * (int64_t)sizeof(T) <= 6144 && aligned && one_batch_per_block)
-    return launch_norm_bulk_as<T, kLayerNorm, true>(x, scale, shift, y, rstd, rows, cols, rpb, xaddr, y_ld,
+    return launch_norm_bulk_as<T, kLayerNorm, true>(x, scale, shift, y, mean, rstd, rows, cols, rpb, xaddr, y_ld,
                                                     mod_stride, eps, st);
-  return launch_norm_bulk_as<T, kLayerNorm, false>(x, scale, shift, y, rstd, rows, cols, rpb, xaddr, y_ld,
+  return launch_norm_bulk_as<T, kLayerNorm, false>(x, scale, shift, y, mean, rstd, rows, cols, rpb, xaddr, y_ld,
                                                    mod_stride, eps, st);
 }
 
 template <typename T>
-static int launch_ln_mod(const void* x, const void* scale, const void* shift, void* y, int64_t rows,
-                         int64_t cols, int64_t rpb, int64_t x_ld, int64_t y_ld, int64_t mod_stride,
+static int launch_ln_mod(const void* x, const void* scale, const void* shift, void* y, float* mean, float* rstd,
+                         int64_t rows, int64_t cols, int64_t rpb, int64_t x_ld, int64_t y_ld, int64_t mod_stride,
                          float eps, cudaStream_t st) {
   constexpr int VN = Vec<T>::N;
   const T* xp = static_cast<const T*>(x);
@@ -437,14 +385,14 @@ static int launch_ln_mod(const void* x, const void* scale, const void* shift, vo
   {
     RowAddr xaddr{1, rows > 0 ? rows : 1, 0, 0, x_ld, 1};
     if (bulk_rows_ok(cols, sizeof(T), xaddr) && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
-      return launch_norm_bulk<T, true>(xp, sc, sh, yp, nullptr, rows, cols, rpb, xaddr, y_ld, mod_stride, eps, st);
+      return launch_norm_bulk<T, true>(xp, sc, sh, yp, mean, rstd, rows, cols, rpb, xaddr, y_ld, mod_stride, eps, st);
     }
   }
 #define FLUXB_LN_CASE(G, VPL)                                                                  \
   if (vecs == (G) * (VPL)) {                                                                   \
     const int64_t gpb = 256 / (G);                                                             \
     ln_mod_rows_kernel<T, G, VPL><<<(unsigned)((rows + gpb - 1) / gpb), 256, 0, st>>>(         \
-        xp, sc, sh, yp, rows, (int)cols, rpb, x_ld, y_ld, mod_stride, eps);                    \
+        xp, sc, sh, yp, mean, rstd, rows, (int)cols, rpb, x_ld, y_ld, mod_stride, eps);        \
     return FLUXB_OK;                                                                           \
   }
   FLUXB_LN_CASE(32, 1) FLUXB_LN_CASE(32, 2) FLUXB_LN_CASE(32, 3) FLUXB_LN_CASE(32, 4)
@@ -452,7 +400,7 @@ static int launch_ln_mod(const void* x, const void* scale, const void* shift, vo
   FLUXB_LN_CASE(32, 24)
 #undef FLUXB_LN_CASE
   ln_mod_generic_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(
-      xp, sc, sh, yp, rows, (int)cols, rpb, x_ld, y_ld, mod_stride, eps);
+      xp, sc, sh, yp, mean, rstd, rows, (int)cols, rpb, x_ld, y_ld, mod_stride, eps);
   return FLUXB_OK;
 }
 
@@ -575,7 +523,7 @@ static int launch_rms(const void* x, const void* w, void* y, float* rstd, int64_
   T* yp = static_cast<T*>(y);
   const int64_t vecs = cols / VN;
   if (bulk_rows_ok(cols, sizeof(T), addr) && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
-    return launch_norm_bulk<T, false>(xp, wp, nullptr, yp, rstd, rows, cols, 1, addr, cols, 0, eps, st);
+    return launch_norm_bulk<T, false>(xp, wp, nullptr, yp, nullptr, rstd, rows, cols, 1, addr, cols, 0, eps, st);
   }
 #define FLUXB_RMS_CASE(G, VPL)                                                                 \
   if (vecs == (G) * (VPL)) {                                                                   \
@@ -1199,11 +1147,9 @@ static inline int launch_status(const char* what) {
 }
 static inline int vec_elems(int dtype) { return dtype == FLUXB_BF16 ? 8 : 4; }
 
-extern "C" int fluxb_layer_norm_modulation(const void* x, const void* scale, const void* shift,
-                                           void* y, int64_t rows, int64_t cols,
-                                           int64_t rows_per_batch, int64_t x_ld, int64_t y_ld,
-                                           int64_t mod_stride, float eps, int dtype,
-                                           fluxb_stream_t stream) {
+static int layer_norm_modulation_impl(const void* x, const void* scale, const void* shift, void* y, float* mean,
+                                      float* rstd, int64_t rows, int64_t cols, int64_t rows_per_batch, int64_t x_ld,
+                                      int64_t y_ld, int64_t mod_stride, float eps, int dtype, fluxb_stream_t stream) {
   if (dtype != FLUXB_F32 && dtype != FLUXB_BF16)
     return set_error(FLUXB_ERR_UNSUPPORTED, "layer_norm_modulation: dtype %d", dtype);
   if (rows < 0 || cols <= 0 || rows_per_batch < 0)
@@ -1220,12 +1166,30 @@ extern "C" int fluxb_layer_norm_modulation(const void* x, const void* scale, con
                      "pointers 16-byte aligned", vn);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int rc = dtype == FLUXB_BF16
-                     ? launch_ln_mod<__nv_bfloat16>(x, scale, shift, y, rows, cols, rows_per_batch, x_ld, y_ld,
-                                                    mod_stride, eps, st)
-                     : launch_ln_mod<float>(x, scale, shift, y, rows, cols, rows_per_batch, x_ld, y_ld, mod_stride,
-                                            eps, st);
+                     ? launch_ln_mod<__nv_bfloat16>(x, scale, shift, y, mean, rstd, rows, cols, rows_per_batch, x_ld,
+                                                    y_ld, mod_stride, eps, st)
+                     : launch_ln_mod<float>(x, scale, shift, y, mean, rstd, rows, cols, rows_per_batch, x_ld, y_ld,
+                                            mod_stride, eps, st);
   if (rc != FLUXB_OK) return rc;
   return launch_status("layer_norm_modulation");
+}
+
+extern "C" int fluxb_layer_norm_modulation(const void* x, const void* scale, const void* shift,
+                                           void* y, int64_t rows, int64_t cols,
+                                           int64_t rows_per_batch, int64_t x_ld, int64_t y_ld,
+                                           int64_t mod_stride, float eps, int dtype,
+                                           fluxb_stream_t stream) {
+  return layer_norm_modulation_impl(x, scale, shift, y, nullptr, nullptr, rows, cols, rows_per_batch, x_ld, y_ld,
+                                    mod_stride, eps, dtype, stream);
+}
+
+extern "C" int fluxb_layer_norm_modulation_stats(const void* x, const void* scale, const void* shift, void* y,
+                                                 float* mean, float* rstd, int64_t rows, int64_t cols,
+                                                 int64_t rows_per_batch, int64_t x_ld, int64_t y_ld, int64_t mod_stride,
+                                                 float eps, int dtype, fluxb_stream_t stream) {
+  if (rows > 0 && (!mean || !rstd)) return set_error(FLUXB_ERR_BAD_ARG, "layer_norm_modulation_stats: null pointer");
+  return layer_norm_modulation_impl(x, scale, shift, y, mean, rstd, rows, cols, rows_per_batch, x_ld, y_ld, mod_stride,
+                                    eps, dtype, stream);
 }
 
 extern "C" int fluxb_rms_norm(const void* x, const void* w, void* y, float* rstd, int64_t n0,

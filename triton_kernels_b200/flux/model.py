@@ -22,6 +22,7 @@ from torch import Tensor, nn
 from triton_kernels_b200 import _lib
 from triton_kernels_b200.kernels.linear import linear, linear_into
 from triton_kernels_b200.kernels.normalization import layer_norm_modulation_into
+from triton_kernels_b200.kernels.positional_embedding import apply_rope_axes
 from triton_kernels_b200.modules.blocks import DoubleStreamBlock, SingleStreamBlock
 from triton_kernels_b200.ops.fused import modulation_silu_linear
 
@@ -47,6 +48,11 @@ class EmbedND(nn.Module):
     def forward(self, ids: Tensor) -> Tensor:
         tables = [rope_table(ids[..., a], self.axes_dim[a], self.theta) for a in range(ids.shape[-1])]
         return torch.cat(tables, dim=-3).unsqueeze(1)
+
+    def rotate(self, xq: Tensor, xk: Tensor, ids: Tensor) -> tuple[Tensor, Tensor]:
+        """xq and xk [B, H, L, D] rotated by the positions `ids` [B or 1, L, n_axes], without a table:
+        requests of one batch may have positions of their own, and gradients pass."""
+        return apply_rope_axes(xq, xk, ids, self.axes_dim, self.theta)
 
 
 def flux_position_ids(txt_len: int, grid_h: int, grid_w: int, device=None) -> Tensor:

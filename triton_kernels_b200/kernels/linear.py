@@ -1,4 +1,5 @@
-"""`linear(x, w, b, activation)` on the tcgen05 GEMM (reference: triton_kernels/kernels/linear.py:104-151)."""
+"""`linear(x, w, b, activation)` on the tcgen05 GEMM (reference: triton_kernels/kernels/linear.py:104-151), and
+`linear_lora`, the same projection with a low-rank adapter per request."""
 from __future__ import annotations
 
 import torch
@@ -207,3 +208,64 @@ def linear(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None, activation:
     else:
         linear_into(x2d, w, b, y, epi=_lib.EPI_GELU if activation == "GELU" else _lib.EPI_NONE)
     return y.reshape(*lead, N)
+
+
+def _dense16(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous and 16-byte aligned; a copy where it is not."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def linear_lora(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None, lora_a: torch.Tensor, lora_b: torch.Tensor,
+                adapter: torch.Tensor, lora_scale: torch.Tensor | None = None, activation: str = "") -> torch.Tensor:
+    """act(x @ w.T + b + scale_a * (x @ A_a.T) @ B_a.T): a projection shared by all requests plus one
+    low-rank adapter per request, a = adapter[request].  bf16 in/out, fp32 accumulation; forward only.
+
+    x [B, ..., K]: the first dim counts the requests (x [B, K] is one row per request).  w [N, K], b
+    [N] or None as in `linear`; lora_a [n, R, K], lora_b [n, N, R] bf16; lora_scale [n] fp32 or None
+    (ones); adapter [B] int32 or int64 on x's device, -1 for a request without an adapter.  The
+    values of `adapter` are read on the device: one outside [-1, n) counts as -1 and is recorded in
+    the device status word (`_lib.device_status`).  activation: "" or "GELU" (tanh form)."""
+    assert x.dim() >= 2 and x.shape[-1] == w.shape[-1], "Incompatible dimensions"
+    N, K = w.shape
+    n, R = lora_a.shape[:2]
+    assert n > 0 and R > 0 and lora_a.shape == (n, R, K) and lora_b.shape == (n, N, R), (
+        f"lora_a must be [n, R, {K}] and lora_b [n, {N}, R], got {tuple(lora_a.shape)} and {tuple(lora_b.shape)}")
+    assert adapter.shape == x.shape[:1], "adapter holds one index per request (x's first dim)"
+    assert b is None or b.shape == (N,)
+    assert lora_scale is None or lora_scale.shape == (n,)
+    assert activation in ("", "GELU"), f"unknown activation {activation!r}"
+    _lib.require_cuda(x, w, b, lora_a, lora_b, adapter, lora_scale)
+    _lib.require_same_device(x, w, b, lora_a, lora_b, adapter, lora_scale)
+    for t in (x, w, lora_a, lora_b):
+        if t.dtype != torch.bfloat16:
+            raise UnsupportedDtype(t.dtype)
+    if adapter.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"adapter indices are int32 or int64, got {adapter.dtype}")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, lora_a, lora_b, lora_scale)):
+        raise NotImplementedError("linear_lora is forward only: call it under torch.no_grad() or detach its inputs")
+    B = x.shape[0]
+    y = torch.empty((*x.shape[:-1], N), device=x.device, dtype=x.dtype)
+    if y.numel() == 0:
+        return y
+    x2d = _as_2d(x, K)
+    M = x2d.shape[0]
+    if w.stride(1) != 1 or w.stride(0) % 8 or w.data_ptr() % 16:
+        w = _dense16(w)
+    if b is not None:
+        b = _dense16(b.to(torch.bfloat16))
+    lora_a, lora_b = _dense16(lora_a), _dense16(lora_b)
+    if lora_scale is not None:
+        lora_scale = lora_scale.to(torch.float32).contiguous()
+    adapter = adapter.contiguous()
+    lib = _lib.load()
+    scratch = torch.empty(lib.fluxb_linear_lora_scratch_bytes(M, N, K, R), device=x.device, dtype=torch.uint8)
+    with _lib.on_device_of(x):
+        _lib.check(
+            lib.fluxb_linear_lora(
+                x2d.data_ptr(), w.data_ptr(), _lib.ptr(b), y.data_ptr(), lora_a.data_ptr(), lora_b.data_ptr(),
+                _lib.ptr(lora_scale), adapter.data_ptr(), int(adapter.dtype == torch.int64), scratch.data_ptr(), B, M // B, N,
+                K, R, n, x2d.stride(0), w.stride(0), N, _lib.EPI_GELU if activation else _lib.EPI_NONE, _lib.stream_handle(),
+            )
+        )
+    return y

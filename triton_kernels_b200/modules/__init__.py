@@ -4,15 +4,16 @@ from triton_kernels_b200.modules.blocks import (
     DoubleStreamBlock,
     Linear,
     LinearGELU,
+    LinearLoRA,
     Modulation,
     ModulationOut,
     SelfAttention,
     SingleStreamBlock,
     attention,
 )
-from triton_kernels_b200.modules.normalization import QKNorm, RMSNorm
+from triton_kernels_b200.modules.normalization import LayerNorm, QKNorm, RMSNorm
 
 __all__ = [
     "MLP", "DoubleStreamBlock", "Linear", "LinearGELU", "Modulation", "ModulationOut", "SelfAttention",
-    "SingleStreamBlock", "attention", "QKNorm", "RMSNorm",
+    "SingleStreamBlock", "attention", "QKNorm", "RMSNorm", "LayerNorm", "LinearLoRA",
 ]

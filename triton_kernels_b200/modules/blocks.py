@@ -38,6 +38,7 @@ from triton_kernels_b200.kernels.linear import (
     linear,
     linear_grouped_into,
     linear_into,
+    linear_lora,
     linear_qkv_grouped_into,
     qkv_projection_scatter_supported,
     qkv_projection_supported,
@@ -72,6 +73,24 @@ class Linear(nn.Linear):
 class LinearGELU(nn.Linear):
     def forward(self, input: Tensor) -> Tensor:
         return linear(input, self.weight, self.bias, activation="GELU")
+
+
+class LinearLoRA(Linear):
+    """Linear with `num_adapters` low-rank adapters of one rank; each request of a batch names its
+    own.  The adapters are buffers (`lora_a` [n, R, in], `lora_b` [n, out, R], fp32 `lora_scale` [n]):
+    they are served, not trained, here.  B starts at zero, as a fresh adapter does."""
+
+    def __init__(self, in_features: int, out_features: int, num_adapters: int, rank: int, bias: bool = True):
+        super().__init__(in_features, out_features, bias=bias)
+        self.register_buffer("lora_a", torch.randn(num_adapters, rank, in_features) * in_features**-0.5)
+        self.register_buffer("lora_b", torch.zeros(num_adapters, out_features, rank))
+        self.register_buffer("lora_scale", torch.ones(num_adapters))
+
+    def forward(self, input: Tensor, adapter: Tensor | None = None) -> Tensor:
+        """`adapter` [B] int32 or int64, -1 for none; without it the shared projection alone."""
+        if adapter is None:
+            return super().forward(input)
+        return linear_lora(input, self.weight, self.bias, self.lora_a, self.lora_b, adapter, self.lora_scale)
 
 
 def MLP(hidden_size: int, mlp_hidden_dim: int, bias: bool = True) -> nn.Sequential:

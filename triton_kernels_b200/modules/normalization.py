@@ -1,10 +1,10 @@
-"""RMSNorm / QKNorm modules (reference: triton_kernels/modules/normalization.py:8-26)."""
+"""RMSNorm / QKNorm modules (reference: triton_kernels/modules/normalization.py:8-26) and LayerNorm."""
 from __future__ import annotations
 
 import torch
 from torch import Tensor, nn
 
-from triton_kernels_b200.kernels.normalization import rms_norm
+from triton_kernels_b200.kernels.normalization import layer_norm, rms_norm
 
 
 class RMSNorm(nn.Module):
@@ -16,6 +16,15 @@ class RMSNorm(nn.Module):
 
     def forward(self, x: Tensor) -> Tensor:
         return rms_norm(x, self.scale)
+
+
+class LayerNorm(nn.LayerNorm):
+    """nn.LayerNorm over the last dim (same parameters and state-dict keys) on `layer_norm`."""
+
+    def forward(self, input: Tensor) -> Tensor:
+        assert len(self.normalized_shape) == 1, "LayerNorm runs over the last dim only"
+        assert input.shape[-1:] == torch.Size(self.normalized_shape)
+        return layer_norm(input, self.weight, self.bias, self.eps)
 
 
 class QKNorm(nn.Module):
