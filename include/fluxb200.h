@@ -349,8 +349,8 @@ int fluxb_rope_axes(const void* q, void* oq, const int64_t* q_strides, const int
  * A shared projection plus one low-rank adapter per request:
  *   y[m] = act(x[m] w^T + bias + scale[a] (x[m] A_a^T) B_a^T),  a = adapter[m / L],  m < B*L
  * bf16, fp32 accumulation; epi FLUXB_EPI_NONE or FLUXB_EPI_GELU.  x [B*L, K] (ldx), w [N, K] (ldw),
- * y [B*L, N] (ldy), lora_a [n_adapters, R, K], lora_b [n_adapters, N, R] contiguous, lora_scale
- * fp32 [n_adapters] or NULL (ones), adapter int32 or int64 [B] on the device.  adapter -1: the
+ * y [B*L, N] (ldy), lora_a [n_adapters, R, K] contiguous, lora_b [n_adapters, N, R] with rows ldb
+ * apart and adapters N*ldb apart, R <= 256, lora_scale fp32 [n_adapters] or NULL (ones), adapter int32 or int64 [B] on the device.  adapter -1: the
  * request has none; any other value outside [0, n_adapters) counts as -1 and sets the device
  * status word (FLUXB_ERR_BAD_ARG, site 81).  K, N and the row strides are multiples of 8, pointers
  * 16-byte aligned.  scratch: fluxb_linear_lora_scratch_bytes() bytes.
@@ -359,7 +359,7 @@ int64_t fluxb_linear_lora_scratch_bytes(int64_t M, int64_t N, int64_t K, int64_t
 int fluxb_linear_lora(const void* x, const void* w, const void* bias, void* y, const void* lora_a, const void* lora_b,
                       const float* lora_scale, const void* adapter, int adapter_is64, void* scratch, int64_t B,
                       int64_t L, int64_t N, int64_t K, int64_t R, int64_t n_adapters, int64_t ldx, int64_t ldw,
-                      int64_t ldy, int epi, fluxb_stream_t stream);
+                      int64_t ldy, int64_t ldb, int epi, fluxb_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------
  * Sequence-parallel (Ulysses) exchange over peer memory.  The reference has no multi-GPU path,

@@ -47,18 +47,18 @@ def test_rope_axes(lib):
         assert rope(lib, **bad) == _lib.ERR_UNSUPPORTED, bad
 
 
-def lora(lib, B=2, L=3, N=64, K=64, R=8, n=2, ldx=None, ldw=None, ldy=None, x=P, adapter=P, scratch=P, epi=0, a=P):
-    return lib.fluxb_linear_lora(x, P, P, P, a, P, None, adapter, 1, scratch, B, L, N, K, R, n, ldx or K, ldw or K, ldy or N, epi, None)
+def lora(lib, B=2, L=3, N=64, K=64, R=8, n=2, ldx=None, ldw=None, ldy=None, ldb=None, x=P, adapter=P, scratch=P, epi=0, a=P):
+    return lib.fluxb_linear_lora(x, P, P, P, a, P, None, adapter, 1, scratch, B, L, N, K, R, n, ldx or K, ldw or K, ldy or N, ldb or R, epi, None)
 
 
 def test_linear_lora(lib):
     from triton_kernels_b200 import _lib
 
     assert lora(lib, B=0) == lora(lib, L=0) == lora(lib, N=0) == 0
-    for bad in (dict(K=0), dict(R=0), dict(n=0), dict(B=-1), dict(K=60), dict(N=60), dict(ldx=60), dict(ldw=56), dict(ldy=56), dict(x=None),
+    for bad in (dict(K=0), dict(R=0), dict(n=0), dict(B=-1), dict(K=60), dict(N=60), dict(ldx=60), dict(ldw=56), dict(ldy=56), dict(ldb=4), dict(R=4), dict(x=None),
                 dict(adapter=None), dict(scratch=None), dict(x=P + 2), dict(a=P + 8)):
         assert lora(lib, **bad) == _lib.ERR_BAD_ARG, bad
-    for bad in (dict(epi=2), dict(R=2048), dict(B=1 << 20, L=1 << 20)):
+    for bad in (dict(epi=2), dict(R=264), dict(B=1 << 20, L=1 << 20)):
         assert lora(lib, **bad) == _lib.ERR_UNSUPPORTED, bad
 
 

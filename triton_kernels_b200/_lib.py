@@ -70,7 +70,7 @@ SIGNATURES = {
     "fluxb_layer_norm_bwd": (_I, [_P] * 9 + [_L] * 7 + [_F, _I, _I, _P]),
     "fluxb_rope_axes": (_I, [_P, _P, _P, _P, _L, _P, _P, _P, _P, _L, _P, _I, _P, _L, _L, _L, _P, _I, c_double, _I, _I, _P]),
     "fluxb_linear_lora_scratch_bytes": (_L, [_L] * 4),
-    "fluxb_linear_lora": (_I, [_P] * 8 + [_I, _P] + [_L] * 9 + [_I, _P]),
+    "fluxb_linear_lora": (_I, [_P] * 8 + [_I, _P] + [_L] * 10 + [_I, _P]),
     "fluxb_peer_header_bytes": (_I, []),
     "fluxb_peer_alloc": (_I, [_L, POINTER(c_void_p)]),
     "fluxb_peer_free": (_I, [_P]),

@@ -177,6 +177,16 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* m, uin
       : "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* m, uint64_t* bar, int c0,
+                                            int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+      "%4, %5}], [%2];"
+      :
+      : "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1),
+        "r"(c2)
+      : "memory");
+}
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* m, uint64_t* bar, int c0,
                                             int c1, int c2, int c3) {
   asm volatile(
@@ -216,14 +226,15 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
 // apart): SBO = 1024, LBO unused.  MN-major 128B-swizzled tile stored as [k][64 mn-elements]
 // rows of 128 bytes: SBO = distance between 8-k groups, LBO = distance between 64-element
 // column blocks along MN.
+// Tiles of 64- or 32-byte rows take the swizzle of their row's size (layout 4 or 6), SBO = 8 rows.
 __device__ __forceinline__ uint64_t make_smem_desc(uint32_t saddr, uint32_t lbo_bytes,
-                                                   uint32_t sbo_bytes) {
+                                                   uint32_t sbo_bytes, uint32_t layout = 2) {
   uint64_t d = 0;
   d |= static_cast<uint64_t>((saddr & 0x3ffffu) >> 4);
   d |= static_cast<uint64_t>((lbo_bytes >> 4) & 0x3fffu) << 16;
   d |= static_cast<uint64_t>((sbo_bytes >> 4) & 0x3fffu) << 32;
   d |= 1ull << 46;
-  d |= 2ull << 61;
+  d |= static_cast<uint64_t>(layout) << 61;
   return d;
 }
 
@@ -343,6 +354,17 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
       : "memory");
 }
 
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* m,
+                                                 uint32_t bar_cluster_addr, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4, %5}], [%2];"
+      :
+      : "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar_cluster_addr), "r"(c0),
+        "r"(c1), "r"(c2)
+      : "memory");
+}
+
 // cta_group::2 forms: one thread of the leader CTA issues an MMA that runs on both SMs of the
 // pair (M = 256: 128 rows per CTA; each CTA supplies half of B).
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_result, uint32_t ncols) {
@@ -370,7 +392,22 @@ __device__ __forceinline__ void umma_ss_pair(uint32_t d_tmem, uint64_t adesc, ui
       : "r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// Same, but the arrival is delivered to the barrier at this offset in BOTH CTAs of the pair.
+// The accumulating form with a lane mask: a set bit leaves that row of D as it is (words 0-3 the
+// leader CTA's 128 rows, words 4-7 its partner's).
+__device__ __forceinline__ void umma_ss_pair_masked(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                                    const uint32_t (&off)[8]) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, 1, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, p;\n\t"
+      "}\n"
+      :
+      : "r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]),
+        "r"(off[4]), "r"(off[5]), "r"(off[6]), "r"(off[7])
+      : "memory");
+}
+// umma_commit whose arrival is delivered to the barrier at this offset in BOTH CTAs of the pair.
 __device__ __forceinline__ void umma_commit_pair_both(uint64_t* bar) {
   const uint16_t mask = 3;
   asm volatile(
@@ -453,6 +490,7 @@ int sm_count();
 // Encodes a tiled bf16 tensor map with 128-byte swizzle.  dims/strides innermost first;
 // strides in bytes for dims 1..rank-1.  Returns 0 or a negative FLUXB_ERR_* code.
 int encode_tmap_bf16(CUtensorMap* out, const void* base, int rank, const uint64_t* dims,
-                     const uint64_t* strides_bytes, const uint32_t* box);
+                     const uint64_t* strides_bytes, const uint32_t* box,
+                     CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
 
 }  // namespace fluxb

@@ -23,7 +23,7 @@
 #include <stdio.h>
 #include <stdlib.h>
 
-#include "common.cuh"
+#include "lora.cuh"
 
 namespace fluxb {
 
@@ -332,13 +332,58 @@ struct Grouped {
 
 static_assert(sizeof(Grouped) <= 4096, "kernel parameters are limited to 4 KB");
 
-__device__ __forceinline__ int find_problem(const Grouped& g, int tile) {
+// One problem whose requests add low-rank adapters (kMode 3).
+struct LoraGrouped {
+  Problem prob[1];
+  int count;
+  int total_tiles;
+  int pair_stages;
+  CUtensorMap tm_t, tm_b;  // t [M, units*32] box 32 x 128 (64-byte rows), B [n, N, R] box 16 x 128 (32-byte rows)
+  RequestAdapters req;
+  int units;               // ranks in sixteens
+};
+
+template <typename G>
+__device__ __forceinline__ int find_problem(const G& g, int tile) {
   int i = 0;
 #pragma unroll
-  for (int k = 1; k < MAX_PROBLEMS; ++k)
+  for (int k = 1; k < (int)(sizeof(g.prob) / sizeof(Problem)); ++k)
     if (k < g.count && tile >= g.prob[k].tile_start) i = k;
   return i;
 }
+
+// The adapters of a tile's 256 rows, one warp: lane l holds rows l, 32 + l, ...  next() takes the adapter of the
+// first row that is left, and the mask of the rows that do NOT use it (bit set: row left alone).
+struct TileAdapters {
+  int a[8];
+  __device__ __forceinline__ void load(const RequestAdapters& req, int row0, int rows, int lane) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = row0 + i * 32 + lane;
+      a[i] = row < rows ? req.of_row(row) : -1;
+    }
+  }
+  __device__ __forceinline__ int next(uint32_t (&off)[8]) {
+    int cur = -1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t left = __ballot_sync(0xffffffffu, a[i] >= 0);
+      const int first = __shfl_sync(0xffffffffu, a[i], left != 0 ? __ffs(left) - 1 : 0);
+      if (cur < 0 && left != 0) cur = first;
+    }
+    if (cur < 0) return cur;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      off[i] = ~__ballot_sync(0xffffffffu, a[i] == cur);
+      if (a[i] == cur) a[i] = -1;
+    }
+    return cur;
+  }
+};
+constexpr int LORA_T_BYTES = BM * 64;    // one unit of t: 128 rows of 16 high + 16 low parts
+constexpr int LORA_B_BYTES = BNH * 32;   // one unit of B: 128 rows of 16 ranks
+constexpr int LORA_UNITS = 2;            // units per ring slot
+static_assert(LORA_UNITS * LORA_T_BYTES <= A_BYTES && LORA_UNITS * LORA_B_BYTES <= B_BYTES, "an adapter step fits a ring slot");
 
 // Epilogue of one 128-row x 256-column tile (two heads of q, of k or of v) for EPI_QKV_HEADS:
 // bias, rounding to bf16 (the projection's output precision in the reference), per-head RMS norm
@@ -498,9 +543,15 @@ __device__ __forceinline__ void qkv_tile_epilogue(const Params& p, const CUtenso
 // forms' code or register pressure:
 //   0  ordinary (bias / GELU / gate+residual / column split)
 //   1  q|k|v columns through the head epilogue, columns from `split` on ordinary
-template <int kMode>
+//   3  ordinary epilogue; behind the K loop of a tile the requests' adapters are added.  The low-rank
+//      rows t = scale (x A^T), [M, R] in two bf16 parts (lora.cu), are K columns like any other: for
+//      every adapter that the tile's rows use, the MMAs t_high B^T and t_low B^T accumulate into the
+//      same TMEM tile through the same ring, with a lane mask that leaves the other requests' rows
+//      alone (so a request never meets another one's adapter, not even as a product with zero).
+//      Cost: R / 32 ring slots per adapter of a tile, next to K / 64.
+template <int kMode, typename G = Grouped>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
-gemm_pair_kernel(const __grid_constant__ Grouped g) {
+gemm_pair_kernel(const __grid_constant__ G g) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -549,7 +600,60 @@ gemm_pair_kernel(const __grid_constant__ Grouped g) {
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp == 0) {
+  if (kMode == 3 && warp == 0) {
+    if constexpr (kMode == 3) {
+      // As below, with the whole warp walking the tiles: the adapters of a tile are found by ballots.
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const Problem& pr = g.prob[0];
+      const Params& p = pr.p;
+      const int num_kb = (p.K + BK - 1) / BK;
+      for (int tile = pair_id; ok && tile < num_tiles; tile += num_pairs) {
+        int m_blk, n_blk;
+        tile_coords(p, tile, pr.tiles_m, m_blk, n_blk);
+        const int row0 = m_blk * 2 * BM + (int)rank * BM;
+        const int col0 = n_blk * BN + (int)rank * BNH;
+        TileAdapters rows;
+        rows.load(g.req, m_blk * 2 * BM, p.M, lane);
+        for (int kb = 0; ok && kb < num_kb; ++kb) {
+          if (lane == 0) {
+            ok = mbar_wait_cluster(&empty_bar[stage], phase ^ 1, abort_flag, status, 41);
+            if (ok) {
+              if (leader) mbar_expect_tx(&full_bar[stage], 2 * STAGE_BYTES);
+              const uint32_t full_addr = map_to_cta(smem_u32(&full_bar[stage]), 0);
+              uint8_t* a_dst = smem + stage * STAGE_BYTES;
+              tma_load_2d_pair(a_dst, &pr.tm_a, full_addr, kb * BK, row0);
+              tma_load_2d_pair(a_dst + A_BYTES, &pr.tm_b, full_addr, kb * BK, col0);
+            }
+          }
+          if (++stage == g.pair_stages) { stage = 0; phase ^= 1; }
+        }
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        uint32_t off[8];
+        for (int cur; ok && (cur = rows.next(off)) >= 0;) {
+          for (int u = 0; u < g.units; u += LORA_UNITS) {
+            if (ok && lane == 0) {
+              const int n_units = min(LORA_UNITS, g.units - u);
+              ok = mbar_wait_cluster(&empty_bar[stage], phase ^ 1, abort_flag, status, 46);
+              if (ok) {
+                if (leader) mbar_expect_tx(&full_bar[stage], 2 * n_units * (LORA_T_BYTES + LORA_B_BYTES));
+                const uint32_t full_addr = map_to_cta(smem_u32(&full_bar[stage]), 0);
+                uint8_t* a_dst = smem + stage * STAGE_BYTES;
+                for (int i = 0; i < n_units; ++i) {
+                  tma_load_2d_pair(a_dst + i * LORA_T_BYTES, &g.tm_t, full_addr, (u + i) * 32, row0);
+                  tma_load_3d_pair(a_dst + A_BYTES + i * LORA_B_BYTES, &g.tm_b, full_addr, (u + i) * 16, col0, cur);
+                }
+              }
+            }
+            if (++stage == g.pair_stages) { stage = 0; phase ^= 1; }
+          }
+          ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 0) {
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
@@ -585,6 +689,12 @@ gemm_pair_kernel(const __grid_constant__ Grouped g) {
       int local = 0;
       for (int tile = pair_id; ok && tile < num_tiles; tile += num_pairs, ++local) {
         const int num_kb = (g.prob[find_problem(g, tile)].p.K + BK - 1) / BK;
+        TileAdapters rows;
+        if constexpr (kMode == 3) {
+          int m_blk, n_blk;
+          tile_coords(g.prob[0].p, tile, g.prob[0].tiles_m, m_blk, n_blk);
+          rows.load(g.req, m_blk * 2 * BM, g.prob[0].p.M, lane);
+        }
         const int acc = local & 1;
         const uint32_t acc_phase = (local >> 1) & 1;
         if (!__all_sync(0xffffffffu, mbar_wait_cluster(&acc_empty[acc], acc_phase ^ 1, abort_flag, status, 43))) { ok = false; break; }
@@ -603,6 +713,29 @@ gemm_pair_kernel(const __grid_constant__ Grouped g) {
             umma_commit_pair_both(&empty_bar[stage]);
           }
           if (++stage == g.pair_stages) { stage = 0; phase ^= 1; }
+        }
+        if constexpr (kMode == 3) {
+          uint32_t off[8];
+          for (int cur; ok && (cur = rows.next(off)) >= 0;) {
+            for (int u = 0; ok && u < g.units; u += LORA_UNITS) {
+              ok = __all_sync(0xffffffffu, mbar_wait_cluster(&full_bar[stage], phase, abort_flag, status, 47));
+              if (!ok) break;
+              tc_fence_after_sync();
+              const uint32_t a_addr = smem_u32(smem + stage * STAGE_BYTES);
+              const uint64_t adesc = make_smem_desc(a_addr, 16, 512, 4);
+              const uint64_t bdesc = make_smem_desc(a_addr + A_BYTES, 16, 256, 6);
+              const int n_units = min(LORA_UNITS, g.units - u);
+              if (elect_one()) {
+                for (int i = 0; i < n_units; ++i) {
+                  const uint64_t ad = adesc + i * (LORA_T_BYTES >> 4), bd = bdesc + i * (LORA_B_BYTES >> 4);
+                  umma_ss_pair_masked(d_tmem, ad, bd, idesc, off);      // high parts
+                  umma_ss_pair_masked(d_tmem, ad + 2, bd, idesc, off);  // low parts, 32 bytes further
+                }
+                umma_commit_pair_both(&empty_bar[stage]);
+              }
+              if (++stage == g.pair_stages) { stage = 0; phase ^= 1; }
+            }
+          }
         }
         if (ok && elect_one()) umma_commit_pair_both(&acc_full[acc]);
       }
@@ -642,7 +775,7 @@ gemm_pair_kernel(const __grid_constant__ Grouped g) {
       // The tile leaves in four 64-column pieces: registers -> swizzled staging tile in shared
       // memory -> one TMA store of full 128-byte lines.  (Storing 16 bytes per thread straight
       // to global memory, 32 different rows per warp instruction, cost 9 % of the GEMM.)
-      if (kMode >= 1 && !second) {
+      if ((kMode == 1 || kMode == 2) && !second) {
         const int hd = p.heads * 128;
         const int part = n0 / hd;
         const int head0 = (n0 - part * hd) / 128;
@@ -986,6 +1119,46 @@ extern "C" int fluxb_linear_qkv_grouped_scatter(const fluxb_linear_problem* prob
   const QkvScatter scat{group_bases, n_groups, k_off, v_off, o_sb, o_sh, o_sl};
   return linear_qkv_grouped_impl(problems, streams, count, B, H, D, L_total, K, nullptr, &scat, eps, N2, epi2,
                                  round_before_act, stream);
+}
+
+// The projection of fluxb_linear_lora for more rows than the row-streaming kernel takes; t as lora.cu leaves it.
+int fluxb::launch_lora_gemm(const fluxb_linear_problem& a, int64_t N, int64_t K, int epi, const void* t, const void* lora_b,
+                            int64_t R, int64_t ldb, const RequestAdapters& req, cudaStream_t st) {
+  using namespace fluxb::gemm2;
+  LoraGrouped g;
+  g.count = 1;
+  g.pair_stages = STAGES;
+  Problem& pr = g.prob[0];
+  int rc = prepare_problem(a, N, K, epi, N, FLUXB_EPI_NONE, 0, true, &pr.tm_a, &pr.tm_b, &pr.p);
+  if (rc != FLUXB_OK) return rc;
+  {
+    const uint64_t dims[2] = {(uint64_t)N, (uint64_t)a.M}, strides[1] = {(uint64_t)a.ldy * 2};
+    const uint32_t box[2] = {OUT_CHUNK_COLS, BM};
+    if ((rc = encode_tmap_bf16(&pr.tm_y, a.y, 2, dims, strides, box)) != FLUXB_OK) return rc;
+    pr.tm_y2 = pr.tm_y;
+  }
+  g.units = (int)((R + 15) / 16);
+  {
+    const uint64_t dims[2] = {(uint64_t)g.units * 32, (uint64_t)a.M}, strides[1] = {(uint64_t)g.units * 64};
+    const uint32_t box[2] = {32, BM};
+    if ((rc = encode_tmap_bf16(&g.tm_t, t, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B)) != FLUXB_OK) return rc;
+  }
+  {
+    const uint64_t dims[3] = {(uint64_t)R, (uint64_t)N, (uint64_t)req.n_adapters};
+    const uint64_t strides[2] = {(uint64_t)ldb * 2, (uint64_t)(N * ldb) * 2};
+    const uint32_t box[3] = {16, BNH, 1};
+    if ((rc = encode_tmap_bf16(&g.tm_b, lora_b, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_32B)) != FLUXB_OK) return rc;
+  }
+  g.req = req;
+  pr.tiles_m = (int)((a.M + 255) / 256);
+  pr.tile_start = 0;
+  g.total_tiles = pr.tiles_m * pr.p.tiles_n;
+  auto kern = gemm_pair_kernel<3, LoraGrouped>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+  if (e != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "linear_lora: cannot set shared memory size: %s", cudaGetErrorString(e));
+  const int pairs = g.total_tiles < sm_count() / 2 ? g.total_tiles : sm_count() / 2;
+  kern<<<2 * pairs, THREADS, SMEM_BYTES, st>>>(g);
+  return FLUXB_OK;
 }
 
 extern "C" int fluxb_linear(const void* x, const void* w, const void* bias, void* y, int64_t M,

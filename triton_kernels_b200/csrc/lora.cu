@@ -1,86 +1,232 @@
 // A projection shared by all requests plus one low-rank adapter per request:
 //   y[m] = act(x[m] W^T + bias + s_a (x[m] A_a^T) B_a^T),   a = adapter[m / L]   (a < 0: no adapter)
-// x holds L rows per request.  An adapter index outside [-1, n) leaves its request without an adapter and is
-// recorded in the device status word (site 81).
-#include "vec.cuh"
+// x holds L rows per request.  Two launches: the low-rank rows t = s_a (x A_a^T) here, then the projection with
+// the adapters' second half fused in (gemm_tcgen05.cu).  t is carried as two bf16 parts, high and low
+// (t = high + low to 2^-17 of |t|), so that the tensor cores take it without the rounding a single bf16 would put
+// between the two products.  An adapter index outside [-1, n) leaves its request without an adapter and is recorded
+// in the device status word (site 81).
+#include "lora.cuh"
 
 namespace fluxb {
 
-struct LoraArgs {
-  const __nv_bfloat16 *x, *w, *bias, *a, *b;
+namespace shrink {
+constexpr int BM = 128;
+constexpr int BK = 64;
+constexpr int THREADS = 192;
+constexpr int MAX_STAGES = 12;
+constexpr int MAX_SMEM = 200 * 1024;
+
+struct Params {
+  CUtensorMap tm_x;  // [M, K], box 64 x box_rows
+  CUtensorMap tm_a;  // [n, R, K], box 64 x rpad
+  RequestAdapters req;
   const float* scale;  // nullptr: ones
-  const void* adapter;
-  __nv_bfloat16* y;
-  float* t;  // [M, R]
-  int64_t M, L, ldx, ldw, ldy;
-  int N, K, R, n_adapters, adapter_is64, epi;
+  __nv_bfloat16* t;    // [M, units * 32]: per 16 ranks, 16 high parts then 16 low parts
+  int L, tiles_per_request, box_rows;
+  int num_kb, ksplit, rpad, stages, tmem_cols;
   DeviceStatus* status;
 };
 
-__device__ __forceinline__ int adapter_of(const LoraArgs& p, int64_t request) {
-  const int64_t a = p.adapter_is64 ? static_cast<const int64_t*>(p.adapter)[request]
-                                   : static_cast<const int32_t*>(p.adapter)[request];
-  if (a < -1 || a >= p.n_adapters) {
-    report_error(p.status, FLUXB_ERR_BAD_ARG, 81);
-    return -1;
-  }
-  return static_cast<int>(a);
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
 }
 
-// t[m, j] = s_a sum_k x[m, k] A_a[j, k]: one warp per (row, rank).
-__global__ void __launch_bounds__(256) lora_shrink_any_kernel(const LoraArgs p) {
-  const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (i >= p.M * p.R) return;
-  const int64_t m = i / p.R;
-  const int j = (int)(i % p.R);
-  const int a = adapter_of(p, m / p.L);
-  float s = 0.f;
-  if (a >= 0) {
-    const __nv_bfloat16* x = p.x + m * p.ldx;
-    const __nv_bfloat16* w = p.a + ((int64_t)a * p.R + j) * p.K;
-    for (int k = threadIdx.x & 31; k < p.K; k += 32) s = fmaf(__bfloat162float(x[k]), __bfloat162float(w[k]), s);
-    s = warp_sum(s) * (p.scale != nullptr ? p.scale[a] : 1.f);
+// One cluster of `ksplit` CTAs per 128 rows of one request: each CTA multiplies its share of K (x and A tiles by TMA,
+// fp32 accumulator in TMEM, N = the rank in sixteens), leaves its partial sums in shared memory, and after a cluster
+// barrier each takes a share of the outputs, adds the partial sums in a fixed order, scales, splits and stores.
+__global__ void __launch_bounds__(THREADS, 1) lora_shrink_kernel(const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], acc_full;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  volatile int* abort_flag = &abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_ctarank();
+  const int tile = blockIdx.x / p.ksplit;
+  const int request = tile / p.tiles_per_request;
+  const int l0 = (tile - request * p.tiles_per_request) * BM;
+  const int row0 = request * p.L + l0;
+  const int rows = min(BM, p.L - l0);
+  const int adapter = p.req.of_request(request);
+  if (adapter < 0) {  // the whole cluster leaves; nobody reads these rows of t
+    if (threadIdx.x == 0 && rank == 0 && l0 == 0 && p.req.raw(request) != -1) report_error(p.status, FLUXB_ERR_BAD_ARG, 81);
+    return;
   }
-  if ((threadIdx.x & 31) == 0) p.t[i] = s;
+  const int stage_bytes = BM * BK * 2 + p.rpad * BK * 2;
+  const int kb0 = rank * p.num_kb / p.ksplit, kb1 = (rank + 1) * p.num_kb / p.ksplit;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(&acc_full, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&p.tm_x);
+    tma_prefetch_desc(&p.tm_a);
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, p.tmem_cols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      const uint32_t bytes = (uint32_t)(p.box_rows + p.rpad) * BK * 2;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, 82)) break;
+        uint8_t* dst = smem + stage * stage_bytes;
+        mbar_expect_tx(&full_bar[stage], bytes);
+        // rows behind the request are loaded and never stored; rows of the tile that no box covers are never read out
+        tma_load_2d(dst, &p.tm_x, &full_bar[stage], kb * BK, row0);
+        tma_load_3d(dst + BM * BK * 2, &p.tm_a, &full_bar[stage], kb * BK, 0, adapter);
+        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    const uint32_t idesc = make_idesc_bf16(BM, p.rpad, 0, 0);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, abort_flag, p.status, 83));
+      if (!ok) break;
+      tc_fence_after_sync();
+      const uint32_t a_addr = smem_u32(smem + stage * stage_bytes);
+      const uint64_t adesc = make_smem_desc(a_addr, 16, 1024);
+      const uint64_t bdesc = make_smem_desc(a_addr + BM * BK * 2, 16, 1024);
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < BK / 16; ++k)
+          umma_ss(tmem_base, adesc + 2 * k, bdesc + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+        umma_commit(&empty_bar[stage]);
+      }
+      if (++stage == p.stages) { stage = 0; phase ^= 1; }
+    }
+    if (ok && elect_one()) umma_commit(&acc_full);
+    __syncwarp();
+  }
+  float* part = reinterpret_cast<float*>(smem);  // [rpad][128]: the ring's memory, free once the last MMA is done
+  bool ok = true;
+  if (warp >= 2) {
+    const int quad = warp & 3;
+    ok = mbar_wait(&acc_full, 0, abort_flag, p.status, 84);
+    ok = __all_sync(0xffffffffu, ok);
+    if (ok && quad * 32 < rows) {
+      tc_fence_after_sync();
+      const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
+      for (int c = 0; c < p.rpad; c += 16) {
+        uint32_t r[16];
+        tmem_ld_x16(t_addr + c, r);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) part[(c + e) * BM + quad * 32 + lane] = __uint_as_float(r[e]);
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, p.tmem_cols);
+  }
+  cluster_sync_all();
+  const float scale = p.scale != nullptr ? p.scale[adapter] : 1.f;
+  const int t_ld = p.rpad * 2;
+  for (int i = rank * THREADS + threadIdx.x; i < p.rpad / 8 * BM; i += p.ksplit * THREADS) {
+    const int row = i & (BM - 1), c8 = i / BM * 8;
+    if (row >= rows) continue;
+    float v[8] = {};
+    for (int s = 0; s < p.ksplit; ++s) {
+      const uint32_t src = map_to_cta(smem_u32(part + c8 * BM + row), (uint32_t)s);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += ld_cluster_f32(src + e * BM * 4);
+    }
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float a = v[2 * e] * scale, b = v[2 * e + 1] * scale;
+      hi[e] = pack_bf16(a, b);
+      // an infinite product has no low part (inf - inf would be NaN)
+      const float la = a - bf16_lo(hi[e]), lb = b - bf16_hi(hi[e]);
+      lo[e] = pack_bf16(isinf(bf16_lo(hi[e])) ? 0.f : la, isinf(bf16_hi(hi[e])) ? 0.f : lb);
+    }
+    __nv_bfloat16* dst = p.t + (int64_t)(row0 + row) * t_ld + c8 / 16 * 32 + (c8 & 8);
+    *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4*>(dst + 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  }
+  cluster_sync_all();  // no CTA leaves while another reads its partial sums
 }
 
-// 64 x 64 tiles, 4 x 4 outputs per thread, fp32 products.
-__global__ void __launch_bounds__(256) lora_gemm_any_kernel(const LoraArgs p) {
-  __shared__ float xs[16][65], ws[16][65];
-  const int n0 = blockIdx.x * 64;
-  const int64_t m0 = (int64_t)blockIdx.y * 64;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < p.K; k0 += 16) {
-    for (int i = threadIdx.x; i < 1024; i += 256) {
-      const int r = i >> 4, k = k0 + (i & 15);
-      xs[i & 15][r] = m0 + r < p.M && k < p.K ? __bfloat162float(p.x[(m0 + r) * p.ldx + k]) : 0.f;
-      ws[i & 15][r] = n0 + r < p.N && k < p.K ? __bfloat162float(p.w[(int64_t)(n0 + r) * p.ldw + k]) : 0.f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xs[k][ty + 16 * i], ws[k][tx + 16 * j], acc[i][j]);
-    __syncthreads();
+}  // namespace shrink
+
+static int launch_shrink(const void* x, int64_t ldx, const void* lora_a, const float* scale, void* t, const RequestAdapters& req,
+                         int64_t B, int64_t L, int64_t K, int64_t R, cudaStream_t st) {
+  using namespace shrink;
+  Params p;
+  p.req = req;
+  p.scale = scale;
+  p.t = static_cast<__nv_bfloat16*>(t);
+  p.L = (int)L;
+  p.tiles_per_request = (int)((L + BM - 1) / BM);
+  p.box_rows = (int)(L < BM ? (L + 7) / 8 * 8 : BM);
+  p.rpad = (int)((R + 15) / 16 * 16);
+  p.num_kb = (int)((K + BK - 1) / BK);
+  p.status = device_status_ptr();
+  const int64_t tiles = B * p.tiles_per_request;
+  // K is split until the clusters fill the machine, as long as a CTA keeps four 64-wide steps.
+  p.ksplit = 1;
+  while (p.ksplit < 8 && tiles * p.ksplit * 2 <= sm_count() && p.num_kb >= p.ksplit * 2 * 4) p.ksplit *= 2;
+  const int steps = (p.num_kb + p.ksplit - 1) / p.ksplit;
+  const int stage_bytes = BM * BK * 2 + p.rpad * BK * 2;
+  p.stages = MAX_SMEM / stage_bytes < MAX_STAGES ? MAX_SMEM / stage_bytes : MAX_STAGES;
+  if (p.stages > steps) p.stages = steps;
+  int smem = p.stages * stage_bytes;
+  if (smem < p.rpad * BM * 4) smem = p.rpad * BM * 4;
+  smem += 1024;
+  p.tmem_cols = 32;
+  while (p.tmem_cols < p.rpad) p.tmem_cols *= 2;
+  const int64_t M = B * L;
+  {
+    const uint64_t dims[2] = {(uint64_t)K, (uint64_t)M}, strides[1] = {(uint64_t)ldx * 2};
+    const uint32_t box[2] = {BK, (uint32_t)p.box_rows};
+    int rc = encode_tmap_bf16(&p.tm_x, x, 2, dims, strides, box);
+    if (rc != FLUXB_OK) return rc;
   }
-  for (int i = 0; i < 4; ++i) {
-    const int64_t m = m0 + ty + 16 * i;
-    if (m >= p.M) continue;
-    const int a = adapter_of(p, m / p.L);
-    for (int j = 0; j < 4; ++j) {
-      const int n = n0 + tx + 16 * j;
-      if (n >= p.N) continue;
-      float v = acc[i][j] + (p.bias != nullptr ? __bfloat162float(p.bias[n]) : 0.f);
-      if (a >= 0)
-        for (int r = 0; r < p.R; ++r)
-          v = fmaf(p.t[m * p.R + r], __bfloat162float(p.b[((int64_t)a * p.N + n) * p.R + r]), v);
-      if (p.epi == FLUXB_EPI_GELU) v = gelu_tanh(v);
-      p.y[m * p.ldy + n] = __float2bfloat16_rn(v);
-    }
+  {
+    const uint64_t dims[3] = {(uint64_t)K, (uint64_t)R, (uint64_t)req.n_adapters};
+    const uint64_t strides[2] = {(uint64_t)K * 2, (uint64_t)R * K * 2};
+    const uint32_t box[3] = {BK, (uint32_t)p.rpad, 1};
+    int rc = encode_tmap_bf16(&p.tm_a, lora_a, 3, dims, strides, box);
+    if (rc != FLUXB_OK) return rc;
   }
+  cudaError_t e = cudaFuncSetAttribute(lora_shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM + 1024);
+  if (e != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "linear_lora: cannot set shared memory size: %s", cudaGetErrorString(e));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * p.ksplit));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)p.ksplit;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, lora_shrink_kernel, p);
+  if (e != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "linear_lora: launch failed: %s", cudaGetErrorString(e));
+  return FLUXB_OK;
 }
 
 }  // namespace fluxb
@@ -89,33 +235,35 @@ using namespace fluxb;
 
 extern "C" int64_t fluxb_linear_lora_scratch_bytes(int64_t M, int64_t N, int64_t K, int64_t R) {
   (void)N; (void)K;
-  return M <= 0 || R <= 0 ? 0 : M * R * 4;
+  return M <= 0 || R <= 0 ? 0 : M * ((R + 15) / 16) * 64;
 }
 
 extern "C" int fluxb_linear_lora(const void* x, const void* w, const void* bias, void* y, const void* lora_a,
                                  const void* lora_b, const float* lora_scale, const void* adapter, int adapter_is64,
                                  void* scratch, int64_t B, int64_t L, int64_t N, int64_t K, int64_t R, int64_t n_adapters,
-                                 int64_t ldx, int64_t ldw, int64_t ldy, int epi, fluxb_stream_t stream) {
+                                 int64_t ldx, int64_t ldw, int64_t ldy, int64_t ldb, int epi, fluxb_stream_t stream) {
   auto off16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; };
   if (epi != FLUXB_EPI_NONE && epi != FLUXB_EPI_GELU) return set_error(FLUXB_ERR_UNSUPPORTED, "linear_lora: epilogue %d", epi);
   if (B < 0 || L < 0 || N < 0 || K <= 0 || R <= 0 || n_adapters <= 0) return set_error(FLUXB_ERR_BAD_ARG, "linear_lora: bad sizes");
-  if (K % 8 || N % 8 || ldx % 8 || ldw % 8 || ldy % 8 || ldx < K || ldw < K || ldy < N)
+  if (K % 8 || N % 8 || ldx % 8 || ldw % 8 || ldy % 8 || ldb % 8 || ldx < K || ldw < K || ldy < N || ldb < R)
     return set_error(FLUXB_ERR_BAD_ARG, "linear_lora: K, N and row strides must be multiples of 8 (and strides no shorter than rows)");
   if (B == 0 || L == 0 || N == 0) return FLUXB_OK;
-  const int64_t M = B * L;
-  if (M > INT32_MAX / 2 || N > INT32_MAX / 2 || K > INT32_MAX / 2 || R > 1024 || n_adapters > INT32_MAX / 2)
+  if (R > 256) return set_error(FLUXB_ERR_UNSUPPORTED, "linear_lora: rank %lld (at most 256)", (long long)R);
+  const int64_t limit = INT32_MAX / 2;
+  if (B > limit || L > limit || B * L > limit || N > limit || K > limit || n_adapters > limit)
     return set_error(FLUXB_ERR_UNSUPPORTED, "linear_lora: dimension too large");
   if (!x || !w || !y || !lora_a || !lora_b || !adapter || !scratch) return set_error(FLUXB_ERR_BAD_ARG, "linear_lora: null pointer");
   if (off16(x) || off16(w) || off16(bias) || off16(y) || off16(lora_a) || off16(lora_b) || off16(scratch))
     return set_error(FLUXB_ERR_BAD_ARG, "linear_lora: pointers must be 16-byte aligned");
-  typedef const __nv_bfloat16* P;
-  LoraArgs p{static_cast<P>(x), static_cast<P>(w), static_cast<P>(bias), static_cast<P>(lora_a), static_cast<P>(lora_b),
-             lora_scale, adapter, static_cast<__nv_bfloat16*>(y), static_cast<float*>(scratch), M, L, ldx, ldw, ldy,
-             (int)N, (int)K, (int)R, (int)n_adapters, adapter_is64, epi, device_status_ptr()};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if ((M + 63) / 64 > 65535 || (M * R + 7) / 8 > INT32_MAX) return set_error(FLUXB_ERR_UNSUPPORTED, "linear_lora: too many rows");
-  lora_shrink_any_kernel<<<(unsigned)((M * R + 7) / 8), 256, 0, st>>>(p);
-  lora_gemm_any_kernel<<<dim3((unsigned)((N + 63) / 64), (unsigned)((M + 63) / 64)), 256, 0, st>>>(p);
+  const RequestAdapters req{adapter, adapter_is64, (int)L, (int)n_adapters};
+  int rc = launch_shrink(x, ldx, lora_a, lora_scale, scratch, req, B, L, K, R, st);
+  if (rc != FLUXB_OK) return rc;
+  fluxb_linear_problem a = {};
+  a.x = x; a.w = w; a.bias = bias; a.y = y; a.M = B * L; a.ldx = ldx; a.ldw = ldw; a.ldy = ldy;
+  a.rows_per_batch = 1;
+  rc = launch_lora_gemm(a, N, K, epi, scratch, lora_b, R, ldb, req, st);
+  if (rc != FLUXB_OK) return rc;
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "linear_lora: launch failed: %s", cudaGetErrorString(e));
   return FLUXB_OK;

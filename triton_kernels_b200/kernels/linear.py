@@ -225,7 +225,8 @@ def linear_lora(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None, lora_a
     [N] or None as in `linear`; lora_a [n, R, K], lora_b [n, N, R] bf16; lora_scale [n] fp32 or None
     (ones); adapter [B] int32 or int64 on x's device, -1 for a request without an adapter.  The
     values of `adapter` are read on the device: one outside [-1, n) counts as -1 and is recorded in
-    the device status word (`_lib.device_status`).  activation: "" or "GELU" (tanh form)."""
+    the device status word (`_lib.device_status`).  R <= 256; an R that is not a multiple of 8 copies
+    lora_b on every call (keep it padded with zeros instead).  activation: "" or "GELU" (tanh form)."""
     assert x.dim() >= 2 and x.shape[-1] == w.shape[-1], "Incompatible dimensions"
     N, K = w.shape
     n, R = lora_a.shape[:2]
@@ -254,6 +255,8 @@ def linear_lora(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None, lora_a
         w = _dense16(w)
     if b is not None:
         b = _dense16(b.to(torch.bfloat16))
+    if R % 8:  # rows of B that no 16-byte piece fits are copied into wider ones
+        lora_b = torch.nn.functional.pad(lora_b, (0, -R % 8))
     lora_a, lora_b = _dense16(lora_a), _dense16(lora_b)
     if lora_scale is not None:
         lora_scale = lora_scale.to(torch.float32).contiguous()
@@ -265,7 +268,7 @@ def linear_lora(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None, lora_a
             lib.fluxb_linear_lora(
                 x2d.data_ptr(), w.data_ptr(), _lib.ptr(b), y.data_ptr(), lora_a.data_ptr(), lora_b.data_ptr(),
                 _lib.ptr(lora_scale), adapter.data_ptr(), int(adapter.dtype == torch.int64), scratch.data_ptr(), B, M // B, N,
-                K, R, n, x2d.stride(0), w.stride(0), N, _lib.EPI_GELU if activation else _lib.EPI_NONE, _lib.stream_handle(),
+                K, R, n, x2d.stride(0), w.stride(0), N, lora_b.shape[2], _lib.EPI_GELU if activation else _lib.EPI_NONE, _lib.stream_handle(),
             )
         )
     return y
