@@ -407,6 +407,19 @@ __device__ __forceinline__ void umma_ss_pair_masked(uint32_t d_tmem, uint64_t ad
         "r"(off[4]), "r"(off[5]), "r"(off[6]), "r"(off[7])
       : "memory");
 }
+// The one-CTA form: four words for its 128 rows.
+__device__ __forceinline__ void umma_ss_masked(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                               const uint32_t (&off)[4]) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, 1, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, p;\n\t"
+      "}\n"
+      :
+      : "r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
+      : "memory");
+}
 // umma_commit whose arrival is delivered to the barrier at this offset in BOTH CTAs of the pair.
 __device__ __forceinline__ void umma_commit_pair_both(uint64_t* bar) {
   const uint16_t mask = 3;

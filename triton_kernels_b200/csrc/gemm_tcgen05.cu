@@ -352,28 +352,29 @@ __device__ __forceinline__ int find_problem(const G& g, int tile) {
   return i;
 }
 
-// The adapters of a tile's 256 rows, one warp: lane l holds rows l, 32 + l, ...  next() takes the adapter of the
+// The adapters of a tile's W x 32 rows, one warp: lane l holds rows l, 32 + l, ...  next() takes the adapter of the
 // first row that is left, and the mask of the rows that do NOT use it (bit set: row left alone).
+template <int W>
 struct TileAdapters {
-  int a[8];
+  int a[W];
   __device__ __forceinline__ void load(const RequestAdapters& req, int row0, int rows, int lane) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < W; ++i) {
       const int row = row0 + i * 32 + lane;
       a[i] = row < rows ? req.of_row(row) : -1;
     }
   }
-  __device__ __forceinline__ int next(uint32_t (&off)[8]) {
+  __device__ __forceinline__ int next(uint32_t (&off)[W]) {
     int cur = -1;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < W; ++i) {
       const uint32_t left = __ballot_sync(0xffffffffu, a[i] >= 0);
       const int first = __shfl_sync(0xffffffffu, a[i], left != 0 ? __ffs(left) - 1 : 0);
       if (cur < 0 && left != 0) cur = first;
     }
     if (cur < 0) return cur;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < W; ++i) {
       off[i] = ~__ballot_sync(0xffffffffu, a[i] == cur);
       if (a[i] == cur) a[i] = -1;
     }
@@ -614,7 +615,7 @@ gemm_pair_kernel(const __grid_constant__ G g) {
         tile_coords(p, tile, pr.tiles_m, m_blk, n_blk);
         const int row0 = m_blk * 2 * BM + (int)rank * BM;
         const int col0 = n_blk * BN + (int)rank * BNH;
-        TileAdapters rows;
+        TileAdapters<8> rows;
         rows.load(g.req, m_blk * 2 * BM, p.M, lane);
         for (int kb = 0; ok && kb < num_kb; ++kb) {
           if (lane == 0) {
@@ -689,7 +690,7 @@ gemm_pair_kernel(const __grid_constant__ G g) {
       int local = 0;
       for (int tile = pair_id; ok && tile < num_tiles; tile += num_pairs, ++local) {
         const int num_kb = (g.prob[find_problem(g, tile)].p.K + BK - 1) / BK;
-        TileAdapters rows;
+        TileAdapters<8> rows;
         if constexpr (kMode == 3) {
           int m_blk, n_blk;
           tile_coords(g.prob[0].p, tile, g.prob[0].tiles_m, m_blk, n_blk);
@@ -831,6 +832,247 @@ gemm_pair_kernel(const __grid_constant__ G g) {
 }
 
 }  // namespace gemm2
+
+// ----------------------------------------------------------------------------------------
+// The adapter projection for few tiles: 128 x BN tiles, one CTA each, so that a problem of a few hundred rows spreads
+// over the machine instead of filling a handful of CTA pairs.  Same roles and ring as the kernels above; the tile's
+// low-rank rows t stay in shared memory while the adapters of its rows pass through the ring, 64 ranks of B a slot.
+// ----------------------------------------------------------------------------------------
+namespace gemm3 {
+using gemm::BK;
+using gemm::BM;
+using gemm::Params;
+using gemm::epilogue_chunk;
+using gemm2::TileAdapters;
+constexpr int THREADS = 192;
+constexpr int T_BYTES = BM * 64;  // one unit of t: 128 rows of 16 high + 16 low parts
+constexpr int MAX_STAGES = 16;
+constexpr int MAX_SMEM = 224 * 1024;
+
+struct Tiles {
+  CUtensorMap tm_a, tm_b, tm_t, tm_lb;
+  Params p;
+  RequestAdapters req;
+  int units, stages;
+  int a_rows;  // rows of x per box: fewer than 128 when there are fewer; the MMAs then read what lies behind them in
+               // shared memory as the other rows, whose results are never stored
+};
+
+template <int BN>
+__global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_constant__ Tiles g) {
+  const int A_BYTES = g.a_rows * BK * 2, STAGE_BYTES = A_BYTES + BN * BK * 2;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], acc_full[2], acc_empty[2], t_full, t_empty;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  uint8_t* t_smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* smem = t_smem + g.units * T_BYTES;
+  volatile int* abort_flag = &abort_word;
+  const Params& p = g.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int num_kb = (p.K + BK - 1) / BK;
+  const int groups = (g.units + 3) / 4;  // of 64 ranks
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < g.stages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&acc_full[a], 1);
+      mbar_init(&acc_empty[a], 128);
+    }
+    mbar_init(&t_full, 1);
+    mbar_init(&t_empty, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&g.tm_a);
+    tma_prefetch_desc(&g.tm_b);
+    tma_prefetch_desc(&g.tm_t);
+    tma_prefetch_desc(&g.tm_lb);
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, 2 * BN);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = tmem_slot;
+
+  if (warp == 0) {
+    int stage = 0;
+    uint32_t phase = 0, t_phase = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; ok && tile < p.num_tiles; tile += gridDim.x) {
+      const int row0 = tile % p.tiles_m * BM, col0 = tile / p.tiles_m * BN;
+      TileAdapters<4> rows;
+      rows.load(g.req, row0, p.M, lane);
+      if (lane == 0) {
+        for (int kb = 0; kb < num_kb; ++kb) {
+          ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, 91);
+          if (!ok) break;
+          uint8_t* dst = smem + stage * STAGE_BYTES;
+          mbar_expect_tx(&full_bar[stage], STAGE_BYTES);
+          tma_load_2d(dst, &g.tm_a, &full_bar[stage], kb * BK, row0);
+          tma_load_2d(dst + A_BYTES, &g.tm_b, &full_bar[stage], kb * BK, col0);
+          if (++stage == g.stages) { stage = 0; phase ^= 1; }
+        }
+      }
+      __syncwarp();
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+      stage = __shfl_sync(0xffffffffu, stage, 0);
+      phase = __shfl_sync(0xffffffffu, phase, 0);
+      uint32_t off[4];
+      bool first = true;
+      for (int cur; ok && (cur = rows.next(off)) >= 0;) {
+        if (lane == 0) {
+          if (first) {
+            ok = mbar_wait(&t_empty, t_phase ^ 1, abort_flag, p.status, 92);
+            if (ok) {
+              mbar_expect_tx(&t_full, g.units * T_BYTES);
+              for (int u = 0; u < g.units; ++u) tma_load_2d(t_smem + u * T_BYTES, &g.tm_t, &t_full, u * 32, row0);
+            }
+          }
+          for (int q = 0; ok && q < groups; ++q) {
+            ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, 93);
+            if (!ok) break;
+            mbar_expect_tx(&full_bar[stage], BN * BK * 2);
+            tma_load_3d(smem + stage * STAGE_BYTES + A_BYTES, &g.tm_lb, &full_bar[stage], q * 64, col0, cur);
+            if (++stage == g.stages) { stage = 0; phase ^= 1; }
+          }
+        }
+        if (first) t_phase ^= 1;
+        first = false;
+        __syncwarp();
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        stage = __shfl_sync(0xffffffffu, stage, 0);
+        phase = __shfl_sync(0xffffffffu, phase, 0);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = make_idesc_bf16(BM, BN, 0, 0);
+    int stage = 0;
+    uint32_t phase = 0, t_phase = 0;
+    bool ok = true;
+    int local = 0;
+    for (int tile = blockIdx.x; ok && tile < p.num_tiles; tile += gridDim.x, ++local) {
+      TileAdapters<4> rows;
+      rows.load(g.req, tile % p.tiles_m * BM, p.M, lane);
+      const int acc = local & 1;
+      const uint32_t acc_phase = (local >> 1) & 1;
+      ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[acc], acc_phase ^ 1, abort_flag, p.status, 94));
+      if (!ok) break;
+      tc_fence_after_sync();
+      const uint32_t d_tmem = tmem_base + acc * BN;
+      for (int kb = 0; kb < num_kb; ++kb) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, abort_flag, p.status, 95));
+        if (!ok) break;
+        tc_fence_after_sync();
+        const uint32_t a_addr = smem_u32(smem + stage * STAGE_BYTES);
+        const uint64_t adesc = make_smem_desc(a_addr, 16, 1024), bdesc = make_smem_desc(a_addr + A_BYTES, 16, 1024);
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k) umma_ss(d_tmem, adesc + 2 * k, bdesc + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
+          umma_commit(&empty_bar[stage]);
+        }
+        if (++stage == g.stages) { stage = 0; phase ^= 1; }
+      }
+      uint32_t off[4];
+      bool first = true;
+      for (int cur; ok && (cur = rows.next(off)) >= 0;) {
+        if (first) ok = __all_sync(0xffffffffu, mbar_wait(&t_full, t_phase, abort_flag, p.status, 96));
+        for (int q = 0; ok && q < groups; ++q) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, abort_flag, p.status, 97));
+          if (!ok) break;
+          tc_fence_after_sync();
+          const uint64_t adesc = make_smem_desc(smem_u32(t_smem + q * 4 * T_BYTES), 16, 512, 4);
+          const uint64_t bdesc = make_smem_desc(smem_u32(smem + stage * STAGE_BYTES) + A_BYTES, 16, 1024);
+          const int n_units = min(4, g.units - q * 4);
+          if (elect_one()) {
+            for (int i = 0; i < n_units; ++i) {
+              const uint64_t ad = adesc + i * (T_BYTES >> 4);
+              umma_ss_masked(d_tmem, ad, bdesc + 2 * i, idesc, off);      // high parts
+              umma_ss_masked(d_tmem, ad + 2, bdesc + 2 * i, idesc, off);  // low parts, 32 bytes further
+            }
+            umma_commit(&empty_bar[stage]);
+          }
+          if (++stage == g.stages) { stage = 0; phase ^= 1; }
+        }
+        if (first) t_phase ^= 1;
+        first = false;
+      }
+      if (ok && elect_one()) {
+        if (!first) umma_commit(&t_empty);
+        umma_commit(&acc_full[acc]);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int quad = warp & 3;
+    int local = 0;
+    for (int tile = blockIdx.x; tile < p.num_tiles; tile += gridDim.x, ++local) {
+      const int acc = local & 1;
+      const uint32_t acc_phase = (local >> 1) & 1;
+      if (!mbar_wait(&acc_full[acc], acc_phase, abort_flag, p.status, 98)) break;
+      __syncwarp();
+      tc_fence_after_sync();
+      const int row0 = tile % p.tiles_m * BM, n0 = tile / p.tiles_m * BN;
+      const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * BN;
+      if (row0 + quad * 32 < p.M) {
+#pragma unroll 1
+        for (int c = 0; c < BN / 32; ++c) {
+          if (n0 + c * 32 >= p.N) break;  // uniform
+          uint32_t r[32];
+          tmem_ld_x32(t_addr + c * 32, r);
+          tmem_wait_ld();
+          epilogue_chunk(p, r, row0 + quad * 32 + lane, n0 + c * 32, false);
+        }
+      }
+      tc_fence_before_sync();
+      mbar_arrive(&acc_empty[acc]);
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, 2 * BN);
+  }
+}
+
+template <int BN>
+static int launch_tiles(Tiles& g, const fluxb_linear_problem& a, int64_t N, int64_t K, const void* lora_b, int64_t R, int64_t ldb,
+                        cudaStream_t st) {
+  {
+    const uint64_t dims[2] = {(uint64_t)K, (uint64_t)N}, strides[1] = {(uint64_t)a.ldw * 2};
+    const uint32_t box[2] = {BK, BN};
+    int rc = encode_tmap_bf16(&g.tm_b, a.w, 2, dims, strides, box);
+    if (rc != FLUXB_OK) return rc;
+  }
+  {
+    const uint64_t dims[3] = {(uint64_t)R, (uint64_t)N, (uint64_t)g.req.n_adapters};
+    const uint64_t strides[2] = {(uint64_t)ldb * 2, (uint64_t)(N * ldb) * 2};
+    const uint32_t box[3] = {64, BN, 1};
+    int rc = encode_tmap_bf16(&g.tm_lb, lora_b, 3, dims, strides, box);
+    if (rc != FLUXB_OK) return rc;
+  }
+  const int stage_bytes = g.a_rows * BK * 2 + BN * BK * 2, behind = (BM - g.a_rows) * BK * 2;
+  g.stages = (MAX_SMEM - 1024 - 512 - g.units * T_BYTES - behind) / stage_bytes;
+  if (g.stages > MAX_STAGES) g.stages = MAX_STAGES;
+  g.p.tiles_n = (int)((N + BN - 1) / BN);
+  g.p.num_tiles = g.p.tiles_m * g.p.tiles_n;
+  auto kern = lora_tile_kernel<BN>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM);
+  if (e != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "linear_lora: cannot set shared memory size: %s", cudaGetErrorString(e));
+  const int grid = g.p.num_tiles < sm_count() ? g.p.num_tiles : sm_count();
+  kern<<<grid, THREADS, 1024 + g.units * T_BYTES + g.stages * stage_bytes + behind, st>>>(g);
+  return FLUXB_OK;
+}
+
+}  // namespace gemm3
 }  // namespace fluxb
 
 using namespace fluxb;
@@ -1122,8 +1364,40 @@ extern "C" int fluxb_linear_qkv_grouped_scatter(const fluxb_linear_problem* prob
 }
 
 // The projection of fluxb_linear_lora for more rows than the row-streaming kernel takes; t as lora.cu leaves it.
-int fluxb::launch_lora_gemm(const fluxb_linear_problem& a, int64_t N, int64_t K, int epi, const void* t, const void* lora_b,
+int fluxb::launch_lora_gemm(const fluxb_linear_problem& a, int64_t N, int64_t K, int epi, const void* low, const void* lora_b,
                             int64_t R, int64_t ldb, const RequestAdapters& req, cudaStream_t st) {
+  // Which tiles: cycles per 64-wide K step are 512 for a 256 x 256 tile of a CTA pair (its MMAs), and 64 bytes a cycle of
+  // operands for a 128 x BN tile of one CTA; on top of the K loop the last tile's epilogue shows, 20 000 cycles of the
+  // pair kernel's and about 40 per column of the other's.
+  const int64_t kb = (K + 63) / 64, sms = sm_count();
+  const int64_t pair_tiles = ((a.M + 255) / 256) * ((N + 255) / 256);
+  int64_t best = (pair_tiles + sms / 2 - 1) / (sms / 2) * 512 * kb + 20000;
+  const int64_t a_rows = a.M < 128 ? (a.M + 7) / 8 * 8 : 128;
+  int bn = 256;
+  for (int c = 128; c >= 32; c /= 2) {
+    const int64_t tiles = ((a.M + 127) / 128) * ((N + c - 1) / c);
+    const int64_t t = (tiles + sms - 1) / sms * ((a_rows + c) * 2 * kb + 40 * c);
+    if (t < best) { best = t; bn = c; }
+  }
+  if (bn < 256) {
+    fluxb::gemm3::Tiles t;
+    int rc = prepare_problem(a, N, K, epi, N, FLUXB_EPI_NONE, 0, false, &t.tm_a, &t.tm_b, &t.p);
+    if (rc != FLUXB_OK) return rc;
+    t.req = req;
+    t.units = (int)((R + 15) / 16);
+    t.a_rows = (int)a_rows;
+    {
+      const uint64_t dims[2] = {(uint64_t)K, (uint64_t)a.M}, strides[1] = {(uint64_t)a.ldx * 2};
+      const uint32_t box[2] = {64, (uint32_t)a_rows};
+      if ((rc = encode_tmap_bf16(&t.tm_a, a.x, 2, dims, strides, box)) != FLUXB_OK) return rc;
+    }
+    const uint64_t dims[2] = {(uint64_t)t.units * 32, (uint64_t)a.M}, strides[1] = {(uint64_t)t.units * 64};
+    const uint32_t box[2] = {32, fluxb::gemm::BM};
+    if ((rc = encode_tmap_bf16(&t.tm_t, low, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B)) != FLUXB_OK) return rc;
+    if (bn == 128) return fluxb::gemm3::launch_tiles<128>(t, a, N, K, lora_b, R, ldb, st);
+    if (bn == 64) return fluxb::gemm3::launch_tiles<64>(t, a, N, K, lora_b, R, ldb, st);
+    return fluxb::gemm3::launch_tiles<32>(t, a, N, K, lora_b, R, ldb, st);
+  }
   using namespace fluxb::gemm2;
   LoraGrouped g;
   g.count = 1;
@@ -1141,7 +1415,7 @@ int fluxb::launch_lora_gemm(const fluxb_linear_problem& a, int64_t N, int64_t K,
   {
     const uint64_t dims[2] = {(uint64_t)g.units * 32, (uint64_t)a.M}, strides[1] = {(uint64_t)g.units * 64};
     const uint32_t box[2] = {32, BM};
-    if ((rc = encode_tmap_bf16(&g.tm_t, t, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B)) != FLUXB_OK) return rc;
+    if ((rc = encode_tmap_bf16(&g.tm_t, low, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B)) != FLUXB_OK) return rc;
   }
   {
     const uint64_t dims[3] = {(uint64_t)R, (uint64_t)N, (uint64_t)req.n_adapters};

@@ -229,6 +229,148 @@ static int launch_shrink(const void* x, int64_t ldx, const void* lora_a, const f
   return FLUXB_OK;
 }
 
+// ----------------------------------------------------------------------------------------
+// One to eight rows: the projection is a stream of W.  A block takes 16 output columns, its warps share K; a warp's
+// lane loads 16 bytes of two W rows and uses them as the A fragments of mma.m16n8k16 (W's columns are the M side, the
+// rows of x the N side), with x's fragment loaded from the same k positions: the order of k does not matter as long as
+// both sides agree, so no shuffle or shared memory stands between the load and the product.  All 24 loads of a step
+// are in flight at once, and those of the next step leave before the current one is summed over the warps.  The
+// adapters are 2 R more products per output, from the high and low parts of t, in the epilogue.
+// ----------------------------------------------------------------------------------------
+namespace rows {
+constexpr int SLICE = 384;  // k per warp and step: 12 fragments of 32
+constexpr int STEPS = SLICE / 32;
+constexpr int MAX_WARPS = 8;
+
+struct Params {
+  const __nv_bfloat16 *x, *w, *bias, *t, *lora_b;
+  __nv_bfloat16* y;
+  RequestAdapters req;
+  int64_t ldx, ldw, ldy, ldb;
+  int M, N, K, R, rpad, epi, tiles, slices;  // slices: steps of a warp per tile
+};
+
+__device__ __forceinline__ uint4 ld_or_zero(const __nv_bfloat16* p, bool ok) {
+  return ok ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+}
+__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                            uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// sum of t[j] * b[j] over eight ranks; t as high and low parts
+__device__ __forceinline__ float dot8(const uint4& b, const float* t, float acc) {
+  const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) acc = fmaf(bf16_hi(w[e]), t[2 * e + 1], fmaf(bf16_lo(w[e]), t[2 * e], acc));
+  return acc;
+}
+
+// kOne: a warp's share of K is one step, and its fragments of x stay in registers for all tiles.
+template <bool kOne>
+__global__ void __launch_bounds__(MAX_WARPS * 32, 1) lora_rows_kernel(const Params p) {
+  __shared__ float red[2][MAX_WARPS][16][9];
+  __shared__ float t_s[8][256];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int g = lane >> 2, t4 = lane & 3;
+  const __nv_bfloat16* xr = p.x + g * p.ldx;
+  uint4 bx[STEPS], a0[STEPS], a1[STEPS];
+  auto load_x = [&](int slice) {
+    const int k0 = (slice * warps + warp) * SLICE + t4 * 8;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) bx[s] = ld_or_zero(xr + k0 + s * 32, g < p.M && k0 + s * 32 < p.K);
+  };
+  auto load_w = [&](int tile, int slice) {
+    const int k0 = (slice * warps + warp) * SLICE + t4 * 8;
+    const int n = tile * 16 + g;
+    const __nv_bfloat16* w0 = p.w + n * p.ldw + k0;
+    const __nv_bfloat16* w1 = w0 + 8 * p.ldw;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const bool in = k0 + s * 32 < p.K;
+      a0[s] = ld_or_zero(w0 + s * 32, in && n < p.N);
+      a1[s] = ld_or_zero(w1 + s * 32, in && n + 8 < p.N);
+    }
+  };
+  if (kOne) load_x(0);
+  int tile = blockIdx.x;
+  load_w(tile, 0);
+  // t of the requests that have an adapter, widened
+  for (int i = threadIdx.x; i < p.M * p.rpad; i += blockDim.x) {
+    const int m = i / p.rpad, j = i - m * p.rpad;
+    float v = 0.f;
+    if (p.req.of_row(m) >= 0) {
+      const __nv_bfloat16* src = p.t + (int64_t)m * p.rpad * 2 + j / 16 * 32 + j % 16;
+      v = __bfloat162float(src[0]) + __bfloat162float(src[16]);
+    }
+    t_s[m][j] = v;
+  }
+  int buf = 0;
+  for (; tile < p.tiles; tile += gridDim.x) {
+    float c[4] = {};
+    for (int slice = 0; slice < (kOne ? 1 : p.slices); ++slice) {
+      if (!kOne) load_x(slice);
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        mma_16x8x16(c, a0[s].x, a1[s].x, a0[s].y, a1[s].y, bx[s].x, bx[s].y);
+        mma_16x8x16(c, a0[s].z, a1[s].z, a0[s].w, a1[s].w, bx[s].z, bx[s].w);
+      }
+      if (!kOne && slice + 1 < p.slices) load_w(tile, slice + 1);
+      else if (tile + (int)gridDim.x < p.tiles) load_w(tile + gridDim.x, 0);
+    }
+    red[buf][warp][g][2 * t4] = c[0];
+    red[buf][warp][g][2 * t4 + 1] = c[1];
+    red[buf][warp][g + 8][2 * t4] = c[2];
+    red[buf][warp][g + 8][2 * t4 + 1] = c[3];
+    __syncthreads();  // the other buffer's readers are through before anyone gets here again
+    for (int i = threadIdx.x; i < 128; i += blockDim.x) {
+      const int m = i >> 4, n = tile * 16 + (i & 15);
+      if (m >= p.M || n >= p.N) continue;
+      float v = p.bias != nullptr ? __bfloat162float(p.bias[n]) : 0.f;
+      for (int w = 0; w < warps; ++w) v += red[buf][w][i & 15][m];
+      const int a = p.req.of_row(m);
+      if (a >= 0) {
+        const __nv_bfloat16* b = p.lora_b + ((int64_t)a * p.N + n) * p.ldb;
+        float s = 0.f;
+        int j = 0;
+        for (; j + 8 <= p.R; j += 8) s = dot8(__ldg(reinterpret_cast<const uint4*>(b + j)), &t_s[m][j], s);
+        for (; j < p.R; ++j) s = fmaf(__bfloat162float(b[j]), t_s[m][j], s);
+        v += s;
+      }
+      if (p.epi == FLUXB_EPI_GELU) v = gelu_tanh(v);
+      p.y[m * p.ldy + n] = __float2bfloat16_rn(v);
+    }
+    buf ^= 1;
+  }
+}
+
+}  // namespace rows
+
+static int launch_rows(const fluxb_linear_problem& a, int64_t N, int64_t K, int epi, const void* t, const void* lora_b,
+                       int64_t R, int64_t ldb, const RequestAdapters& req, cudaStream_t st) {
+  rows::Params p;
+  typedef const __nv_bfloat16* P;
+  p.x = static_cast<P>(a.x); p.w = static_cast<P>(a.w); p.bias = static_cast<P>(a.bias); p.t = static_cast<P>(t);
+  p.lora_b = static_cast<P>(lora_b);
+  p.y = static_cast<__nv_bfloat16*>(a.y);
+  p.req = req;
+  p.ldx = a.ldx; p.ldw = a.ldw; p.ldy = a.ldy; p.ldb = ldb;
+  p.M = (int)a.M; p.N = (int)N; p.K = (int)K; p.R = (int)R; p.rpad = (int)((R + 15) / 16 * 16); p.epi = epi;
+  p.tiles = (int)((N + 15) / 16);
+  int warps = (int)((K + rows::SLICE - 1) / rows::SLICE);
+  if (warps > rows::MAX_WARPS) warps = rows::MAX_WARPS;
+  p.slices = (int)((K + rows::SLICE * warps - 1) / (rows::SLICE * warps));
+  // every block the same number of tiles, eight warps per SM
+  const int most = sm_count() * (rows::MAX_WARPS / warps);
+  const int per = (p.tiles + most - 1) / most;
+  const int grid = (p.tiles + per - 1) / per;
+  if (p.slices == 1) rows::lora_rows_kernel<true><<<grid, warps * 32, 0, st>>>(p);
+  else rows::lora_rows_kernel<false><<<grid, warps * 32, 0, st>>>(p);
+  return FLUXB_OK;
+}
+
 }  // namespace fluxb
 
 using namespace fluxb;
@@ -262,7 +404,8 @@ extern "C" int fluxb_linear_lora(const void* x, const void* w, const void* bias,
   fluxb_linear_problem a = {};
   a.x = x; a.w = w; a.bias = bias; a.y = y; a.M = B * L; a.ldx = ldx; a.ldw = ldw; a.ldy = ldy;
   a.rows_per_batch = 1;
-  rc = launch_lora_gemm(a, N, K, epi, scratch, lora_b, R, ldb, req, st);
+  rc = a.M <= 8 ? launch_rows(a, N, K, epi, scratch, lora_b, R, ldb, req, st)
+                : launch_lora_gemm(a, N, K, epi, scratch, lora_b, R, ldb, req, st);
   if (rc != FLUXB_OK) return rc;
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "linear_lora: launch failed: %s", cudaGetErrorString(e));
