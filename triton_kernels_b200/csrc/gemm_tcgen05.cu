@@ -338,9 +338,9 @@ struct LoraGrouped {
   int count;
   int total_tiles;
   int pair_stages;
-  CUtensorMap tm_t, tm_b;  // t [M, units*32] box 32 x 128 (64-byte rows), B [n, N, R] box 16 x 128 (32-byte rows)
+  CUtensorMap tm_t, tm_b;  // t [M, ld] box of one line x 128 rows, B [n, N, R] box of one group x 128 rows
   RequestAdapters req;
-  int units;               // ranks in sixteens
+  LowRank low;
 };
 
 template <typename G>
@@ -352,39 +352,57 @@ __device__ __forceinline__ int find_problem(const G& g, int tile) {
   return i;
 }
 
-// The adapters of a tile's W x 32 rows, one warp: lane l holds rows l, 32 + l, ...  next() takes the adapter of the
-// first row that is left, and the mask of the rows that do NOT use it (bit set: row left alone).
+// The adapters of a tile's W x 32 rows, one warp.  fetch() asks for the indices, which next() looks at only behind the
+// tile's K loop, so that nobody waits for them (waiting at the head of each tile cost 5 % of the joint q|k|v
+// projection).  next() gives the adapter of the first row that is left, with the mask of the rows that do NOT use it
+// (bit set: row left alone), or -1.  A tile inside one request, the ordinary case of long requests, is one index and
+// an empty mask; else lane l holds rows l, 32 + l, ...
 template <int W>
 struct TileAdapters {
-  int a[W];
-  __device__ __forceinline__ void load(const RequestAdapters& req, int row0, int rows, int lane) {
+  int64_t raw[W];
+  int n_adapters;
+  bool single;
+  __device__ __forceinline__ void fetch(const RequestAdapters& req, int row0, int rows, int lane) {
+    n_adapters = req.n_adapters;
+    const int first = row0 / req.length;
+    single = min(row0 + W * 32, rows) <= (first + 1) * (int64_t)req.length;
+    if (single) {
+      raw[0] = req.raw(first);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < W; ++i) {
       const int row = row0 + i * 32 + lane;
-      a[i] = row < rows ? req.of_row(row) : -1;
+      raw[i] = row < rows ? req.raw(row / req.length) : -1;
     }
   }
+  __device__ __forceinline__ bool valid(int64_t a) const { return a >= 0 && a < n_adapters; }
   __device__ __forceinline__ int next(uint32_t (&off)[W]) {
     int cur = -1;
+    if (single) {
+      if (valid(raw[0])) cur = (int)raw[0];
+      raw[0] = -1;
+#pragma unroll
+      for (int i = 0; i < W; ++i) off[i] = 0;
+      return cur;
+    }
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-      const uint32_t left = __ballot_sync(0xffffffffu, a[i] >= 0);
-      const int first = __shfl_sync(0xffffffffu, a[i], left != 0 ? __ffs(left) - 1 : 0);
+      const uint32_t left = __ballot_sync(0xffffffffu, valid(raw[i]));
+      const int first = __shfl_sync(0xffffffffu, (int)raw[i], left != 0 ? __ffs(left) - 1 : 0);
       if (cur < 0 && left != 0) cur = first;
     }
     if (cur < 0) return cur;
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-      off[i] = ~__ballot_sync(0xffffffffu, a[i] == cur);
-      if (a[i] == cur) a[i] = -1;
+      off[i] = ~__ballot_sync(0xffffffffu, raw[i] == cur);
+      if (raw[i] == cur) raw[i] = -1;
     }
     return cur;
   }
 };
-constexpr int LORA_T_BYTES = BM * 64;    // one unit of t: 128 rows of 16 high + 16 low parts
-constexpr int LORA_B_BYTES = BNH * 32;   // one unit of B: 128 rows of 16 ranks
-constexpr int LORA_UNITS = 2;            // units per ring slot
-static_assert(LORA_UNITS * LORA_T_BYTES <= A_BYTES && LORA_UNITS * LORA_B_BYTES <= B_BYTES, "an adapter step fits a ring slot");
+// A ring slot of the adapters: a line of t and a group of B; a group of 64 takes two (high parts, low parts).
+__device__ __forceinline__ int lora_slots(const LowRank& low) { return low.group == 64 ? 2 * low.groups : low.groups; }
 
 // Epilogue of one 128-row x 256-column tile (two heads of q, of k or of v) for EPI_QKV_HEADS:
 // bias, rounding to bf16 (the projection's output precision in the reference), per-head RMS norm
@@ -549,7 +567,7 @@ __device__ __forceinline__ void qkv_tile_epilogue(const Params& p, const CUtenso
 //      every adapter that the tile's rows use, the MMAs t_high B^T and t_low B^T accumulate into the
 //      same TMEM tile through the same ring, with a lane mask that leaves the other requests' rows
 //      alone (so a request never meets another one's adapter, not even as a product with zero).
-//      Cost: R / 32 ring slots per adapter of a tile, next to K / 64.
+//      Cost: R / 32 ring slots per adapter of a tile, next to K / 64 of the projection.
 template <int kMode, typename G = Grouped>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 gemm_pair_kernel(const __grid_constant__ G g) {
@@ -616,35 +634,36 @@ gemm_pair_kernel(const __grid_constant__ G g) {
         const int row0 = m_blk * 2 * BM + (int)rank * BM;
         const int col0 = n_blk * BN + (int)rank * BNH;
         TileAdapters<8> rows;
-        rows.load(g.req, m_blk * 2 * BM, p.M, lane);
-        for (int kb = 0; ok && kb < num_kb; ++kb) {
-          if (lane == 0) {
+        rows.fetch(g.req, m_blk * 2 * BM, p.M, lane);
+        if (lane == 0) {
+          for (int kb = 0; kb < num_kb; ++kb) {
             ok = mbar_wait_cluster(&empty_bar[stage], phase ^ 1, abort_flag, status, 41);
-            if (ok) {
-              if (leader) mbar_expect_tx(&full_bar[stage], 2 * STAGE_BYTES);
-              const uint32_t full_addr = map_to_cta(smem_u32(&full_bar[stage]), 0);
-              uint8_t* a_dst = smem + stage * STAGE_BYTES;
-              tma_load_2d_pair(a_dst, &pr.tm_a, full_addr, kb * BK, row0);
-              tma_load_2d_pair(a_dst + A_BYTES, &pr.tm_b, full_addr, kb * BK, col0);
-            }
+            if (!ok) break;
+            if (leader) mbar_expect_tx(&full_bar[stage], 2 * STAGE_BYTES);
+            const uint32_t full_addr = map_to_cta(smem_u32(&full_bar[stage]), 0);
+            uint8_t* a_dst = smem + stage * STAGE_BYTES;
+            tma_load_2d_pair(a_dst, &pr.tm_a, full_addr, kb * BK, row0);
+            tma_load_2d_pair(a_dst + A_BYTES, &pr.tm_b, full_addr, kb * BK, col0);
+            if (++stage == g.pair_stages) { stage = 0; phase ^= 1; }
           }
-          if (++stage == g.pair_stages) { stage = 0; phase ^= 1; }
         }
+        __syncwarp();
         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        stage = __shfl_sync(0xffffffffu, stage, 0);
+        phase = __shfl_sync(0xffffffffu, phase, 0);
+        if (tile == pair_id) pdl_wait();  // t is complete; every CTA passes here, with adapters or without
         uint32_t off[8];
         for (int cur; ok && (cur = rows.next(off)) >= 0;) {
-          for (int u = 0; u < g.units; u += LORA_UNITS) {
+          for (int q = 0; q < lora_slots(g.low); ++q) {
             if (ok && lane == 0) {
-              const int n_units = min(LORA_UNITS, g.units - u);
               ok = mbar_wait_cluster(&empty_bar[stage], phase ^ 1, abort_flag, status, 46);
               if (ok) {
-                if (leader) mbar_expect_tx(&full_bar[stage], 2 * n_units * (LORA_T_BYTES + LORA_B_BYTES));
+                const int line = g.low.group == 16 ? 32 : 64;
+                if (leader) mbar_expect_tx(&full_bar[stage], 2 * (BM * line * 2 + BNH * g.low.group * 2));
                 const uint32_t full_addr = map_to_cta(smem_u32(&full_bar[stage]), 0);
                 uint8_t* a_dst = smem + stage * STAGE_BYTES;
-                for (int i = 0; i < n_units; ++i) {
-                  tma_load_2d_pair(a_dst + i * LORA_T_BYTES, &g.tm_t, full_addr, (u + i) * 32, row0);
-                  tma_load_3d_pair(a_dst + A_BYTES + i * LORA_B_BYTES, &g.tm_b, full_addr, (u + i) * 16, col0, cur);
-                }
+                tma_load_2d_pair(a_dst, &g.tm_t, full_addr, q * line, row0);
+                tma_load_3d_pair(a_dst + A_BYTES, &g.tm_b, full_addr, (g.low.group == 64 ? q >> 1 : q) * g.low.group, col0, cur);
               }
             }
             if (++stage == g.pair_stages) { stage = 0; phase ^= 1; }
@@ -691,11 +710,6 @@ gemm_pair_kernel(const __grid_constant__ G g) {
       for (int tile = pair_id; ok && tile < num_tiles; tile += num_pairs, ++local) {
         const int num_kb = (g.prob[find_problem(g, tile)].p.K + BK - 1) / BK;
         TileAdapters<8> rows;
-        if constexpr (kMode == 3) {
-          int m_blk, n_blk;
-          tile_coords(g.prob[0].p, tile, g.prob[0].tiles_m, m_blk, n_blk);
-          rows.load(g.req, m_blk * 2 * BM, g.prob[0].p.M, lane);
-        }
         const int acc = local & 1;
         const uint32_t acc_phase = (local >> 1) & 1;
         if (!__all_sync(0xffffffffu, mbar_wait_cluster(&acc_empty[acc], acc_phase ^ 1, abort_flag, status, 43))) { ok = false; break; }
@@ -714,23 +728,32 @@ gemm_pair_kernel(const __grid_constant__ G g) {
             umma_commit_pair_both(&empty_bar[stage]);
           }
           if (++stage == g.pair_stages) { stage = 0; phase ^= 1; }
+          if constexpr (kMode == 3) {
+            if (kb == 0) {  // with MMAs under way
+              int m_blk, n_blk;
+              tile_coords(g.prob[0].p, tile, g.prob[0].tiles_m, m_blk, n_blk);
+              rows.fetch(g.req, m_blk * 2 * BM, g.prob[0].p.M, lane);
+            }
+          }
         }
         if constexpr (kMode == 3) {
           uint32_t off[8];
           for (int cur; ok && (cur = rows.next(off)) >= 0;) {
-            for (int u = 0; ok && u < g.units; u += LORA_UNITS) {
+            for (int q = 0; ok && q < lora_slots(g.low); ++q) {
               ok = __all_sync(0xffffffffu, mbar_wait_cluster(&full_bar[stage], phase, abort_flag, status, 47));
               if (!ok) break;
               tc_fence_after_sync();
               const uint32_t a_addr = smem_u32(smem + stage * STAGE_BYTES);
-              const uint64_t adesc = make_smem_desc(a_addr, 16, 512, 4);
-              const uint64_t bdesc = make_smem_desc(a_addr + A_BYTES, 16, 256, 6);
-              const int n_units = min(LORA_UNITS, g.units - u);
+              const uint64_t adesc = g.low.desc(a_addr);
+              const uint64_t bdesc = g.low.group == 64   ? make_smem_desc(a_addr + A_BYTES, 16, 1024)
+                                     : g.low.group == 32 ? make_smem_desc(a_addr + A_BYTES, 16, 512, 4)
+                                                         : make_smem_desc(a_addr + A_BYTES, 16, 256, 6);
+              const int first = (g.low.group == 64 ? q >> 1 : q) * (g.low.group / 16);
+              const int n_units = min(g.low.group / 16, g.low.units - first);
               if (elect_one()) {
                 for (int i = 0; i < n_units; ++i) {
-                  const uint64_t ad = adesc + i * (LORA_T_BYTES >> 4), bd = bdesc + i * (LORA_B_BYTES >> 4);
-                  umma_ss_pair_masked(d_tmem, ad, bd, idesc, off);      // high parts
-                  umma_ss_pair_masked(d_tmem, ad + 2, bd, idesc, off);  // low parts, 32 bytes further
+                  umma_ss_pair_masked(d_tmem, adesc + 2 * i, bdesc + 2 * i, idesc, off);
+                  if (g.low.group < 64) umma_ss_pair_masked(d_tmem, adesc + g.low.low(i), bdesc + 2 * i, idesc, off);
                 }
                 umma_commit_pair_both(&empty_bar[stage]);
               }
@@ -845,7 +868,6 @@ using gemm::Params;
 using gemm::epilogue_chunk;
 using gemm2::TileAdapters;
 constexpr int THREADS = 192;
-constexpr int T_BYTES = BM * 64;  // one unit of t: 128 rows of 16 high + 16 low parts
 constexpr int MAX_STAGES = 16;
 constexpr int MAX_SMEM = 224 * 1024;
 
@@ -853,7 +875,8 @@ struct Tiles {
   CUtensorMap tm_a, tm_b, tm_t, tm_lb;
   Params p;
   RequestAdapters req;
-  int units, stages;
+  LowRank low;
+  int stages;
   int a_rows;  // rows of x per box: fewer than 128 when there are fewer; the MMAs then read what lies behind them in
                // shared memory as the other rows, whose results are never stored
 };
@@ -866,12 +889,13 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   uint8_t* t_smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* smem = t_smem + g.units * T_BYTES;
+  const int T_BYTES = g.low.groups * g.low.tile_bytes();
+  uint8_t* smem = t_smem + T_BYTES;
   volatile int* abort_flag = &abort_word;
   const Params& p = g.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int num_kb = (p.K + BK - 1) / BK;
-  const int groups = (g.units + 3) / 4;  // of 64 ranks
+  const int slots = (g.low.units + 3) / 4;  // of 64 ranks of B
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < g.stages; ++s) {
@@ -907,7 +931,7 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
     for (int tile = blockIdx.x; ok && tile < p.num_tiles; tile += gridDim.x) {
       const int row0 = tile % p.tiles_m * BM, col0 = tile / p.tiles_m * BN;
       TileAdapters<4> rows;
-      rows.load(g.req, row0, p.M, lane);
+      rows.fetch(g.req, row0, p.M, lane);
       if (lane == 0) {
         for (int kb = 0; kb < num_kb; ++kb) {
           ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, 91);
@@ -923,6 +947,7 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
       stage = __shfl_sync(0xffffffffu, stage, 0);
       phase = __shfl_sync(0xffffffffu, phase, 0);
+      if (tile == (int)blockIdx.x) pdl_wait();  // t is complete
       uint32_t off[4];
       bool first = true;
       for (int cur; ok && (cur = rows.next(off)) >= 0;) {
@@ -930,11 +955,12 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
           if (first) {
             ok = mbar_wait(&t_empty, t_phase ^ 1, abort_flag, p.status, 92);
             if (ok) {
-              mbar_expect_tx(&t_full, g.units * T_BYTES);
-              for (int u = 0; u < g.units; ++u) tma_load_2d(t_smem + u * T_BYTES, &g.tm_t, &t_full, u * 32, row0);
+              const int line = g.low.group == 16 ? 32 : 64;
+              mbar_expect_tx(&t_full, T_BYTES);
+              for (int c = 0; c < g.low.ld(); c += line) tma_load_2d(t_smem + c * BM * 2, &g.tm_t, &t_full, c, row0);
             }
           }
-          for (int q = 0; ok && q < groups; ++q) {
+          for (int q = 0; ok && q < slots; ++q) {
             ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, 93);
             if (!ok) break;
             mbar_expect_tx(&full_bar[stage], BN * BK * 2);
@@ -959,7 +985,7 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
     int local = 0;
     for (int tile = blockIdx.x; ok && tile < p.num_tiles; tile += gridDim.x, ++local) {
       TileAdapters<4> rows;
-      rows.load(g.req, tile % p.tiles_m * BM, p.M, lane);
+      rows.fetch(g.req, tile % p.tiles_m * BM, p.M, lane);
       const int acc = local & 1;
       const uint32_t acc_phase = (local >> 1) & 1;
       ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[acc], acc_phase ^ 1, abort_flag, p.status, 94));
@@ -983,18 +1009,18 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
       bool first = true;
       for (int cur; ok && (cur = rows.next(off)) >= 0;) {
         if (first) ok = __all_sync(0xffffffffu, mbar_wait(&t_full, t_phase, abort_flag, p.status, 96));
-        for (int q = 0; ok && q < groups; ++q) {
+        for (int q = 0; ok && q < slots; ++q) {
           ok = __all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, abort_flag, p.status, 97));
           if (!ok) break;
           tc_fence_after_sync();
-          const uint64_t adesc = make_smem_desc(smem_u32(t_smem + q * 4 * T_BYTES), 16, 512, 4);
+          // (more than 64 ranks: groups of 64, one per slot; up to 64 there is one group and one slot)
+          const uint64_t adesc = g.low.desc(smem_u32(t_smem + q * g.low.tile_bytes()));
           const uint64_t bdesc = make_smem_desc(smem_u32(smem + stage * STAGE_BYTES) + A_BYTES, 16, 1024);
-          const int n_units = min(4, g.units - q * 4);
+          const int n_units = min(4, g.low.units - q * 4);
           if (elect_one()) {
             for (int i = 0; i < n_units; ++i) {
-              const uint64_t ad = adesc + i * (T_BYTES >> 4);
-              umma_ss_masked(d_tmem, ad, bdesc + 2 * i, idesc, off);      // high parts
-              umma_ss_masked(d_tmem, ad + 2, bdesc + 2 * i, idesc, off);  // low parts, 32 bytes further
+              umma_ss_masked(d_tmem, adesc + g.low.high(i), bdesc + 2 * i, idesc, off);
+              umma_ss_masked(d_tmem, adesc + g.low.low(i), bdesc + 2 * i, idesc, off);
             }
             umma_commit(&empty_bar[stage]);
           }
@@ -1044,7 +1070,7 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
 }
 
 template <int BN>
-static int launch_tiles(Tiles& g, const fluxb_linear_problem& a, int64_t N, int64_t K, const void* lora_b, int64_t R, int64_t ldb,
+static int launch_tiles(Tiles& g, const fluxb_linear_problem& a, int64_t N, int64_t K, const void* lora_b, int64_t ldb,
                         cudaStream_t st) {
   {
     const uint64_t dims[2] = {(uint64_t)K, (uint64_t)N}, strides[1] = {(uint64_t)a.ldw * 2};
@@ -1053,14 +1079,15 @@ static int launch_tiles(Tiles& g, const fluxb_linear_problem& a, int64_t N, int6
     if (rc != FLUXB_OK) return rc;
   }
   {
-    const uint64_t dims[3] = {(uint64_t)R, (uint64_t)N, (uint64_t)g.req.n_adapters};
+    const uint64_t dims[3] = {(uint64_t)g.low.R, (uint64_t)N, (uint64_t)g.req.n_adapters};
     const uint64_t strides[2] = {(uint64_t)ldb * 2, (uint64_t)(N * ldb) * 2};
     const uint32_t box[3] = {64, BN, 1};
     int rc = encode_tmap_bf16(&g.tm_lb, lora_b, 3, dims, strides, box);
     if (rc != FLUXB_OK) return rc;
   }
   const int stage_bytes = g.a_rows * BK * 2 + BN * BK * 2, behind = (BM - g.a_rows) * BK * 2;
-  g.stages = (MAX_SMEM - 1024 - 512 - g.units * T_BYTES - behind) / stage_bytes;
+  const int t_bytes = g.low.groups * g.low.group * 512;
+  g.stages = (MAX_SMEM - 1024 - 512 - t_bytes - behind) / stage_bytes;
   if (g.stages > MAX_STAGES) g.stages = MAX_STAGES;
   g.p.tiles_n = (int)((N + BN - 1) / BN);
   g.p.num_tiles = g.p.tiles_m * g.p.tiles_n;
@@ -1068,7 +1095,8 @@ static int launch_tiles(Tiles& g, const fluxb_linear_problem& a, int64_t N, int6
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM);
   if (e != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "linear_lora: cannot set shared memory size: %s", cudaGetErrorString(e));
   const int grid = g.p.num_tiles < sm_count() ? g.p.num_tiles : sm_count();
-  kern<<<grid, THREADS, 1024 + g.units * T_BYTES + g.stages * stage_bytes + behind, st>>>(g);
+  e = launch_after(kern, grid, THREADS, 1024 + t_bytes + g.stages * stage_bytes + behind, st, g);
+  if (e != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "linear_lora: launch failed: %s", cudaGetErrorString(e));
   return FLUXB_OK;
 }
 
@@ -1363,9 +1391,17 @@ extern "C" int fluxb_linear_qkv_grouped_scatter(const fluxb_linear_problem* prob
                                  round_before_act, stream);
 }
 
+// t [M, ld] in boxes of one line x 128 rows.
+static int encode_low_rank(CUtensorMap* out, const void* t_rows, int64_t M, const LowRank& low) {
+  const uint64_t dims[2] = {(uint64_t)low.ld(), (uint64_t)M}, strides[1] = {(uint64_t)low.ld() * 2};
+  const uint32_t box[2] = {(uint32_t)(low.group == 16 ? 32 : 64), fluxb::gemm::BM};
+  return encode_tmap_bf16(out, t_rows, 2, dims, strides, box,
+                          low.group == 16 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 // The projection of fluxb_linear_lora for more rows than the row-streaming kernel takes; t as lora.cu leaves it.
-int fluxb::launch_lora_gemm(const fluxb_linear_problem& a, int64_t N, int64_t K, int epi, const void* low, const void* lora_b,
-                            int64_t R, int64_t ldb, const RequestAdapters& req, cudaStream_t st) {
+int fluxb::launch_lora_gemm(const fluxb_linear_problem& a, int64_t N, int64_t K, int epi, const void* t_rows,
+                            const void* lora_b, const LowRank& low, int64_t ldb, const RequestAdapters& req, cudaStream_t st) {
   // Which tiles: cycles per 64-wide K step are 512 for a 256 x 256 tile of a CTA pair (its MMAs), and 64 bytes a cycle of
   // operands for a 128 x BN tile of one CTA; on top of the K loop the last tile's epilogue shows, 20 000 cycles of the
   // pair kernel's and about 40 per column of the other's.
@@ -1384,19 +1420,17 @@ int fluxb::launch_lora_gemm(const fluxb_linear_problem& a, int64_t N, int64_t K,
     int rc = prepare_problem(a, N, K, epi, N, FLUXB_EPI_NONE, 0, false, &t.tm_a, &t.tm_b, &t.p);
     if (rc != FLUXB_OK) return rc;
     t.req = req;
-    t.units = (int)((R + 15) / 16);
+    t.low = low;
     t.a_rows = (int)a_rows;
     {
       const uint64_t dims[2] = {(uint64_t)K, (uint64_t)a.M}, strides[1] = {(uint64_t)a.ldx * 2};
       const uint32_t box[2] = {64, (uint32_t)a_rows};
       if ((rc = encode_tmap_bf16(&t.tm_a, a.x, 2, dims, strides, box)) != FLUXB_OK) return rc;
     }
-    const uint64_t dims[2] = {(uint64_t)t.units * 32, (uint64_t)a.M}, strides[1] = {(uint64_t)t.units * 64};
-    const uint32_t box[2] = {32, fluxb::gemm::BM};
-    if ((rc = encode_tmap_bf16(&t.tm_t, low, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B)) != FLUXB_OK) return rc;
-    if (bn == 128) return fluxb::gemm3::launch_tiles<128>(t, a, N, K, lora_b, R, ldb, st);
-    if (bn == 64) return fluxb::gemm3::launch_tiles<64>(t, a, N, K, lora_b, R, ldb, st);
-    return fluxb::gemm3::launch_tiles<32>(t, a, N, K, lora_b, R, ldb, st);
+    if ((rc = encode_low_rank(&t.tm_t, t_rows, a.M, low)) != FLUXB_OK) return rc;
+    if (bn == 128) return fluxb::gemm3::launch_tiles<128>(t, a, N, K, lora_b, ldb, st);
+    if (bn == 64) return fluxb::gemm3::launch_tiles<64>(t, a, N, K, lora_b, ldb, st);
+    return fluxb::gemm3::launch_tiles<32>(t, a, N, K, lora_b, ldb, st);
   }
   using namespace fluxb::gemm2;
   LoraGrouped g;
@@ -1411,17 +1445,16 @@ int fluxb::launch_lora_gemm(const fluxb_linear_problem& a, int64_t N, int64_t K,
     if ((rc = encode_tmap_bf16(&pr.tm_y, a.y, 2, dims, strides, box)) != FLUXB_OK) return rc;
     pr.tm_y2 = pr.tm_y;
   }
-  g.units = (int)((R + 15) / 16);
+  g.low = low;
+  if ((rc = encode_low_rank(&g.tm_t, t_rows, a.M, low)) != FLUXB_OK) return rc;
   {
-    const uint64_t dims[2] = {(uint64_t)g.units * 32, (uint64_t)a.M}, strides[1] = {(uint64_t)g.units * 64};
-    const uint32_t box[2] = {32, BM};
-    if ((rc = encode_tmap_bf16(&g.tm_t, low, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B)) != FLUXB_OK) return rc;
-  }
-  {
-    const uint64_t dims[3] = {(uint64_t)R, (uint64_t)N, (uint64_t)req.n_adapters};
+    const uint64_t dims[3] = {(uint64_t)low.R, (uint64_t)N, (uint64_t)req.n_adapters};
     const uint64_t strides[2] = {(uint64_t)ldb * 2, (uint64_t)(N * ldb) * 2};
-    const uint32_t box[3] = {16, BNH, 1};
-    if ((rc = encode_tmap_bf16(&g.tm_b, lora_b, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_32B)) != FLUXB_OK) return rc;
+    const uint32_t box[3] = {(uint32_t)low.group, BNH, 1};
+    const CUtensorMapSwizzle swz = low.group == 64   ? CU_TENSOR_MAP_SWIZZLE_128B
+                                   : low.group == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                     : CU_TENSOR_MAP_SWIZZLE_32B;
+    if ((rc = encode_tmap_bf16(&g.tm_b, lora_b, 3, dims, strides, box, swz)) != FLUXB_OK) return rc;
   }
   g.req = req;
   pr.tiles_m = (int)((a.M + 255) / 256);
@@ -1431,7 +1464,8 @@ int fluxb::launch_lora_gemm(const fluxb_linear_problem& a, int64_t N, int64_t K,
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
   if (e != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "linear_lora: cannot set shared memory size: %s", cudaGetErrorString(e));
   const int pairs = g.total_tiles < sm_count() / 2 ? g.total_tiles : sm_count() / 2;
-  kern<<<2 * pairs, THREADS, SMEM_BYTES, st>>>(g);
+  e = launch_after(kern, 2 * pairs, THREADS, SMEM_BYTES, st, g);
+  if (e != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "linear_lora: launch failed: %s", cudaGetErrorString(e));
   return FLUXB_OK;
 }
 

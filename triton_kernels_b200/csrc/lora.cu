@@ -21,7 +21,8 @@ struct Params {
   CUtensorMap tm_a;  // [n, R, K], box 64 x rpad
   RequestAdapters req;
   const float* scale;  // nullptr: ones
-  __nv_bfloat16* t;    // [M, units * 32]: per 16 ranks, 16 high parts then 16 low parts
+  __nv_bfloat16* t;    // [M, low.ld()]
+  LowRank low;
   int L, tiles_per_request, box_rows;
   int num_kb, ksplit, rpad, stages, tmem_cols;
   DeviceStatus* status;
@@ -77,6 +78,7 @@ __global__ void __launch_bounds__(THREADS, 1) lora_shrink_kernel(const __grid_co
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = tmem_slot;
+  pdl_release();  // behind the TMEM allocation: the projection's blocks take all of an SM's TMEM
 
   if (warp == 0) {
     if (lane == 0) {
@@ -143,7 +145,7 @@ __global__ void __launch_bounds__(THREADS, 1) lora_shrink_kernel(const __grid_co
   }
   cluster_sync_all();
   const float scale = p.scale != nullptr ? p.scale[adapter] : 1.f;
-  const int t_ld = p.rpad * 2;
+  const int t_ld = p.low.ld();
   for (int i = rank * THREADS + threadIdx.x; i < p.rpad / 8 * BM; i += p.ksplit * THREADS) {
     const int row = i & (BM - 1), c8 = i / BM * 8;
     if (row >= rows) continue;
@@ -162,9 +164,9 @@ __global__ void __launch_bounds__(THREADS, 1) lora_shrink_kernel(const __grid_co
       const float la = a - bf16_lo(hi[e]), lb = b - bf16_hi(hi[e]);
       lo[e] = pack_bf16(isinf(bf16_lo(hi[e])) ? 0.f : la, isinf(bf16_hi(hi[e])) ? 0.f : lb);
     }
-    __nv_bfloat16* dst = p.t + (int64_t)(row0 + row) * t_ld + c8 / 16 * 32 + (c8 & 8);
+    __nv_bfloat16* dst = p.t + (int64_t)(row0 + row) * t_ld + p.low.column(c8);
     *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    *reinterpret_cast<uint4*>(dst + 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    *reinterpret_cast<uint4*>(dst + p.low.group) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
   cluster_sync_all();  // no CTA leaves while another reads its partial sums
 }
@@ -172,22 +174,24 @@ __global__ void __launch_bounds__(THREADS, 1) lora_shrink_kernel(const __grid_co
 }  // namespace shrink
 
 static int launch_shrink(const void* x, int64_t ldx, const void* lora_a, const float* scale, void* t, const RequestAdapters& req,
-                         int64_t B, int64_t L, int64_t K, int64_t R, cudaStream_t st) {
+                         int64_t B, int64_t L, int64_t K, const LowRank& low, cudaStream_t st) {
   using namespace shrink;
   Params p;
   p.req = req;
+  p.low = low;
   p.scale = scale;
   p.t = static_cast<__nv_bfloat16*>(t);
   p.L = (int)L;
   p.tiles_per_request = (int)((L + BM - 1) / BM);
   p.box_rows = (int)(L < BM ? (L + 7) / 8 * 8 : BM);
-  p.rpad = (int)((R + 15) / 16 * 16);
+  p.rpad = low.units * 16;
   p.num_kb = (int)((K + BK - 1) / BK);
   p.status = device_status_ptr();
   const int64_t tiles = B * p.tiles_per_request;
-  // K is split until the clusters fill the machine, as long as a CTA keeps four 64-wide steps.
+  // K is split until the clusters fill the machine, as long as a CTA keeps four 64-wide steps.  Clusters of eight do
+  // not all find a place at once from 16 on (2048 rows, K 3072: 16.7 us with eight, 9.9 with four, 12.0 with two).
   p.ksplit = 1;
-  while (p.ksplit < 8 && tiles * p.ksplit * 2 <= sm_count() && p.num_kb >= p.ksplit * 2 * 4) p.ksplit *= 2;
+  while (p.ksplit < (tiles < 12 ? 8 : 4) && tiles * p.ksplit * 2 <= sm_count() && p.num_kb >= p.ksplit * 2 * 4) p.ksplit *= 2;
   const int steps = (p.num_kb + p.ksplit - 1) / p.ksplit;
   const int stage_bytes = BM * BK * 2 + p.rpad * BK * 2;
   p.stages = MAX_SMEM / stage_bytes < MAX_STAGES ? MAX_SMEM / stage_bytes : MAX_STAGES;
@@ -205,8 +209,8 @@ static int launch_shrink(const void* x, int64_t ldx, const void* lora_a, const f
     if (rc != FLUXB_OK) return rc;
   }
   {
-    const uint64_t dims[3] = {(uint64_t)K, (uint64_t)R, (uint64_t)req.n_adapters};
-    const uint64_t strides[2] = {(uint64_t)K * 2, (uint64_t)R * K * 2};
+    const uint64_t dims[3] = {(uint64_t)K, (uint64_t)low.R, (uint64_t)req.n_adapters};
+    const uint64_t strides[2] = {(uint64_t)K * 2, (uint64_t)(low.R * K) * 2};
     const uint32_t box[3] = {BK, (uint32_t)p.rpad, 1};
     int rc = encode_tmap_bf16(&p.tm_a, lora_a, 3, dims, strides, box);
     if (rc != FLUXB_OK) return rc;
@@ -230,29 +234,133 @@ static int launch_shrink(const void* x, int64_t ldx, const void* lora_a, const f
 }
 
 // ----------------------------------------------------------------------------------------
-// One to eight rows: the projection is a stream of W.  A block takes 16 output columns, its warps share K; a warp's
-// lane loads 16 bytes of two W rows and uses them as the A fragments of mma.m16n8k16 (W's columns are the M side, the
-// rows of x the N side), with x's fragment loaded from the same k positions: the order of k does not matter as long as
-// both sides agree, so no shuffle or shared memory stands between the load and the product.  All 24 loads of a step
-// are in flight at once, and those of the next step leave before the current one is summed over the warps.  The
-// adapters are 2 R more products per output, from the high and low parts of t, in the epilogue.
+// Low-rank rows of short requests (up to eight rows): rows of A against the request's rows of x by the threads of
+// a block.  The tensor-core kernel above takes 7 us for eight requests of one row, almost all of it set-up (tensor maps,
+// TMEM, cluster barriers); this one 4.7.  It needs next to no shared memory, so the row-streaming projection can start
+// beside it.
+// ----------------------------------------------------------------------------------------
+namespace shrink {
+constexpr int SHORT = 8;
+struct ShortParams {
+  const __nv_bfloat16 *x, *a;
+  const float* scale;
+  __nv_bfloat16* t;
+  RequestAdapters req;
+  LowRank low;
+  int64_t ldx;
+  int K;
+  DeviceStatus* status;
+};
+
+// Four warps share K; a block takes kRanks ranks of one request.
+template <int kRanks>
+__global__ void __launch_bounds__(128) lora_shrink_short_kernel(const ShortParams p) {
+  __shared__ float red[4][kRanks][SHORT];
+  const int ranks = p.low.units * 16;  // the ranks behind R are zeros: the tensor cores multiply them, too
+  const int request = blockIdx.x / (ranks / kRanks), j0 = (blockIdx.x - request * (ranks / kRanks)) * kRanks;
+  const int L = p.req.length, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int adapter = p.req.of_request(request);
+  if (adapter < 0) {
+    if (j0 == 0 && threadIdx.x == 0 && p.req.raw(request) != -1) report_error(p.status, FLUXB_ERR_BAD_ARG, 81);
+    return;
+  }
+  const __nv_bfloat16* a = p.a + ((int64_t)adapter * p.low.R + j0) * p.K;
+  const __nv_bfloat16* x = p.x + (int64_t)request * L * p.ldx;
+  float acc[kRanks][SHORT] = {};
+  constexpr int kAhead = kRanks == 1 ? 4 : 1;  // steps whose loads are in flight together
+  for (int k0 = threadIdx.x * 8; k0 < p.K; k0 += 1024 * kAhead) {
+    uint4 av[kAhead][kRanks];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+      for (int r = 0; r < kRanks; ++r)
+        av[i][r] = k0 + i * 1024 < p.K && j0 + r < p.low.R ? __ldg(reinterpret_cast<const uint4*>(a + (int64_t)r * p.K + k0 + i * 1024))
+                                                          : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (k0 + i * 1024 >= p.K) break;
+#pragma unroll
+      for (int l = 0; l < SHORT; ++l) {
+        if (l < L) {
+          const uint4 xv = __ldg(reinterpret_cast<const uint4*>(x + l * p.ldx + k0 + i * 1024));
+          const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
+#pragma unroll
+          for (int r = 0; r < kRanks; ++r) {
+            const uint32_t aw[4] = {av[i][r].x, av[i][r].y, av[i][r].z, av[i][r].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              acc[r][l] = fmaf(bf16_hi(aw[e]), bf16_hi(xw[e]), fmaf(bf16_lo(aw[e]), bf16_lo(xw[e]), acc[r][l]));
+          }
+        }
+      }
+    }
+  }
+  pdl_release();  // behind the loads: the projection's stream of W would get in front of them
+#pragma unroll
+  for (int l = 0; l < SHORT; ++l) {
+    if (l < L) {
+#pragma unroll
+      for (int r = 0; r < kRanks; ++r) {
+        const float s = warp_sum(acc[r][l]);
+        if (lane == 0) red[warp][r][l] = s;
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kRanks * L; i += 128) {
+    const int r = i % kRanks, l = i / kRanks;
+    float v = 0.f;
+    if (j0 + r < p.low.R)  // (a rank of zeros would be NaN beside an infinite x)
+      v = (red[0][r][l] + red[1][r][l] + red[2][r][l] + red[3][r][l]) * (p.scale != nullptr ? p.scale[adapter] : 1.f);
+    const __nv_bfloat16 hi = __float2bfloat16_rn(v);
+    const float h = __bfloat162float(hi);
+    __nv_bfloat16* dst = p.t + ((int64_t)request * L + l) * p.low.ld() + p.low.column(j0 + r);
+    dst[0] = hi;
+    dst[p.low.group] = __float2bfloat16_rn(isinf(h) ? 0.f : v - h);
+  }
+}
+}  // namespace shrink
+
+static int launch_shrink_short(const void* x, int64_t ldx, const void* lora_a, const float* scale, void* t,
+                               const RequestAdapters& req, int64_t B, int64_t K, const LowRank& low, cudaStream_t st) {
+  if (B * low.units * 16 > INT32_MAX) return set_error(FLUXB_ERR_UNSUPPORTED, "linear_lora: too many requests");
+  shrink::ShortParams p{static_cast<const __nv_bfloat16*>(x), static_cast<const __nv_bfloat16*>(lora_a), scale,
+                        static_cast<__nv_bfloat16*>(t), req, low, ldx, (int)K, device_status_ptr()};
+  const int64_t ranks = B * low.units * 16;
+  // four ranks a block read x a quarter as often; one a block spreads few requests over the machine
+  if (ranks >= 4 * sm_count()) shrink::lora_shrink_short_kernel<4><<<(unsigned)(ranks / 4), 128, 0, st>>>(p);
+  else shrink::lora_shrink_short_kernel<1><<<(unsigned)ranks, 128, 0, st>>>(p);
+  return FLUXB_OK;
+}
+
+// ----------------------------------------------------------------------------------------
+// One to eight rows: the projection is a stream of W.  A block takes 16 output columns at a time; the 16 rows of W
+// come through a ring in shared memory by bulk copies (2 KB of a row each, 200 KB in flight per SM: the block keeps
+// asking while it computes), and its eight warps share a piece's columns.  The products run as mma.m16n8k16 with W's
+// rows on the M side and the rows of x on the N side; a lane reads 16 consecutive bytes of two W rows and uses them as
+// its A fragments of two MMAs, with x's fragment taken from the same k positions: the order of k does not matter as
+// long as both sides agree.  x's fragments stay in registers for all tiles (kPieces pieces of W; 0: read each time).
+// The adapters are R more products per output, from t's two parts widened to fp32.
+// (With W loaded straight to registers, 98 KB in flight per SM: 27 us for 18432 x 3072 instead.)
 // ----------------------------------------------------------------------------------------
 namespace rows {
-constexpr int SLICE = 384;  // k per warp and step: 12 fragments of 32
-constexpr int STEPS = SLICE / 32;
-constexpr int MAX_WARPS = 8;
+constexpr int WARPS = 8;
+constexpr int THREADS = WARPS * 32 + 32 + 128;  // and a warp that issues the copies, and four that finish the outputs
+constexpr int AHEAD = 4;                  // eights of ranks whose loads leave ahead of a tile's sums
+constexpr int PIECE = 1024;               // most columns of W per ring slot
+constexpr int MAX_SLOTS = 12;
+constexpr int RING_BYTES = 200 * 1024;
 
 struct Params {
   const __nv_bfloat16 *x, *w, *bias, *t, *lora_b;
   __nv_bfloat16* y;
   RequestAdapters req;
+  LowRank low;
   int64_t ldx, ldw, ldy, ldb;
-  int M, N, K, R, rpad, epi, tiles, slices;  // slices: steps of a warp per tile
+  int M, N, K, epi, tiles, piece, pieces, slots;
+  DeviceStatus* status;
 };
 
-__device__ __forceinline__ uint4 ld_or_zero(const __nv_bfloat16* p, bool ok) {
-  return ok ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
-}
 __device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                             uint32_t b1) {
   asm volatile(
@@ -260,7 +368,6 @@ __device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// sum of t[j] * b[j] over eight ranks; t as high and low parts
 __device__ __forceinline__ float dot8(const uint4& b, const float* t, float acc) {
   const uint32_t w[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
@@ -268,106 +375,206 @@ __device__ __forceinline__ float dot8(const uint4& b, const float* t, float acc)
   return acc;
 }
 
-// kOne: a warp's share of K is one step, and its fragments of x stay in registers for all tiles.
-template <bool kOne>
-__global__ void __launch_bounds__(MAX_WARPS * 32, 1) lora_rows_kernel(const Params p) {
-  __shared__ float red[2][MAX_WARPS][16][9];
+template <int kPieces>
+__global__ void __launch_bounds__(THREADS, 1) lora_rows_kernel(const Params p) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ uint64_t full_bar[MAX_SLOTS], empty_bar[MAX_SLOTS], red_full[2], red_empty[2];
+  __shared__ float red[2][WARPS][16][9];
   __shared__ float t_s[8][256];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const int g = lane >> 2, t4 = lane & 3;
-  const __nv_bfloat16* xr = p.x + g * p.ldx;
-  uint4 bx[STEPS], a0[STEPS], a1[STEPS];
-  auto load_x = [&](int slice) {
-    const int k0 = (slice * warps + warp) * SLICE + t4 * 8;
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) bx[s] = ld_or_zero(xr + k0 + s * 32, g < p.M && k0 + s * 32 < p.K);
-  };
-  auto load_w = [&](int tile, int slice) {
-    const int k0 = (slice * warps + warp) * SLICE + t4 * 8;
-    const int n = tile * 16 + g;
-    const __nv_bfloat16* w0 = p.w + n * p.ldw + k0;
-    const __nv_bfloat16* w1 = w0 + 8 * p.ldw;
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      const bool in = k0 + s * 32 < p.K;
-      a0[s] = ld_or_zero(w0 + s * 32, in && n < p.N);
-      a1[s] = ld_or_zero(w1 + s * 32, in && n + 8 < p.N);
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // 64 bytes behind each row: eight lanes that read two rows then touch all banks once
+  const int pitch = p.piece * 2 + 64, slot_bytes = 16 * pitch;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.slots; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], WARPS);
     }
-  };
-  if (kOne) load_x(0);
-  int tile = blockIdx.x;
-  load_w(tile, 0);
-  // t of the requests that have an adapter, widened
-  for (int i = threadIdx.x; i < p.M * p.rpad; i += blockDim.x) {
-    const int m = i / p.rpad, j = i - m * p.rpad;
-    float v = 0.f;
-    if (p.req.of_row(m) >= 0) {
-      const __nv_bfloat16* src = p.t + (int64_t)m * p.rpad * 2 + j / 16 * 32 + j % 16;
-      v = __bfloat162float(src[0]) + __bfloat162float(src[16]);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&red_full[i], WARPS);
+      mbar_init(&red_empty[i], 4);
     }
-    t_s[m][j] = v;
+    *abort_flag = 0;
+    mbar_fence_init();
+    fence_proxy_async_smem();
   }
-  int buf = 0;
-  for (; tile < p.tiles; tile += gridDim.x) {
-    float c[4] = {};
-    for (int slice = 0; slice < (kOne ? 1 : p.slices); ++slice) {
-      if (!kOne) load_x(slice);
+  __syncthreads();
+  int slot = 0;
+  uint32_t phase = 0;
+  if (warp == WARPS) {
+    for (int tile = blockIdx.x; tile < p.tiles; tile += gridDim.x) {
+      const int rows = min(16, p.N - tile * 16);
+      for (int piece = 0; piece < p.pieces; ++piece) {
+        const uint32_t bytes = min(p.piece, p.K - piece * p.piece) * 2;
+        bool ok = true;
+        if (lane == 0) {
+          ok = mbar_wait(&empty_bar[slot], phase ^ 1, abort_flag, p.status, 85);
+          if (ok) mbar_expect_tx(&full_bar[slot], rows * bytes);
+        }
+        if (!__shfl_sync(0xffffffffu, (int)ok, 0)) return;
+        if (lane < rows) {
+          const __nv_bfloat16* src = p.w + (int64_t)(tile * 16 + lane) * p.ldw + piece * p.piece;
+          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                           smem_u32(ring + slot * slot_bytes + lane * pitch)),
+                       "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(&full_bar[slot]))
+                       : "memory");
+        }
+        if (++slot == p.slots) { slot = 0; phase ^= 1; }
+      }
+    }
+    return;
+  }
+  if (warp > WARPS) {
+    // One thread per output of a tile: sums the eight warps' shares and adds bias and adapter.  Warps of their own,
+    // which ask for their rows of B before they wait, because a tile's finish is all latency: done by the streaming
+    // warps it cost a third of the time (29.8 us).
+    const int e = threadIdx.x - (WARPS + 1) * 32;
+    const int m = e >> 4, nl = e & 15;
+    const int adapter = m < p.M ? p.req.of_row(m) : -1;
+    const int ahead = min(p.low.R / 8, AHEAD);
+    int parity = 0;
+    uint32_t red_phase = 0;
+    for (int tile = blockIdx.x; tile < p.tiles; tile += gridDim.x) {
+      const int n = tile * 16 + nl;
+      const bool mine = m < p.M && n < p.N;
+      const __nv_bfloat16* b = p.lora_b + ((int64_t)adapter * p.N + n) * p.ldb;
+      uint4 bv[AHEAD];
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        mma_16x8x16(c, a0[s].x, a1[s].x, a0[s].y, a1[s].y, bx[s].x, bx[s].y);
-        mma_16x8x16(c, a0[s].z, a1[s].z, a0[s].w, a1[s].w, bx[s].z, bx[s].w);
+      for (int i = 0; i < AHEAD; ++i)
+        if (mine && adapter >= 0 && i < ahead) bv[i] = __ldg(reinterpret_cast<const uint4*>(b + i * 8));
+      float v = mine && p.bias != nullptr ? __bfloat162float(p.bias[n]) : 0.f;
+      if (tile == (int)blockIdx.x) {  // t of the requests that have an adapter, widened
+        pdl_wait();
+        for (int i = e; i < p.M * p.low.R; i += 128) {
+          const int mm = i / p.low.R, j = i - mm * p.low.R;
+          float w = 0.f;
+          if (p.req.of_row(mm) >= 0) {
+            const __nv_bfloat16* src = p.t + (int64_t)mm * p.low.ld() + p.low.column(j);
+            w = __bfloat162float(src[0]) + __bfloat162float(src[p.low.group]);
+          }
+          t_s[mm][j] = w;
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
       }
-      if (!kOne && slice + 1 < p.slices) load_w(tile, slice + 1);
-      else if (tile + (int)gridDim.x < p.tiles) load_w(tile + gridDim.x, 0);
-    }
-    red[buf][warp][g][2 * t4] = c[0];
-    red[buf][warp][g][2 * t4 + 1] = c[1];
-    red[buf][warp][g + 8][2 * t4] = c[2];
-    red[buf][warp][g + 8][2 * t4 + 1] = c[3];
-    __syncthreads();  // the other buffer's readers are through before anyone gets here again
-    for (int i = threadIdx.x; i < 128; i += blockDim.x) {
-      const int m = i >> 4, n = tile * 16 + (i & 15);
-      if (m >= p.M || n >= p.N) continue;
-      float v = p.bias != nullptr ? __bfloat162float(p.bias[n]) : 0.f;
-      for (int w = 0; w < warps; ++w) v += red[buf][w][i & 15][m];
-      const int a = p.req.of_row(m);
-      if (a >= 0) {
-        const __nv_bfloat16* b = p.lora_b + ((int64_t)a * p.N + n) * p.ldb;
-        float s = 0.f;
-        int j = 0;
-        for (; j + 8 <= p.R; j += 8) s = dot8(__ldg(reinterpret_cast<const uint4*>(b + j)), &t_s[m][j], s);
-        for (; j < p.R; ++j) s = fmaf(__bfloat162float(b[j]), t_s[m][j], s);
-        v += s;
+      float s = 0.f;
+      if (mine && adapter >= 0) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+          if (i < ahead) s = dot8(bv[i], &t_s[m][i * 8], s);
+        int j = ahead * 8;
+#pragma unroll 4
+        for (; j + 8 <= p.low.R; j += 8) s = dot8(__ldg(reinterpret_cast<const uint4*>(b + j)), &t_s[m][j], s);
+        for (; j < p.low.R; ++j) s = fmaf(__bfloat162float(b[j]), t_s[m][j], s);
       }
+      __syncwarp();
+      if (!__all_sync(0xffffffffu, mbar_wait(&red_full[parity], red_phase, abort_flag, p.status, 88))) return;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) v += red[parity][w][nl][m];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&red_empty[parity]);
+      v += s;
       if (p.epi == FLUXB_EPI_GELU) v = gelu_tanh(v);
-      p.y[m * p.ldy + n] = __float2bfloat16_rn(v);
+      if (mine) p.y[m * p.ldy + n] = __float2bfloat16_rn(v);
+      if ((parity ^= 1) == 0) red_phase ^= 1;
     }
-    buf ^= 1;
+    return;
+  }
+  const int g = lane >> 2, t4 = lane & 3;
+  const int steps = p.piece / (WARPS * 32);  // of 32 columns per warp and piece, at most four
+  const int col = warp * (p.piece / WARPS) + t4 * 8;
+  const __nv_bfloat16* xr = p.x + g * p.ldx;
+  auto load_x = [&](int piece, int s) {
+    const int k = piece * p.piece + col + s * 32;
+    return g < p.M && s < steps && k < p.K ? __ldg(reinterpret_cast<const uint4*>(xr + k)) : make_uint4(0, 0, 0, 0);
+  };
+  uint4 bx[kPieces > 0 ? kPieces : 1][4];
+  if (kPieces > 0) {
+#pragma unroll
+    for (int q = 0; q < kPieces; ++q)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) bx[q][s] = load_x(q, s);
+  }
+  int parity = 0;
+  uint32_t red_phase = 0;
+  for (int tile = blockIdx.x; tile < p.tiles; tile += gridDim.x) {
+    float c[4] = {};
+    auto work = [&](int piece, const uint4 (&b)[4]) -> bool {
+      if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[slot], phase, abort_flag, p.status, 86))) return false;
+      const uint8_t* base = ring + slot * slot_bytes + g * pitch + col * 2;
+      const bool whole = (piece + 1) * p.piece <= p.K;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        if (s < steps) {
+          uint4 a0 = *reinterpret_cast<const uint4*>(base + s * 64);
+          uint4 a1 = *reinterpret_cast<const uint4*>(base + 8 * pitch + s * 64);
+          if (!whole && piece * p.piece + col + s * 32 >= p.K) a0 = a1 = make_uint4(0, 0, 0, 0);  // behind the copy
+          mma_16x8x16(c, a0.x, a1.x, a0.y, a1.y, b[s].x, b[s].y);
+          mma_16x8x16(c, a0.z, a1.z, a0.w, a1.w, b[s].z, b[s].w);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty_bar[slot]);
+      if (++slot == p.slots) { slot = 0; phase ^= 1; }
+      return true;
+    };
+    bool ok = true;
+    if (kPieces > 0) {
+#pragma unroll
+      for (int q = 0; q < kPieces; ++q) ok = ok && work(q, bx[q]);
+    } else {
+      for (int q = 0; ok && q < p.pieces; ++q) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) bx[0][s] = load_x(q, s);
+        ok = work(q, bx[0]);
+      }
+    }
+    ok = ok && __all_sync(0xffffffffu, mbar_wait(&red_empty[parity], red_phase ^ 1, abort_flag, p.status, 87));
+    if (!ok) return;
+    red[parity][warp][g][2 * t4] = c[0];
+    red[parity][warp][g][2 * t4 + 1] = c[1];
+    red[parity][warp][g + 8][2 * t4] = c[2];
+    red[parity][warp][g + 8][2 * t4 + 1] = c[3];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&red_full[parity]);
+    if ((parity ^= 1) == 0) red_phase ^= 1;
   }
 }
 
 }  // namespace rows
 
 static int launch_rows(const fluxb_linear_problem& a, int64_t N, int64_t K, int epi, const void* t, const void* lora_b,
-                       int64_t R, int64_t ldb, const RequestAdapters& req, cudaStream_t st) {
-  rows::Params p;
+                       const LowRank& low, int64_t ldb, const RequestAdapters& req, cudaStream_t st) {
+  using namespace rows;
+  Params p;
   typedef const __nv_bfloat16* P;
   p.x = static_cast<P>(a.x); p.w = static_cast<P>(a.w); p.bias = static_cast<P>(a.bias); p.t = static_cast<P>(t);
   p.lora_b = static_cast<P>(lora_b);
   p.y = static_cast<__nv_bfloat16*>(a.y);
   p.req = req;
+  p.low = low;
   p.ldx = a.ldx; p.ldw = a.ldw; p.ldy = a.ldy; p.ldb = ldb;
-  p.M = (int)a.M; p.N = (int)N; p.K = (int)K; p.R = (int)R; p.rpad = (int)((R + 15) / 16 * 16); p.epi = epi;
+  p.M = (int)a.M; p.N = (int)N; p.K = (int)K; p.epi = epi;
   p.tiles = (int)((N + 15) / 16);
-  int warps = (int)((K + rows::SLICE - 1) / rows::SLICE);
-  if (warps > rows::MAX_WARPS) warps = rows::MAX_WARPS;
-  p.slices = (int)((K + rows::SLICE * warps - 1) / (rows::SLICE * warps));
-  // every block the same number of tiles, eight warps per SM
-  const int most = sm_count() * (rows::MAX_WARPS / warps);
-  const int per = (p.tiles + most - 1) / most;
+  p.piece = K < PIECE ? (int)((K + 255) / 256 * 256) : PIECE;
+  p.pieces = (int)((K + p.piece - 1) / p.piece);
+  p.status = device_status_ptr();
+  const int slot_bytes = 16 * (p.piece * 2 + 64);
+  // every block the same number of tiles
+  const int per = (p.tiles + sm_count() - 1) / sm_count();
   const int grid = (p.tiles + per - 1) / per;
-  if (p.slices == 1) rows::lora_rows_kernel<true><<<grid, warps * 32, 0, st>>>(p);
-  else rows::lora_rows_kernel<false><<<grid, warps * 32, 0, st>>>(p);
+  p.slots = RING_BYTES / slot_bytes;
+  if (p.slots > MAX_SLOTS) p.slots = MAX_SLOTS;
+  if (p.slots > per * p.pieces) p.slots = per * p.pieces;
+  auto kern = p.pieces == 1   ? lora_rows_kernel<1>
+              : p.pieces == 2 ? lora_rows_kernel<2>
+              : p.pieces == 3 ? lora_rows_kernel<3>
+              : p.pieces == 4 ? lora_rows_kernel<4>
+                              : lora_rows_kernel<0>;  // (the fragments of more pieces spill)
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES);
+  if (e != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "linear_lora: cannot set shared memory size: %s", cudaGetErrorString(e));
+  e = launch_after(kern, grid, THREADS, (size_t)p.slots * slot_bytes, st, p);
+  if (e != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "linear_lora: launch failed: %s", cudaGetErrorString(e));
   return FLUXB_OK;
 }
 
@@ -377,7 +584,7 @@ using namespace fluxb;
 
 extern "C" int64_t fluxb_linear_lora_scratch_bytes(int64_t M, int64_t N, int64_t K, int64_t R) {
   (void)N; (void)K;
-  return M <= 0 || R <= 0 ? 0 : M * ((R + 15) / 16) * 64;
+  return M <= 0 || R <= 0 ? 0 : M * LowRank(R).ld() * 2;
 }
 
 extern "C" int fluxb_linear_lora(const void* x, const void* w, const void* bias, void* y, const void* lora_a,
@@ -399,13 +606,15 @@ extern "C" int fluxb_linear_lora(const void* x, const void* w, const void* bias,
     return set_error(FLUXB_ERR_BAD_ARG, "linear_lora: pointers must be 16-byte aligned");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const RequestAdapters req{adapter, adapter_is64, (int)L, (int)n_adapters};
-  int rc = launch_shrink(x, ldx, lora_a, lora_scale, scratch, req, B, L, K, R, st);
+  const LowRank low(R);
+  int rc = L <= shrink::SHORT ? launch_shrink_short(x, ldx, lora_a, lora_scale, scratch, req, B, K, low, st)
+                              : launch_shrink(x, ldx, lora_a, lora_scale, scratch, req, B, L, K, low, st);
   if (rc != FLUXB_OK) return rc;
   fluxb_linear_problem a = {};
   a.x = x; a.w = w; a.bias = bias; a.y = y; a.M = B * L; a.ldx = ldx; a.ldw = ldw; a.ldy = ldy;
   a.rows_per_batch = 1;
-  rc = a.M <= 8 ? launch_rows(a, N, K, epi, scratch, lora_b, R, ldb, req, st)
-                : launch_lora_gemm(a, N, K, epi, scratch, lora_b, R, ldb, req, st);
+  rc = a.M <= 8 ? launch_rows(a, N, K, epi, scratch, lora_b, low, ldb, req, st)
+                : launch_lora_gemm(a, N, K, epi, scratch, lora_b, low, ldb, req, st);
   if (rc != FLUXB_OK) return rc;
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "linear_lora: launch failed: %s", cudaGetErrorString(e));

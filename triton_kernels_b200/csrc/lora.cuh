@@ -22,7 +22,28 @@ struct RequestAdapters {
   __device__ __forceinline__ int of_row(int row) const { return of_request(row / length); }
 };
 
+// Layout of the low-rank rows t: ranks in groups of 16, 32 or 64 (the smallest that holds R, else 64), each group as
+// its high parts, then its low parts: a group of 16 is a 64-byte line, of 32 a 128-byte line, of 64 two of them.  TMA
+// moves a line of up to 128 bytes per request, so wide lines matter: with 16-rank pieces throughout (64- and 32-byte
+// lines) the adapters cost the joint q|k|v projection at rank 128 20 % of its time.
+struct LowRank {
+  int R, units, group, groups;  // units: sixteens of ranks in use
+  explicit LowRank(int64_t rank = 16)
+      : R((int)rank), units((int)((rank + 15) / 16)), group(rank <= 16 ? 16 : (rank <= 32 ? 32 : 64)),
+        groups((int)((rank + group - 1) / group)) {}
+  __host__ __device__ int ld() const { return groups * group * 2; }  // elements per row of t
+  __device__ __forceinline__ int column(int rank) const { return rank / group * 2 * group + rank % group; }  // of its high part
+  // Shared-memory tiles of one group, 128 rows: one tile of `group` * 4 bytes a row, or two of 128 bytes (high, low).
+  __device__ __forceinline__ int tile_bytes() const { return group * 512; }
+  __device__ __forceinline__ uint64_t desc(uint32_t saddr) const {
+    return group == 16 ? make_smem_desc(saddr, 16, 512, 4) : make_smem_desc(saddr, 16, 1024);
+  }
+  // Where unit i of a group lies, in 16-byte steps: high parts and low parts
+  __device__ __forceinline__ int high(int i) const { return 2 * i; }
+  __device__ __forceinline__ int low(int i) const { return 2 * i + (group == 64 ? 1024 : group / 8); }
+};
+
 int launch_lora_gemm(const fluxb_linear_problem& a, int64_t N, int64_t K, int epi, const void* t, const void* lora_b,
-                     int64_t R, int64_t ldb, const RequestAdapters& req, cudaStream_t st);
+                     const LowRank& low, int64_t ldb, const RequestAdapters& req, cudaStream_t st);
 
 }  // namespace fluxb
