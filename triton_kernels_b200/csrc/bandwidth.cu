@@ -16,6 +16,7 @@
 
 #include <mutex>
 
+#include "norm.cuh"
 #include "vec.cuh"
 
 namespace fluxb {
@@ -46,11 +47,20 @@ struct RowAddr {
   }
 };
 
+// What a row norm does with its per-column vectors.
+enum Norm {
+  kRms = 0,       // x rstd scale
+  kModulated = 1, // h (1 + scale) + shift
+  kAffine = 2     // h scale + shift (LayerNorm with a learned scale)
+};
+template <int kNorm>
+__device__ __forceinline__ float scale_of(float a) { return kNorm == kAffine ? a : 1.0f + a; }
+
 // ----------------------------------------------------------------------------------------
 // LayerNorm (no affine) + modulation.  G lanes own one row; each lane holds VPL vectors.
 // cols == G * VPL * Vec<T>::N.
 // ----------------------------------------------------------------------------------------
-template <typename T, int G, int VPL>
+template <typename T, int G, int VPL, int kNorm>
 __global__ void __launch_bounds__(256, (VPL <= 12 ? 3 : (VPL <= 24 ? 2 : 1)))
 ln_mod_rows_kernel(const T* __restrict__ x, const T* __restrict__ scale, const T* __restrict__ shift,
                    T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t rows, int cols,
@@ -107,13 +117,13 @@ ln_mod_rows_kernel(const T* __restrict__ x, const T* __restrict__ scale, const T
     a.load_nc(sc + c);
     d.load_nc(sh + c);
 #pragma unroll
-    for (int j = 0; j < VN; ++j) t.v[j] = (t.v[j] - mean) * rstd * (1.0f + a.v[j]) + d.v[j];
+    for (int j = 0; j < VN; ++j) t.v[j] = (t.v[j] - mean) * rstd * scale_of<kNorm>(a.v[j]) + d.v[j];
     if (active) t.store(yr + c);
   }
 }
 
 // Any cols (multiple of the vector width): one warp per row, three passes over the row.
-template <typename T>
+template <typename T, int kNorm>
 __global__ void __launch_bounds__(256)
 ln_mod_generic_kernel(const T* __restrict__ x, const T* __restrict__ scale,
                       const T* __restrict__ shift, T* __restrict__ y, float* __restrict__ mean_out,
@@ -154,7 +164,7 @@ ln_mod_generic_kernel(const T* __restrict__ x, const T* __restrict__ scale,
     a.load_nc(sc + c);
     d.load_nc(sh + c);
 #pragma unroll
-    for (int j = 0; j < VN; ++j) t.v[j] = (t.v[j] - mean) * rstd * (1.0f + a.v[j]) + d.v[j];
+    for (int j = 0; j < VN; ++j) t.v[j] = (t.v[j] - mean) * rstd * scale_of<kNorm>(a.v[j]) + d.v[j];
     t.store(yr + c);
   }
 }
@@ -177,14 +187,6 @@ ln_mod_generic_kernel(const T* __restrict__ x, const T* __restrict__ scale,
 // element of the row keeps the subtraction benign when |mean| >> std (the plain
 // E[x^2] - mean^2 form is not).
 // ----------------------------------------------------------------------------------------
-__device__ __forceinline__ void bulk_load_row(void* smem_dst, const void* gsrc, uint32_t bytes, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-      :
-      : "r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(gsrc)), "r"(bytes), "r"(smem_u32(bar))
-      : "memory");
-}
-
 // Waits (bounded) for a staged copy.  If the copy never lands the row stays unwritten, so the
 // give-up is recorded in the device status word like every other bounded wait (site 71).
 __device__ __forceinline__ bool wait_row(uint64_t* bar, DeviceStatus* status) {
@@ -196,13 +198,14 @@ __device__ __forceinline__ bool wait_row(uint64_t* bar, DeviceStatus* status) {
 
 constexpr int kBulkHeaderBytes = 256;  // mbarriers: one per warp (up to 16) + one for the vectors
 
-template <typename T, bool kLayerNorm, bool kStagedMod, int kVPL>
+template <typename T, int kNorm, bool kStagedMod, int kVPL>
 __global__ void __launch_bounds__(512, 2)
 norm_rows_bulk_kernel(const T* __restrict__ x, const T* __restrict__ scale, const T* __restrict__ shift,
                       T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t rows, int cols,
                       int64_t rows_per_batch, RowAddr xaddr, int64_t y_ld, int64_t mod_stride, float eps,
                       DeviceStatus* status) {
   constexpr int VN = Vec<T>::N;
+  constexpr bool kLayerNorm = kNorm != kRms;
   constexpr int kModVecs = kLayerNorm ? 2 : 1;
   extern __shared__ __align__(128) uint8_t bulk_smem[];
   const int warp = threadIdx.x >> 5;
@@ -243,10 +246,12 @@ norm_rows_bulk_kernel(const T* __restrict__ x, const T* __restrict__ scale, cons
   const int nvec = kVPL > 0 ? kVPL * 32 : cols / VN;
   float mean = 0.f, rstd;
   if (kLayerNorm) {
-    // 16-bit rows need no shift: their own quantisation (2^-9 of |x|) is 64 times the fp32
-    // cancellation error of the unshifted form at any mean/std ratio.
+    // The modulated form does not shift 16-bit rows: their own quantisation (2^-9 of |x|) is 64 times
+    // the fp32 cancellation error of the unshifted form at any mean/std ratio of rows that vary from
+    // element to element.  The affine form shifts every type.
+    constexpr bool kShift = sizeof(T) > 2 || kNorm == kAffine;
     float pivot = 0.f;
-    if (sizeof(T) > 2) {
+    if (kShift) {
       Vec<T> first;
       first.load(srow);
       pivot = first.v[0];
@@ -258,7 +263,7 @@ norm_rows_bulk_kernel(const T* __restrict__ x, const T* __restrict__ scale, cons
       t.load(srow + i * VN);
 #pragma unroll
       for (int j = 0; j < VN; ++j) {
-        const float d = sizeof(T) > 2 ? t.v[j] - pivot : t.v[j];
+        const float d = kShift ? t.v[j] - pivot : t.v[j];
         s += d;
         q = fmaf(d, d, q);
       }
@@ -303,7 +308,7 @@ norm_rows_bulk_kernel(const T* __restrict__ x, const T* __restrict__ scale, cons
         d.load_nc(sh + i * VN);
       }
 #pragma unroll
-      for (int j = 0; j < VN; ++j) t.v[j] = fmaf(fmaf(t.v[j], rstd, neg_mean_rstd), 1.0f + a.v[j], d.v[j]);
+      for (int j = 0; j < VN; ++j) t.v[j] = fmaf(fmaf(t.v[j], rstd, neg_mean_rstd), scale_of<kNorm>(a.v[j]), d.v[j]);
       t.store(srow + i * VN);
     }
   } else {
@@ -337,16 +342,16 @@ static inline bool bulk_rows_ok(int64_t cols, size_t elt, const RowAddr& a) {
   return (a.s0 * (int64_t)elt) % 16 == 0 && (a.s1 * (int64_t)elt) % 16 == 0 && (a.s2 * (int64_t)elt) % 16 == 0;
 }
 
-template <typename T, bool kLayerNorm, bool kStagedMod>
+template <typename T, int kNorm, bool kStagedMod>
 static int launch_norm_bulk_as(const T* x, const T* scale, const T* shift, T* y, float* mean, float* rstd, int64_t rows,
                                int64_t cols, int64_t rpb, RowAddr xaddr, int64_t y_ld, int64_t mod_stride,
                                float eps, cudaStream_t st) {
   const int warps = kStagedMod ? 16 : 8;
-  const size_t smem = kBulkHeaderBytes + ((kStagedMod ? (kLayerNorm ? 2 : 1) : 0) + warps) * (size_t)cols * sizeof(T);
+  const size_t smem = kBulkHeaderBytes + ((kStagedMod ? (kNorm != kRms ? 2 : 1) : 0) + warps) * (size_t)cols * sizeof(T);
   // Rows of 12 vectors per lane (3072 bf16 columns, the Flux hidden size) get the unrolled form.
   constexpr int kUnrolled = 12;
-  auto kern = cols == kUnrolled * 32 * Vec<T>::N ? norm_rows_bulk_kernel<T, kLayerNorm, kStagedMod, kUnrolled>
-                                                 : norm_rows_bulk_kernel<T, kLayerNorm, kStagedMod, 0>;
+  auto kern = cols == kUnrolled * 32 * Vec<T>::N ? norm_rows_bulk_kernel<T, kNorm, kStagedMod, kUnrolled>
+                                                 : norm_rows_bulk_kernel<T, kNorm, kStagedMod, 0>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess)
     return set_error(FLUXB_ERR_CUDA, "row norm: cannot set shared memory size: %s", cudaGetErrorString(e));
@@ -357,22 +362,22 @@ static int launch_norm_bulk_as(const T* x, const T* scale, const T* shift, T* y,
 
 // Rows of up to 6 KB whose blocks of 16 rows each stay inside one batch element, with 16-byte
 // aligned per-column vectors, take the form that stages those vectors in shared memory.
-template <typename T, bool kLayerNorm>
+template <typename T, int kNorm>
 static int launch_norm_bulk(const T* x, const T* scale, const T* shift, T* y, float* mean, float* rstd, int64_t rows,
                             int64_t cols, int64_t rpb, RowAddr xaddr, int64_t y_ld, int64_t mod_stride, float eps,
                             cudaStream_t st) {
   const bool aligned = (reinterpret_cast<uintptr_t>(scale) & 15) == 0 &&
-                       (!kLayerNorm || ((reinterpret_cast<uintptr_t>(shift) & 15) == 0 &&
+                       (kNorm == kRms || ((reinterpret_cast<uintptr_t>(shift) & 15) == 0 &&
                                         (mod_stride * (int64_t)sizeof(T)) % 16 == 0));
-  const bool one_batch_per_block = !kLayerNorm || rpb % 16 == 0 || rows <= rpb;
+  const bool one_batch_per_block = kNorm == kRms || rpb % 16 == 0 || rows <= rpb;
   if (cols * (int64_t)sizeof(T) <= 6144 && aligned && one_batch_per_block)
-    return launch_norm_bulk_as<T, kLayerNorm, true>(x, scale, shift, y, mean, rstd, rows, cols, rpb, xaddr, y_ld,
+    return launch_norm_bulk_as<T, kNorm, true>(x, scale, shift, y, mean, rstd, rows, cols, rpb, xaddr, y_ld,
                                                     mod_stride, eps, st);
-  return launch_norm_bulk_as<T, kLayerNorm, false>(x, scale, shift, y, mean, rstd, rows, cols, rpb, xaddr, y_ld,
+  return launch_norm_bulk_as<T, kNorm, false>(x, scale, shift, y, mean, rstd, rows, cols, rpb, xaddr, y_ld,
                                                    mod_stride, eps, st);
 }
 
-template <typename T>
+template <typename T, int kNorm>
 static int launch_ln_mod(const void* x, const void* scale, const void* shift, void* y, float* mean, float* rstd,
                          int64_t rows, int64_t cols, int64_t rpb, int64_t x_ld, int64_t y_ld, int64_t mod_stride,
                          float eps, cudaStream_t st) {
@@ -385,13 +390,13 @@ static int launch_ln_mod(const void* x, const void* scale, const void* shift, vo
   {
     RowAddr xaddr{1, rows > 0 ? rows : 1, 0, 0, x_ld, 1};
     if (bulk_rows_ok(cols, sizeof(T), xaddr) && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
-      return launch_norm_bulk<T, true>(xp, sc, sh, yp, mean, rstd, rows, cols, rpb, xaddr, y_ld, mod_stride, eps, st);
+      return launch_norm_bulk<T, kNorm>(xp, sc, sh, yp, mean, rstd, rows, cols, rpb, xaddr, y_ld, mod_stride, eps, st);
     }
   }
 #define FLUXB_LN_CASE(G, VPL)                                                                  \
   if (vecs == (G) * (VPL)) {                                                                   \
     const int64_t gpb = 256 / (G);                                                             \
-    ln_mod_rows_kernel<T, G, VPL><<<(unsigned)((rows + gpb - 1) / gpb), 256, 0, st>>>(         \
+    ln_mod_rows_kernel<T, G, VPL, kNorm><<<(unsigned)((rows + gpb - 1) / gpb), 256, 0, st>>>(         \
         xp, sc, sh, yp, mean, rstd, rows, (int)cols, rpb, x_ld, y_ld, mod_stride, eps);        \
     return FLUXB_OK;                                                                           \
   }
@@ -399,9 +404,16 @@ static int launch_ln_mod(const void* x, const void* scale, const void* shift, vo
   FLUXB_LN_CASE(32, 6) FLUXB_LN_CASE(32, 8) FLUXB_LN_CASE(32, 12) FLUXB_LN_CASE(32, 16)
   FLUXB_LN_CASE(32, 24)
 #undef FLUXB_LN_CASE
-  ln_mod_generic_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(
+  ln_mod_generic_kernel<T, kNorm><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(
       xp, sc, sh, yp, mean, rstd, rows, (int)cols, rpb, x_ld, y_ld, mod_stride, eps);
   return FLUXB_OK;
+}
+
+int launch_layer_norm_affine(const void* x, const void* factor, const void* offset, void* y, float* mean, float* rstd,
+                             int64_t rows, int64_t cols, int64_t x_ld, int64_t y_ld, float eps, int dtype, cudaStream_t st) {
+  return dtype == FLUXB_BF16
+             ? launch_ln_mod<__nv_bfloat16, kAffine>(x, factor, offset, y, mean, rstd, rows, cols, rows, x_ld, y_ld, 0, eps, st)
+             : launch_ln_mod<float, kAffine>(x, factor, offset, y, mean, rstd, rows, cols, rows, x_ld, y_ld, 0, eps, st);
 }
 
 // ----------------------------------------------------------------------------------------
@@ -523,7 +535,7 @@ static int launch_rms(const void* x, const void* w, void* y, float* rstd, int64_
   T* yp = static_cast<T*>(y);
   const int64_t vecs = cols / VN;
   if (bulk_rows_ok(cols, sizeof(T), addr) && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
-    return launch_norm_bulk<T, false>(xp, wp, nullptr, yp, nullptr, rstd, rows, cols, 1, addr, cols, 0, eps, st);
+    return launch_norm_bulk<T, kRms>(xp, wp, nullptr, yp, nullptr, rstd, rows, cols, 1, addr, cols, 0, eps, st);
   }
 #define FLUXB_RMS_CASE(G, VPL)                                                                 \
   if (vecs == (G) * (VPL)) {                                                                   \
@@ -1166,9 +1178,9 @@ static int layer_norm_modulation_impl(const void* x, const void* scale, const vo
                      "pointers 16-byte aligned", vn);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int rc = dtype == FLUXB_BF16
-                     ? launch_ln_mod<__nv_bfloat16>(x, scale, shift, y, mean, rstd, rows, cols, rows_per_batch, x_ld,
+                     ? launch_ln_mod<__nv_bfloat16, kModulated>(x, scale, shift, y, mean, rstd, rows, cols, rows_per_batch, x_ld,
                                                     y_ld, mod_stride, eps, st)
-                     : launch_ln_mod<float>(x, scale, shift, y, mean, rstd, rows, cols, rows_per_batch, x_ld, y_ld,
+                     : launch_ln_mod<float, kModulated>(x, scale, shift, y, mean, rstd, rows, cols, rows_per_batch, x_ld, y_ld,
                                             mod_stride, eps, st);
   if (rc != FLUXB_OK) return rc;
   return launch_status("layer_norm_modulation");

@@ -28,6 +28,7 @@ struct RopeAxesArgs {
   const void* ids;
   int64_t id_sb, id_sl, id_sa;
   int64_t B, L;
+  int groups;    // of heads, one per blockIdx.y
   int D, pairs;  // pairs <= D/2; the columns from 2*pairs on are copied
   float sign;    // +1 forward, -1 backward
   double turns[kMaxPairs];
@@ -44,7 +45,68 @@ __device__ __forceinline__ float2 turn_of(const RopeAxesArgs& a, int64_t b, int6
   return make_float2(c, a.sign * s);
 }
 
-// One thread per (token, pair or trailing element pair), over all heads of q and k.
+// Rows of whole 16-byte pieces: a thread owns one piece of one token's rows and walks heads of q and k, so its sines and
+// cosines stay in registers for all of them and no table is read or written; eight pieces are in flight per thread,
+// the first eight while the angles are taken.  The heads are dealt to blockIdx.y when there are few tokens.  Bound by
+// HBM: every element is read once and written once.
+template <typename T, typename Id>
+__global__ void __launch_bounds__(256) rope_axes_vec_kernel(const __grid_constant__ RopeAxesArgs a) {
+  constexpr int VN = Vec<T>::N;
+  constexpr int kAhead = 8;
+  const int pieces = a.D / VN;
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= (int)(a.B * a.L) * pieces) return;
+  const int tok = i / pieces, piece = i - tok * pieces;
+  const int b = tok / (int)a.L, l = tok - b * (int)a.L;
+  const int heads = a.t[0].heads + a.t[1].heads;
+  const int h0 = (int)((int64_t)blockIdx.y * heads / a.groups), h1 = (int)((int64_t)(blockIdx.y + 1) * heads / a.groups);
+  const T* src[2];
+  T* dst[2];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    src[w] = static_cast<const T*>(a.t[w].src) + b * a.t[w].sb + l * a.t[w].sl + piece * VN;
+    dst[w] = static_cast<T*>(a.t[w].dst) + b * a.t[w].ob + l * a.t[w].ol + piece * VN;
+  }
+  const int hq = a.t[0].heads;
+  uint4 raw[kAhead];
+  auto ask = [&](int h) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (h + u < h1) raw[u] = ld_nc_u4(h + u < hq ? src[0] + (h + u) * a.t[0].sh : src[1] + (h + u - hq) * a.t[1].sh);
+    }
+  };
+  ask(h0);
+  const int j0 = piece * (VN / 2);
+  float2 cs[VN / 2];
+#pragma unroll
+  for (int p = 0; p < VN / 2; ++p) cs[p] = j0 + p < a.pairs ? turn_of<Id>(a, b, l, j0 + p) : make_float2(1.f, 0.f);
+  for (int h = h0; h < h1; h += kAhead) {
+    if (h > h0) ask(h);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (h + u < h1) {
+        T* out = h + u < hq ? dst[0] + (h + u) * a.t[0].oh : dst[1] + (h + u - hq) * a.t[1].oh;
+        if (j0 >= a.pairs) {  // behind the axes: copied
+          *reinterpret_cast<uint4*>(out) = raw[u];
+          continue;
+        }
+        Vec<T> v;
+        v.unpack(raw[u]);
+#pragma unroll
+        for (int p = 0; p < VN / 2; ++p) {
+          if (j0 + p < a.pairs) {
+            const float x0 = v.v[2 * p], x1 = v.v[2 * p + 1];
+            v.v[2 * p] = x0 * cs[p].x - x1 * cs[p].y;
+            v.v[2 * p + 1] = x0 * cs[p].y + x1 * cs[p].x;
+          }
+        }
+        v.store(out);
+      }
+    }
+  }
+}
+
+// Any other layout.  One thread per (token, pair or trailing element pair), over all heads of q and k.
 template <typename T, typename Id>
 __global__ void __launch_bounds__(256) rope_axes_any_kernel(const __grid_constant__ RopeAxesArgs a) {
   const int half = (a.D + 1) / 2;
@@ -123,6 +185,35 @@ extern "C" int fluxb_rope_axes(const void* q, void* oq, const int64_t* q_strides
       a.axis[p] = (uint8_t)i;
     }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int vn = dtype == FLUXB_BF16 ? 8 : 4;
+  const int64_t vthreads = B * L * (D / vn);
+  bool whole = D % vn == 0 && vthreads <= INT32_MAX - 256;
+  for (const RopeTensor& t : a.t) {
+    if (t.heads == 0) continue;
+    whole = whole && ((reinterpret_cast<uintptr_t>(t.src) | reinterpret_cast<uintptr_t>(t.dst)) & 15u) == 0;
+    for (int64_t s : {t.sb, t.sh, t.sl, t.ob, t.oh, t.ol}) whole = whole && s % vn == 0;
+  }
+  if (whole) {
+    // heads are split until there are about four blocks per SM, as long as a thread keeps eight
+    const int64_t blocks = (vthreads + 255) / 256, heads = Hq + Hk;
+    int64_t groups = 4 * sm_count() / blocks;
+    if (groups > heads / 8) groups = heads / 8;
+    if (groups < 1) groups = 1;
+    a.groups = (int)groups;
+    const dim3 vgrid((unsigned)blocks, (unsigned)groups);
+#define FLUXB_ROPE_AXES(T)                                                                    \
+  do {                                                                                        \
+    if (id_type == FLUXB_ID_F32) rope_axes_vec_kernel<T, float><<<vgrid, 256, 0, st>>>(a);    \
+    else if (id_type == FLUXB_ID_I32) rope_axes_vec_kernel<T, int><<<vgrid, 256, 0, st>>>(a); \
+    else rope_axes_vec_kernel<T, long long><<<vgrid, 256, 0, st>>>(a);                        \
+  } while (0)
+    if (dtype == FLUXB_BF16) FLUXB_ROPE_AXES(__nv_bfloat16);
+    else FLUXB_ROPE_AXES(float);
+#undef FLUXB_ROPE_AXES
+    cudaError_t ve = cudaGetLastError();
+    if (ve != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "rope_axes: %s", cudaGetErrorString(ve));
+    return FLUXB_OK;
+  }
   const unsigned grid = (unsigned)((B * L * half + 255) / 256);
 #define FLUXB_ROPE_AXES(T)                                                               \
   do {                                                                                   \

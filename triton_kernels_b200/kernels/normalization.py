@@ -26,14 +26,19 @@ def layer_norm_modulation_into(x2d, scale2d, shift2d, y2d, rows_per_batch: int, 
     )
 
 
+def _dense16(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous and 16-byte aligned; a copy where it is not."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
 def _rows(x: torch.Tensor) -> torch.Tensor:
-    """x as [rows, C] with unit column stride; a view where the rows are evenly spaced."""
+    """x as [rows, C] with unit column stride and 16-byte aligned rows (of whole 16-byte pieces); a
+    view where the rows are evenly spaced."""
     C = x.shape[-1]
-    if x.is_contiguous():
-        return x.view(-1, C)
-    if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= C:
+    if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= C and x.stride(0) % _vec(x) == 0 and x.data_ptr() % 16 == 0:
         return x
-    return x.contiguous().view(-1, C)
+    return _dense16(x).view(-1, C)
 
 
 def _norm_backward(dy, x2, factor2, mean, rstd, unit: float, groups: int, want_dx: bool, want_sums: bool, grads_dtype):
@@ -93,7 +98,7 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x2, weight, mean, rstd = ctx.saved_tensors
         need_x, need_w, need_b, _ = ctx.needs_input_grad
-        dx, dw, db = _norm_backward(dy, x2, weight[None] if weight is not None else None, mean, rstd, 0.0, 1, need_x,
+        dx, dw, db = _norm_backward(dy, x2, weight[None], mean, rstd, 0.0, 1, need_x,
                                     need_w or need_b, x2.dtype)
         return dx.view(ctx.shape) if need_x else None, dw[0] if need_w else None, db[0] if need_b else None, None
 
@@ -112,7 +117,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
             assert p.shape == x.shape[-1:], "weight and bias are vectors of x's last dim"
             assert p.dtype == x.dtype, "Incompatible dtypes"
     _lib.dtype_code(x)
-    weight, bias = (p if p is None or p.is_contiguous() else p.contiguous() for p in (weight, bias))
+    C = x.shape[-1:]
+    weight = torch.ones(C, device=x.device, dtype=x.dtype) if weight is None else _dense16(weight)
+    bias = torch.zeros(C, device=x.device, dtype=x.dtype) if bias is None else _dense16(bias)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return _LayerNorm.apply(x, weight, bias, eps)
     return _layer_norm_forward(x, weight, bias, eps, False)[1]
