@@ -201,6 +201,83 @@ __global__ void __launch_bounds__(256) ln_fwd_block_kernel(const LnArgs a) {
   }
 }
 
+// Sixteen bytes as pairs of fp32: the backward kernels work on pairs (one instruction for two columns), because with
+// one column at a time they were bound by the instructions that they issued, not by memory.
+template <typename T>
+struct Pairs {
+  static constexpr int N = 8 / sizeof(T);
+  float2 v[N];
+  __device__ __forceinline__ void unpack(const uint4& t) {
+    if constexpr (sizeof(T) == 2) {
+      v[0] = make_float2(bf16_lo(t.x), bf16_hi(t.x)); v[1] = make_float2(bf16_lo(t.y), bf16_hi(t.y));
+      v[2] = make_float2(bf16_lo(t.z), bf16_hi(t.z)); v[3] = make_float2(bf16_lo(t.w), bf16_hi(t.w));
+    } else {
+      v[0] = make_float2(__uint_as_float(t.x), __uint_as_float(t.y));
+      v[1] = make_float2(__uint_as_float(t.z), __uint_as_float(t.w));
+    }
+  }
+  __device__ __forceinline__ uint4 pack() const {
+    if constexpr (sizeof(T) == 2)
+      return make_uint4(pack_bf16(v[0].x, v[0].y), pack_bf16(v[1].x, v[1].y), pack_bf16(v[2].x, v[2].y), pack_bf16(v[3].x, v[3].y));
+    else
+      return make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
+  }
+};
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// The widened factor in shared memory: the first four columns of every 16-byte piece, then (bf16) the other four, so
+// that neighbouring lanes read neighbouring float4s (in column order they would meet in the same banks).
+template <typename T>
+__device__ __forceinline__ void fill_factor(float* factor, const T* f, float unit, int cols) {
+  constexpr int VN = Vec<T>::N;
+  for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+    const int piece = c / VN, j = c % VN;
+    factor[(j / 4 * (cols / VN) + piece) * 4 + j % 4] = f != nullptr ? unit + to_f(f[c]) : 1.f;
+  }
+}
+
+// What a row's piece adds: h and g for dx, the two sums of the row, the column sums.
+template <typename T>
+__device__ __forceinline__ void bwd_piece(const uint4& xr, const uint4& dr, const float4* factor, int piece, int pieces,
+                                          float2 neg_mean, float2 rstd, Pairs<T>& g, Pairs<T>& h, float2& s1, float2& s2,
+                                          Pairs<T>& df, Pairs<T>& dof) {
+  Pairs<T> x, d;
+  x.unpack(xr);
+  d.unpack(dr);
+#pragma unroll
+  for (int q = 0; q < Pairs<T>::N / 2; ++q) {
+    const float4 f = factor[q * pieces + piece];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = 2 * q + e;
+      h.v[i] = __fmul2_rn(__fadd2_rn(x.v[i], neg_mean), rstd);
+      g.v[i] = __fmul2_rn(d.v[i], e == 0 ? make_float2(f.x, f.y) : make_float2(f.z, f.w));
+      s1 = __fadd2_rn(s1, g.v[i]);
+      s2 = __ffma2_rn(g.v[i], h.v[i], s2);
+      df.v[i] = __ffma2_rn(d.v[i], h.v[i], df.v[i]);
+      dof.v[i] = __fadd2_rn(dof.v[i], d.v[i]);
+    }
+  }
+}
+// rstd (g - mean(g) - h mean(g h)) with k1 = -rstd mean(g), k2 = -rstd mean(g h)
+template <typename T>
+__device__ __forceinline__ uint4 bwd_dx(const Pairs<T>& g, const Pairs<T>& h, float2 rstd, float2 k1, float2 k2) {
+  Pairs<T> o;
+#pragma unroll
+  for (int i = 0; i < Pairs<T>::N; ++i) o.v[i] = __ffma2_rn(h.v[i], k2, __ffma2_rn(g.v[i], rstd, k1));
+  return o.pack();
+}
+// Two sums over a warp at once: lanes 0-15 get the first one's total, lanes 16-31 the second one's.
+__device__ __forceinline__ float warp_sum_two(float2 s1, float2 s2, int lane) {
+  const float a = s1.x + s1.y, b = s2.x + s2.y;
+  const bool upper = (lane & 16) != 0;
+  float keep = upper ? b : a;
+  keep += __shfl_xor_sync(0xffffffffu, upper ? a : b, 16);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) keep += __shfl_xor_sync(0xffffffffu, keep, o);
+  return keep;
+}
+
 // Backward, one pass over x and dy: a team of `wpr` warps walks whole rows and keeps the column sums of its columns in
 // registers (kV 16-byte pieces per thread), so a row is read once and everything that it gives - dx, its share of df and
 // do - leaves from there.  The rows come through a ring in shared memory by bulk copies, one x row and one dy row a
@@ -208,117 +285,108 @@ __global__ void __launch_bounds__(256) ln_fwd_block_kernel(const LnArgs a) {
 // in the team: shuffles, then one named barrier, whose other side also frees the row's slot for the next copy.  The
 // factor is kept widened in shared memory.  At the end the block's teams add up their column sums in a fixed order and
 // the block writes one partial row; ln_bwd_reduce_kernel adds those.
-template <typename T, int kV>
+// kFull: the row is exactly kV pieces per thread.
+template <typename T, int kV, bool kFull>
 __global__ void __launch_bounds__(512, 1) ln_bwd_team_kernel(const LnBwdArgs a) {
   constexpr int VN = Vec<T>::N;
   extern __shared__ __align__(128) uint8_t dyn[];
   __shared__ uint64_t bars[kMaxTeamSlots];
-  __shared__ float2 red[2][16];
+  __shared__ float red[2][16][2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int team = warp / a.wpr, team_threads = a.wpr * 32, tid = threadIdx.x - team * team_threads;
-  const int64_t group = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+  const int group = blockIdx.x / a.parts, part = blockIdx.x - group * a.parts;
+  const int pieces = a.cols / VN, rows = (int)a.rows_per_group;
   const uint32_t row_bytes = (uint32_t)a.cols * sizeof(T);
-  float* factor = reinterpret_cast<float*>(dyn);  // [cols], then the teams' rings
-  uint8_t* ring = dyn + (size_t)(a.cols * 4 + 127) / 128 * 128 + (size_t)team * a.slots * 2 * row_bytes;
+  const float4* factor = reinterpret_cast<const float4*>(dyn);  // [cols] floats, then the teams' rings
+  uint8_t* ring = dyn + (a.cols * 4 + 127) / 128 * 128 + team * a.slots * 2 * row_bytes;
   uint64_t* full = bars + team * a.slots;
   if (tid == 0) {
     for (int i = 0; i < a.slots; ++i) mbar_init(&full[i], 1);
     mbar_fence_init();
     fence_proxy_async_smem();
   }
-  const T* x = static_cast<const T*>(a.x) + group * a.rows_per_group * a.x_ld;
-  const T* dy = static_cast<const T*>(a.dy) + group * a.rows_per_group * a.dy_ld;
-  const int64_t step = (int64_t)a.parts * a.teams;
-  const int64_t first = part * a.teams + team;
-  auto ask = [&](int64_t row, int slot) {
-    uint8_t* dst = ring + (size_t)slot * 2 * row_bytes;
+  const int64_t base = (int64_t)group * rows;
+  const T* x = static_cast<const T*>(a.x) + base * a.x_ld;
+  const T* dy = static_cast<const T*>(a.dy) + base * a.dy_ld;
+  const int step = a.parts * a.teams, first = part * a.teams + team;
+  auto ask = [&](int row, int slot) {
+    uint8_t* dst = ring + slot * 2 * row_bytes;
     mbar_expect_tx(&full[slot], 2 * row_bytes);
     bulk_load_row(dst, x + row * a.x_ld, row_bytes, &full[slot]);
     bulk_load_row(dst + row_bytes, dy + row * a.dy_ld, row_bytes, &full[slot]);
   };
   if (tid == 0) {
     for (int i = 0; i < a.slots; ++i)
-      if (first + i * step < a.rows_per_group) ask(first + i * step, i);
+      if (first + i * step < rows) ask(first + i * step, i);
   }
-  const T* fp = a.factor != nullptr ? static_cast<const T*>(a.factor) + group * a.vec_stride : nullptr;
-  for (int c = threadIdx.x; c < a.cols; c += blockDim.x) factor[c] = fp != nullptr ? a.unit + to_f(fp[c]) : 1.f;
+  fill_factor<T>(reinterpret_cast<float*>(dyn),
+                 a.factor != nullptr ? static_cast<const T*>(a.factor) + group * a.vec_stride : nullptr, a.unit, a.cols);
   __syncthreads();
 
-  float df[kV][VN], dof[kV][VN];
+  Pairs<T> df[kV], dof[kV];
 #pragma unroll
   for (int i = 0; i < kV; ++i)
 #pragma unroll
-    for (int j = 0; j < VN; ++j) df[i][j] = dof[i][j] = 0.f;
+    for (int j = 0; j < Pairs<T>::N; ++j) df[i].v[j] = dof[i].v[j] = both(0.f);
   const float inv_cols = 1.f / a.cols;
   int slot = 0, buf = 0;
   uint32_t phase = 0;
-  for (int64_t r = first; r < a.rows_per_group; r += step) {
-    const int64_t row = group * a.rows_per_group + r;
-    const float mean = __ldg(a.mean + row), rstd = __ldg(a.rstd + row);
-    bool ok = false;
+  const float *mean_p = a.mean + base + first, *rstd_p = a.rstd + base + first;
+  float next_mean = 0.f, next_rstd = 0.f;
+  if (first < rows) { next_mean = __ldg(mean_p); next_rstd = __ldg(rstd_p); }
+  T* dx = static_cast<T*>(a.dx) + (base + first) * a.dx_ld + tid * VN;
+  for (int r = first; r < rows; r += step) {
+    const float rstd = next_rstd;
+    const float2 neg_mean = both(-next_mean), rstd2 = both(rstd);
+    mean_p += step;
+    rstd_p += step;
+    if (r + step < rows) { next_mean = __ldg(mean_p); next_rstd = __ldg(rstd_p); }
+    bool ok = mbar_try_wait(&full[slot], phase);
     for (uint32_t spin = 0; spin < (1u << 24) && !ok; ++spin) ok = mbar_try_wait(&full[slot], phase);
     if (!ok) report_error(a.status, FLUXB_ERR_TIMEOUT, 72);  // carries on: the row's numbers are lost, nobody hangs
-    const T* xs = reinterpret_cast<const T*>(ring + (size_t)slot * 2 * row_bytes);
-    const T* ds = xs + a.cols;
-    float g[kV][VN], h[kV][VN];
-    float s1 = 0.f, s2 = 0.f;
+    const uint4* xs = reinterpret_cast<const uint4*>(ring + slot * 2 * row_bytes) + tid;
+    const uint4* ds = xs + pieces;
+    Pairs<T> g[kV], h[kV];
+    float2 s1 = both(0.f), s2 = both(0.f);
 #pragma unroll
     for (int i = 0; i < kV; ++i) {
-      const int c = (i * team_threads + tid) * VN;
-      if (c < a.cols) {
-        Vec<T> xv, dv;
-        xv.load(xs + c);
-        dv.load(ds + c);
-#pragma unroll
-        for (int j = 0; j < VN; ++j) {
-          h[i][j] = (xv.v[j] - mean) * rstd;
-          g[i][j] = dv.v[j] * factor[c + j];
-          s1 += g[i][j];
-          s2 = fmaf(g[i][j], h[i][j], s2);
-          df[i][j] = fmaf(dv.v[j], h[i][j], df[i][j]);
-          dof[i][j] += dv.v[j];
-        }
-      }
+      const int piece = i * team_threads + tid;
+      if (kFull || piece < pieces)
+        bwd_piece<T>(xs[i * team_threads], ds[i * team_threads], factor, piece, pieces, neg_mean, rstd2, g[i], h[i], s1, s2,
+                     df[i], dof[i]);
     }
-    s1 = warp_sum(s1);
-    s2 = warp_sum(s2);
-    if (lane == 0) red[buf][warp] = make_float2(s1, s2);
+    const float sum = warp_sum_two(s1, s2, lane);
+    if ((lane & 15) == 0) red[buf][warp][lane >> 4] = sum;
     asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(team_threads) : "memory");
-    if (tid == 0 && r + a.slots * step < a.rows_per_group) ask(r + a.slots * step, slot);
-    s1 = s2 = 0.f;
-    for (int w = 0; w < a.wpr; ++w) {
-      const float2 v = red[buf][team * a.wpr + w];
-      s1 += v.x;
-      s2 += v.y;
-    }
+    if (tid == 0 && r + a.slots * step < rows) ask(r + a.slots * step, slot);
+    float2 t = both(0.f);
+    for (int w = 0; w < a.wpr; ++w) t = __fadd2_rn(t, *reinterpret_cast<const float2*>(red[buf][team * a.wpr + w]));
     if (a.dx != nullptr) {
-      const float k1 = -s1 * inv_cols * rstd, k2 = -s2 * inv_cols * rstd;
-      T* dx = static_cast<T*>(a.dx) + row * a.dx_ld;
+      const float2 k1 = both(-t.x * inv_cols * rstd), k2 = both(-t.y * inv_cols * rstd);
 #pragma unroll
       for (int i = 0; i < kV; ++i) {
-        const int c = (i * team_threads + tid) * VN;
-        if (c < a.cols) {
-          Vec<T> o;
-#pragma unroll
-          for (int j = 0; j < VN; ++j) o.v[j] = fmaf(h[i][j], k2, fmaf(g[i][j], rstd, k1));
-          o.store(dx + c);
-        }
+        if (kFull || i * team_threads + tid < pieces)
+          *reinterpret_cast<uint4*>(dx + i * team_threads * VN) = bwd_dx<T>(g[i], h[i], rstd2, k1, k2);
       }
+      dx += step * a.dx_ld;
     }
     buf ^= 1;
     if (++slot == a.slots) { slot = 0; phase ^= 1; }
   }
   // the teams' column sums, added up by the first one; all copies have landed, the rings are free
-  float* other = reinterpret_cast<float*>(dyn + (size_t)(a.cols * 4 + 127) / 128 * 128);
+  float2* other = reinterpret_cast<float2*>(dyn + (a.cols * 4 + 127) / 128 * 128);  // [2][cols / 2]
   for (int t = 1; t < a.teams; ++t) {
     __syncthreads();
     if (team == t) {
 #pragma unroll
       for (int i = 0; i < kV; ++i) {
-        const int c = (i * team_threads + tid) * VN;
-        if (c < a.cols) {
+        const int piece = i * team_threads + tid;
+        if (kFull || piece < pieces) {
 #pragma unroll
-          for (int j = 0; j < VN; ++j) { other[c + j] = df[i][j]; other[a.cols + c + j] = dof[i][j]; }
+          for (int j = 0; j < Pairs<T>::N; ++j) {
+            other[j * pieces + piece] = df[i].v[j];
+            other[a.cols / 2 + j * pieces + piece] = dof[i].v[j];
+          }
         }
       }
     }
@@ -326,10 +394,13 @@ __global__ void __launch_bounds__(512, 1) ln_bwd_team_kernel(const LnBwdArgs a) 
     if (team == 0) {
 #pragma unroll
       for (int i = 0; i < kV; ++i) {
-        const int c = (i * team_threads + tid) * VN;
-        if (c < a.cols) {
+        const int piece = i * team_threads + tid;
+        if (kFull || piece < pieces) {
 #pragma unroll
-          for (int j = 0; j < VN; ++j) { df[i][j] += other[c + j]; dof[i][j] += other[a.cols + c + j]; }
+          for (int j = 0; j < Pairs<T>::N; ++j) {
+            df[i].v[j] = __fadd2_rn(df[i].v[j], other[j * pieces + piece]);
+            dof[i].v[j] = __fadd2_rn(dof[i].v[j], other[a.cols / 2 + j * pieces + piece]);
+          }
         }
       }
     }
@@ -338,12 +409,13 @@ __global__ void __launch_bounds__(512, 1) ln_bwd_team_kernel(const LnBwdArgs a) 
     float* out = a.partial + (int64_t)blockIdx.x * 2 * a.cols;
 #pragma unroll
     for (int i = 0; i < kV; ++i) {
-      const int c = (i * team_threads + tid) * VN;
-      if (c < a.cols) {
+      const int piece = i * team_threads + tid;
+      if (kFull || piece < pieces) {
 #pragma unroll
-        for (int j = 0; j < VN; j += 4) {
-          *reinterpret_cast<float4*>(out + c + j) = make_float4(df[i][j], df[i][j + 1], df[i][j + 2], df[i][j + 3]);
-          *reinterpret_cast<float4*>(out + a.cols + c + j) = make_float4(dof[i][j], dof[i][j + 1], dof[i][j + 2], dof[i][j + 3]);
+        for (int j = 0; j < Pairs<T>::N; j += 2) {
+          float* at = out + piece * VN + 2 * j;
+          *reinterpret_cast<float4*>(at) = make_float4(df[i].v[j].x, df[i].v[j].y, df[i].v[j + 1].x, df[i].v[j + 1].y);
+          *reinterpret_cast<float4*>(at + a.cols) = make_float4(dof[i].v[j].x, dof[i].v[j].y, dof[i].v[j + 1].x, dof[i].v[j + 1].y);
         }
       }
     }
@@ -358,46 +430,46 @@ __global__ void __launch_bounds__(384, 1) ln_bwd_warp_kernel(const LnBwdArgs a) 
   constexpr int kRows = kV == 1 ? 4 : (kV == 2 ? 2 : 1);
   constexpr int kWarps = 12;
   extern __shared__ __align__(128) uint8_t dyn[];
-  float* factor = reinterpret_cast<float*>(dyn);         // [cols]
-  float* sums = factor + (a.cols + 31) / 32 * 32;        // [kWarps][2][cols]
+  const float4* factor = reinterpret_cast<const float4*>(dyn);                       // [cols] floats
+  float2* sums = reinterpret_cast<float2*>(dyn + (size_t)(a.cols + 31) / 32 * 128);  // [kWarps][2][cols / 2]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t group = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
-  const int64_t base = group * a.rows_per_group;
-  const T* x = static_cast<const T*>(a.x) + base * a.x_ld;
-  const T* dy = static_cast<const T*>(a.dy) + base * a.dy_ld;
-  const int64_t step = (int64_t)a.parts * kWarps * kRows;
+  const int group = blockIdx.x / a.parts, part = blockIdx.x - group * a.parts;
+  const int pieces = a.cols / VN, rows = (int)a.rows_per_group;
+  const int64_t base = (int64_t)group * rows;
+  const T* x = static_cast<const T*>(a.x) + base * a.x_ld + lane * VN;
+  const T* dy = static_cast<const T*>(a.dy) + base * a.dy_ld + lane * VN;
+  const int step = a.parts * kWarps * kRows;
   uint4 xn[kRows][kV], dn[kRows][kV];
   float mn[kRows], rn[kRows];
-  auto ask = [&](int64_t r0) {
+  auto ask = [&](int r0) {
 #pragma unroll
     for (int q = 0; q < kRows; ++q) {
-      const int64_t r = r0 + q;
-      if (r < a.rows_per_group) {
+      const int r = r0 + q;
+      if (r < rows) {
         mn[q] = __ldg(a.mean + base + r);
         rn[q] = __ldg(a.rstd + base + r);
 #pragma unroll
         for (int i = 0; i < kV; ++i) {
-          const int c = (i * 32 + lane) * VN;
-          if (c < a.cols) {
-            xn[q][i] = ld_nc_u4(x + r * a.x_ld + c);
-            dn[q][i] = ld_nc_u4(dy + r * a.dy_ld + c);
+          if (i * 32 + lane < pieces) {
+            xn[q][i] = ld_nc_u4(x + r * a.x_ld + i * 32 * VN);
+            dn[q][i] = ld_nc_u4(dy + r * a.dy_ld + i * 32 * VN);
           }
         }
       }
     }
   };
-  int64_t r0 = (part * kWarps + warp) * kRows;
+  int r0 = (part * kWarps + warp) * kRows;
   ask(r0);
-  const T* fp = a.factor != nullptr ? static_cast<const T*>(a.factor) + group * a.vec_stride : nullptr;
-  for (int c = threadIdx.x; c < a.cols; c += blockDim.x) factor[c] = fp != nullptr ? a.unit + to_f(fp[c]) : 1.f;
+  fill_factor<T>(reinterpret_cast<float*>(dyn),
+                 a.factor != nullptr ? static_cast<const T*>(a.factor) + group * a.vec_stride : nullptr, a.unit, a.cols);
   __syncthreads();
-  float df[kV][VN], dof[kV][VN];
+  Pairs<T> df[kV], dof[kV];
 #pragma unroll
   for (int i = 0; i < kV; ++i)
 #pragma unroll
-    for (int j = 0; j < VN; ++j) df[i][j] = dof[i][j] = 0.f;
+    for (int j = 0; j < Pairs<T>::N; ++j) df[i].v[j] = dof[i].v[j] = both(0.f);
   const float inv_cols = 1.f / a.cols;
-  for (; r0 < a.rows_per_group; r0 += step) {
+  for (; r0 < rows; r0 += step) {
     uint4 xc[kRows][kV], dc[kRows][kV];
     float mc[kRows], rc[kRows];
 #pragma unroll
@@ -410,59 +482,47 @@ __global__ void __launch_bounds__(384, 1) ln_bwd_warp_kernel(const LnBwdArgs a) 
     ask(r0 + step);
 #pragma unroll
     for (int q = 0; q < kRows; ++q) {
-      if (r0 + q >= a.rows_per_group) break;
-      float g[kV][VN], h[kV][VN];
-      float s1 = 0.f, s2 = 0.f;
+      if (r0 + q >= rows) break;
+      Pairs<T> g[kV], h[kV];
+      float2 s1 = both(0.f), s2 = both(0.f);
 #pragma unroll
-      for (int i = 0; i < kV; ++i) {
-        const int c = (i * 32 + lane) * VN;
-        if (c < a.cols) {
-          Vec<T> xv, dv;
-          xv.unpack(xc[q][i]);
-          dv.unpack(dc[q][i]);
-#pragma unroll
-          for (int j = 0; j < VN; ++j) {
-            h[i][j] = (xv.v[j] - mc[q]) * rc[q];
-            g[i][j] = dv.v[j] * factor[c + j];
-            s1 += g[i][j];
-            s2 = fmaf(g[i][j], h[i][j], s2);
-            df[i][j] = fmaf(dv.v[j], h[i][j], df[i][j]);
-            dof[i][j] += dv.v[j];
-          }
-        }
-      }
-      const float k1 = -warp_sum(s1) * inv_cols * rc[q], k2 = -warp_sum(s2) * inv_cols * rc[q];
+      for (int i = 0; i < kV; ++i)
+        if (i * 32 + lane < pieces)
+          bwd_piece<T>(xc[q][i], dc[q][i], factor, i * 32 + lane, pieces, both(-mc[q]), both(rc[q]), g[i], h[i], s1, s2, df[i],
+                       dof[i]);
+      const float keep = warp_sum_two(s1, s2, lane);
+      const float over = __shfl_xor_sync(0xffffffffu, keep, 16);
       if (a.dx != nullptr) {
-        T* dx = static_cast<T*>(a.dx) + (base + r0 + q) * a.dx_ld;
+        const float k = -inv_cols * rc[q];
+        const float2 k1 = both(k * ((lane & 16) ? over : keep)), k2 = both(k * ((lane & 16) ? keep : over));
+        T* dx = static_cast<T*>(a.dx) + (base + r0 + q) * a.dx_ld + lane * VN;
 #pragma unroll
-        for (int i = 0; i < kV; ++i) {
-          const int c = (i * 32 + lane) * VN;
-          if (c < a.cols) {
-            Vec<T> o;
-#pragma unroll
-            for (int j = 0; j < VN; ++j) o.v[j] = fmaf(h[i][j], k2, fmaf(g[i][j], rc[q], k1));
-            o.store(dx + c);
-          }
-        }
+        for (int i = 0; i < kV; ++i)
+          if (i * 32 + lane < pieces)
+            *reinterpret_cast<uint4*>(dx + i * 32 * VN) = bwd_dx<T>(g[i], h[i], both(rc[q]), k1, k2);
       }
     }
   }
   if (a.partial == nullptr) return;
-  float* mine = sums + (size_t)warp * 2 * a.cols;
+  float2* mine = sums + (size_t)warp * a.cols;
 #pragma unroll
   for (int i = 0; i < kV; ++i) {
-    const int c = (i * 32 + lane) * VN;
-    if (c < a.cols) {
+    const int piece = i * 32 + lane;
+    if (piece < pieces) {
 #pragma unroll
-      for (int j = 0; j < VN; ++j) { mine[c + j] = df[i][j]; mine[a.cols + c + j] = dof[i][j]; }
+      for (int j = 0; j < Pairs<T>::N; ++j) {
+        mine[piece * (VN / 2) + j] = df[i].v[j];
+        mine[a.cols / 2 + piece * (VN / 2) + j] = dof[i].v[j];
+      }
     }
   }
   __syncthreads();
   float* out = a.partial + (int64_t)blockIdx.x * 2 * a.cols;
+  const float* all = reinterpret_cast<const float*>(sums);
   for (int c = threadIdx.x; c < 2 * a.cols; c += blockDim.x) {
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) s += sums[(size_t)w * 2 * a.cols + c];
+    for (int w = 0; w < kWarps; ++w) s += all[(size_t)w * 2 * a.cols + c];
     out[c] = s;
   }
 }
@@ -512,10 +572,10 @@ static BwdPlan bwd_plan(int64_t groups, int64_t rows_per_group, int64_t cols, in
       rows_at_once = 12;
       p.smem = ((size_t)(cols + 31) / 32 * 32 + 24 * (size_t)cols) * 4;
     } else {
-      // pieces per thread: the most that registers hold (three of bf16, four of fp32), unless fewer leave fewer
-      // lanes without a column
+      // pieces per thread: the most that registers hold (two of bf16, four of fp32; three of bf16 spill and are left
+      // to rows of more than 8192), unless fewer leave fewer lanes without a column
       int64_t best = -1;
-      for (int k = vn == 8 ? 3 : 4; k >= 1; --k) {
+      for (int k = vn == 8 ? (v > 1024 ? 3 : 2) : 4; k >= 1; --k) {
         const int64_t w = (v + 32 * k - 1) / (32 * k);
         if (w < 2 || w > 16) continue;  // (named barriers and slots are counted for eight teams)
         const int64_t idle = (w * 32 * k - v) * 64 / v;  // in 64ths of a row
@@ -623,6 +683,14 @@ extern "C" int64_t fluxb_layer_norm_bwd_scratch(int64_t rows, int64_t cols, int6
   return groups * parts * 2 * cols;
 }
 
+template <typename T, bool kFull>
+static auto team_kernel(int vecs) -> void (*)(LnBwdArgs) {
+  if (vecs == 1) return ln_bwd_team_kernel<T, 1, kFull>;
+  if (vecs == 2) return ln_bwd_team_kernel<T, 2, kFull>;
+  if (vecs == 3) return ln_bwd_team_kernel<T, 3, kFull>;
+  return ln_bwd_team_kernel<T, sizeof(T) == 2 ? 3 : 4, kFull>;  // (four of bf16 are never planned)
+}
+
 template <typename T>
 static int launch_bwd(const LnBwdArgs& a, const BwdPlan& p, bool sums, cudaStream_t st) {
   const unsigned grid = (unsigned)(a.groups * a.parts);
@@ -635,10 +703,7 @@ static int launch_bwd(const LnBwdArgs& a, const BwdPlan& p, bool sums, cudaStrea
   if (p.kind == BwdPlan::kWarp)
     kern = p.vecs == 1 ? ln_bwd_warp_kernel<T, 1> : (p.vecs == 2 ? ln_bwd_warp_kernel<T, 2> : ln_bwd_warp_kernel<T, 3>);
   else
-    kern = p.vecs == 1   ? ln_bwd_team_kernel<T, 1>
-           : p.vecs == 2 ? ln_bwd_team_kernel<T, 2>
-           : p.vecs == 3 ? ln_bwd_team_kernel<T, 3>
-                         : ln_bwd_team_kernel<T, sizeof(T) == 2 ? 3 : 4>;
+    kern = a.cols * (int)sizeof(T) == p.vecs * p.wpr * 512 ? team_kernel<T, true>(p.vecs) : team_kernel<T, false>(p.vecs);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem);
   if (e != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "layer_norm_bwd: cannot set shared memory size: %s", cudaGetErrorString(e));
   kern<<<grid, p.kind == BwdPlan::kWarp ? 384 : p.teams * p.wpr * 32, p.smem, st>>>(a);
