@@ -4,8 +4,9 @@
 // same rotation by the negative angle.
 //
 // Angles: the position times the pair's turns per unit position (theta^(-2j'/d) / 2 pi, from the host in fp64) is
-// taken in fp64 and reduced to [-1/2, 1/2] turns there, so that positions of any size keep an angle exact to
-// 2^-25 turns; sine and cosine of the reduced turn are fp32.
+// taken exactly enough that the turn left over after whole turns, in [-1/2, 1/2], is right to 2^-25: in two fp32 parts
+// for positions below 2^24, in fp64 beyond (fp64 throughout took as long as the memory traffic of 16 heads); sine
+// and cosine of the reduced turn are fp32.
 #include <math.h>
 
 #include "vec.cuh"
@@ -35,11 +36,26 @@ struct RopeAxesArgs {
   uint8_t axis[kMaxPairs];
 };
 
+// A frequency as two fp32 parts.
+__device__ __forceinline__ float2 split(double f) {
+  const float high = static_cast<float>(f);
+  return make_float2(high, static_cast<float>(f - high));
+}
+
 template <typename Id>
-__device__ __forceinline__ float2 turn_of(const RopeAxesArgs& a, int64_t b, int64_t l, int j) {
-  const double pos = static_cast<double>(static_cast<const Id*>(a.ids)[b * a.id_sb + l * a.id_sl + a.axis[j] * a.id_sa]);
-  const double t = pos * a.turns[j];
-  const float r = static_cast<float>(t - rint(t));
+__device__ __forceinline__ float2 turn_of(const RopeAxesArgs& a, int64_t b, int64_t l, int j, float2 turns, int axis) {
+  const Id id = __ldg(static_cast<const Id*>(a.ids) + b * a.id_sb + l * a.id_sl + axis * a.id_sa);
+  float r;
+  if (id > static_cast<Id>(-(1 << 24)) && id < static_cast<Id>(1 << 24)) {
+    // pos is exact in fp32 and the turn count below 2^22: the product as high part and error, both exact, the whole
+    // turns taken off the high part (exact, too), then what the frequency's low part adds (2^-49 of the turns off)
+    const float pos = static_cast<float>(id), high = pos * turns.x;
+    const float whole = (high + 12582912.f) - 12582912.f;  // 1.5 * 2^23: to the nearest integer
+    r = (high - whole) + fmaf(pos, turns.y, fmaf(pos, turns.x, -high));
+  } else {
+    const double t = static_cast<double>(id) * a.turns[j];
+    r = static_cast<float>(t - rint(t));
+  }
   float s, c;
   sincospif(2.f * r, &s, &c);
   return make_float2(c, a.sign * s);
@@ -48,83 +64,113 @@ __device__ __forceinline__ float2 turn_of(const RopeAxesArgs& a, int64_t b, int6
 // Rows of whole 16-byte pieces.  A block takes a few tokens: its threads first take one angle each, sines and cosines go
 // through shared memory, and then every thread owns one piece of one token's rows, keeps its four pairs' sines and
 // cosines in registers and walks every `slots`-th head of q and k.  A pair's angle is so taken once, no table is read or
-// written, and kAhead pieces per thread are on their way at any time: the next one is asked for as soon as one is
-// done.  Bound by HBM: every element is read once and written once.  (With the angles per thread instead, taken again
-// for every group of heads: 37 us for 24 + 24 heads of 4608 tokens.)
+// written, and the next kAhead pieces of a thread are on their way while it works on the current ones.  Bound by HBM:
+// every element is read once and written once.  (With the angles per thread instead, taken again for every group of
+// heads: 37 us for 24 + 24 heads of 4608 tokens.)
 template <typename T, typename Id>
 __global__ void __launch_bounds__(256, 4) rope_axes_vec_kernel(const __grid_constant__ RopeAxesArgs a) {
   constexpr int VN = Vec<T>::N;
-  constexpr int kAhead = 4;
+  constexpr int kAhead = 3;
   extern __shared__ float2 table[];  // [tokens][D / 2]
+  __shared__ float2 turns[kMaxPairs];
+  __shared__ uint8_t axis[kMaxPairs];
+  // (the kernel's parameters can be read at one address per warp and cycle only: lanes that each read their own pair's
+  // made the angles of 65536 tokens with one head take 45 us)
+  if (threadIdx.x < a.pairs) {
+    turns[threadIdx.x] = split(a.turns[threadIdx.x]);
+    axis[threadIdx.x] = a.axis[threadIdx.x];
+  }
+  __syncthreads();
   const int pieces = a.D / VN, half = a.D / 2;
-  const int tokens = (int)(a.B * a.L), tok0 = blockIdx.x * a.tokens;
+  const int tokens = (int)(a.B * a.L);
   const int piece = threadIdx.x % pieces, rest = threadIdx.x / pieces;
   const int t = rest % a.tokens, slot = rest / a.tokens;
+  for (int tok0 = blockIdx.x * a.tokens; tok0 < tokens; tok0 += gridDim.x * a.tokens) {
   const int tok = tok0 + t;
   const bool active = slot < a.slots && tok < tokens;
   const int b = tok / (int)a.L, l = tok - b * (int)a.L;
-  const int hq = a.t[0].heads, heads = hq + a.t[1].heads;
-  // This thread's heads are slot, slot + slots, ... of q's and then k's; where to read and write runs along with them.
-  const int64_t src0 = b * a.t[0].sb + l * a.t[0].sl + piece * VN, src1 = b * a.t[1].sb + l * a.t[1].sl + piece * VN;
-  const int64_t dst0 = b * a.t[0].ob + l * a.t[0].ol + piece * VN, dst1 = b * a.t[1].ob + l * a.t[1].ol + piece * VN;
-  const int hk = slot < hq ? (hq - slot + a.slots - 1) / a.slots * a.slots + slot - hq : slot - hq;  // its first of k's
-  const T* k_src = static_cast<const T*>(a.t[1].src) + src1 + hk * a.t[1].sh;
-  T* k_dst = static_cast<T*>(a.t[1].dst) + dst1 + hk * a.t[1].oh;
-  const int64_t q_step = a.slots * a.t[0].sh, k_step = a.slots * a.t[1].sh;
-  const int64_t qo_step = a.slots * a.t[0].oh, ko_step = a.slots * a.t[1].oh;
-  const T* src = slot < hq ? static_cast<const T*>(a.t[0].src) + src0 + slot * a.t[0].sh : k_src;
-  T* dst = slot < hq ? static_cast<T*>(a.t[0].dst) + dst0 + slot * a.t[0].oh : k_dst;
-  int ask = slot, done = slot;  // next head to ask for, next head to finish
-  uint4 raw[kAhead];
-  auto load = [&](uint4& to) {
-    if (ask < heads) to = ld_nc_u4(src);
-    const bool was_q = ask < hq;
-    ask += a.slots;
-    src = was_q && ask >= hq ? k_src : src + (was_q ? q_step : k_step);
-  };
-  if (active) {
+  // This thread's heads are slot, slot + slots, ... of q and then of k, kAhead at a time.
+  const int64_t at[4] = {b * a.t[0].sb + l * a.t[0].sl + slot * a.t[0].sh, b * a.t[1].sb + l * a.t[1].sl + slot * a.t[1].sh,
+                         b * a.t[0].ob + l * a.t[0].ol + slot * a.t[0].oh, b * a.t[1].ob + l * a.t[1].ol + slot * a.t[1].oh};
+  const T *sq = static_cast<const T*>(a.t[0].src) + at[0] + piece * VN, *sk = static_cast<const T*>(a.t[1].src) + at[1] + piece * VN;
+  T *dq = static_cast<T*>(a.t[0].dst) + at[2] + piece * VN, *dk = static_cast<T*>(a.t[1].dst) + at[3] + piece * VN;
+  const int64_t qs = a.slots * a.t[0].sh, ks = a.slots * a.t[1].sh, qo = a.slots * a.t[0].oh, ko = a.slots * a.t[1].oh;
+  int nq = active && slot < a.t[0].heads ? (a.t[0].heads - slot + a.slots - 1) / a.slots : 0;
+  int nk = active && slot < a.t[1].heads ? (a.t[1].heads - slot + a.slots - 1) / a.slots : 0;
+  uint4 next[kAhead];
+  auto load = [&](const T* p, int64_t step, int n) {
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) load(raw[u]);
-  }
+    for (int u = 0; u < kAhead; ++u, p += step)
+      if (u < n) next[u] = ld_nc_u4(p);
+  };
+  if (nq > 0) load(sq, qs, nq);
+  else load(sk, ks, nk);
+#pragma unroll 4
   for (int i = threadIdx.x; i < a.tokens * half; i += 256) {
     const int ti = i / half, j = i - ti * half;
     if (tok0 + ti < tokens && j < a.pairs) {
       const int bi = (tok0 + ti) / (int)a.L;
-      table[i] = turn_of<Id>(a, bi, tok0 + ti - bi * (int)a.L, j);
+      table[i] = turn_of<Id>(a, bi, tok0 + ti - bi * (int)a.L, j, turns[j], axis[j]);
     }
   }
   __syncthreads();
-  if (!active) return;
-  const int j0 = piece * (VN / 2);
+  const int rotated = min(VN / 2, a.pairs - piece * (VN / 2));  // pairs of this piece: all, some, or none (0 or less)
   float2 cs[VN / 2];
 #pragma unroll
-  for (int p = 0; p < VN / 2; ++p) cs[p] = j0 + p < a.pairs ? table[t * half + j0 + p] : make_float2(1.f, 0.f);
-  const bool whole = j0 + VN / 2 <= a.pairs;
-  while (done < heads) {
+  for (int p = 0; p < VN / 2; ++p)
+    if (active && p < rotated) cs[p] = table[t * half + piece * (VN / 2) + p];
+  auto finish = [&](T* p, int64_t step, const uint4 (&now)[kAhead], int n) {
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (done >= heads) break;
-      const uint4 now = raw[u];
-      load(raw[u]);
-      if (j0 >= a.pairs) {  // behind the axes: copied
-        *reinterpret_cast<uint4*>(dst) = now;
+    for (int u = 0; u < kAhead; ++u, p += step) {
+      if (u >= n) break;
+      if (rotated == VN / 2) {
+        Vec<T> v;
+        v.unpack(now[u]);
+#pragma unroll
+        for (int e = 0; e < VN / 2; ++e) {
+          const float x0 = v.v[2 * e], x1 = v.v[2 * e + 1];
+          v.v[2 * e] = x0 * cs[e].x - x1 * cs[e].y;
+          v.v[2 * e + 1] = x0 * cs[e].y + x1 * cs[e].x;
+        }
+        v.store(p);
+      } else if (rotated <= 0) {  // behind the axes: copied
+        *reinterpret_cast<uint4*>(p) = now[u];
       } else {
         Vec<T> v;
-        v.unpack(now);
+        v.unpack(now[u]);
 #pragma unroll
-        for (int p = 0; p < VN / 2; ++p) {
-          if (whole || j0 + p < a.pairs) {
-            const float x0 = v.v[2 * p], x1 = v.v[2 * p + 1];
-            v.v[2 * p] = x0 * cs[p].x - x1 * cs[p].y;
-            v.v[2 * p + 1] = x0 * cs[p].y + x1 * cs[p].x;
+        for (int e = 0; e < VN / 2; ++e) {
+          if (e < rotated) {
+            const float x0 = v.v[2 * e], x1 = v.v[2 * e + 1];
+            v.v[2 * e] = x0 * cs[e].x - x1 * cs[e].y;
+            v.v[2 * e + 1] = x0 * cs[e].y + x1 * cs[e].x;
           }
         }
-        v.store(dst);
+        v.store(p);
       }
-      const bool was_q = done < hq;
-      done += a.slots;
-      dst = was_q && done >= hq ? k_dst : dst + (was_q ? qo_step : ko_step);
     }
+  };
+  uint4 now[kAhead];
+  while (nq > 0) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) now[u] = next[u];
+    sq += kAhead * qs;
+    if (nq > kAhead) load(sq, qs, nq - kAhead);
+    else load(sk, ks, nk);
+    finish(dq, qo, now, nq);
+    dq += kAhead * qo;
+    nq -= kAhead;
+  }
+  while (nk > 0) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) now[u] = next[u];
+    sk += kAhead * ks;
+    if (nk > kAhead) load(sk, ks, nk - kAhead);
+    finish(dk, ko, now, nk);
+    dk += kAhead * ko;
+    nk -= kAhead;
+  }
+  __syncthreads();  // the table is free
   }
 }
 
@@ -137,7 +183,7 @@ __global__ void __launch_bounds__(256) rope_axes_any_kernel(const __grid_constan
   const int j = (int)(i % half);
   const int64_t tok = i / half, b = tok / a.L, l = tok % a.L;
   const bool rot = j < a.pairs;
-  const float2 cs = rot ? turn_of<Id>(a, b, l, j) : make_float2(1.f, 0.f);
+  const float2 cs = rot ? turn_of<Id>(a, b, l, j, split(a.turns[j]), a.axis[j]) : make_float2(1.f, 0.f);
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
     const RopeTensor& t = a.t[w];
@@ -216,13 +262,14 @@ extern "C" int fluxb_rope_axes(const void* q, void* oq, const int64_t* q_strides
     for (int64_t s : {t.sb, t.sh, t.sl, t.ob, t.oh, t.ol}) whole = whole && s % vn == 0;
   }
   if (whole) {
-    // Threads of a block: pieces x tokens x slots of heads.  Four slots, more when the tokens fill too few blocks.
-    int64_t slots = 4, heads = Hq + Hk;
-    while (slots > 1 && pieces * slots > 256) slots /= 2;
+    // Threads of a block: pieces x tokens x slots of heads.  A thread takes all heads (16 heads: 16.5 us with one slot,
+    // 18.0 with four), unless the tokens fill too few blocks.
+    int64_t slots = 1, heads = Hq + Hk;
     while (slots * 2 <= heads && pieces * slots * 2 <= 256 && B * L <= 2 * sm_count() * (256 / (pieces * slots))) slots *= 2;
     a.slots = (int)slots;
     a.tokens = (int)(256 / (pieces * slots));
-    const unsigned vgrid = (unsigned)((B * L + a.tokens - 1) / a.tokens);
+    const int64_t most = 4 * sm_count(), blocks = (B * L + a.tokens - 1) / a.tokens;
+    const unsigned vgrid = (unsigned)(blocks < most ? blocks : most);
     const size_t smem = (size_t)a.tokens * (D / 2) * sizeof(float2);
 #define FLUXB_ROPE_AXES(T)                                                                    \
   do {                                                                                        \
