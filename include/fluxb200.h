@@ -339,11 +339,11 @@ int fluxb_layer_norm_bwd(const void* dy, const void* x, const void* factor, cons
  *   on D; Hq and Hk may differ and either may be 0.  ids: [B, L, n_axes] of id_type
  *   (FLUXB_ID_*) with its three strides (0 to share).  At most 8 axes and 128 rotated pairs.
  */
-int fluxb_rope_axes(const void* q, void* oq, const int64_t* q_strides, const int64_t* oq_strides, int64_t Hq,
-                    const void* k, void* ok, const int64_t* k_strides, const int64_t* ok_strides, int64_t Hk,
-                    const void* ids, int id_type, const int64_t* id_strides, int64_t B, int64_t L, int64_t D,
-                    const int64_t* axes_dim, int n_axes, double theta, int backward, int dtype,
-                    fluxb_stream_t stream);
+int fluxb_rope_axes(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sl, void* oq, int64_t oq_sb, int64_t oq_sh,
+                    int64_t oq_sl, int64_t Hq, const void* k, int64_t k_sb, int64_t k_sh, int64_t k_sl, void* ok,
+                    int64_t ok_sb, int64_t ok_sh, int64_t ok_sl, int64_t Hk, const void* ids, int id_type, int64_t id_sb,
+                    int64_t id_sl, int64_t id_sa, int64_t B, int64_t L, int64_t D, const int64_t* axes_dim, int n_axes,
+                    double theta, int backward, int dtype, fluxb_stream_t stream);
 
 /*
  * A shared projection plus one low-rank adapter per request:

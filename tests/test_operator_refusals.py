@@ -31,9 +31,9 @@ def test_layer_norm(lib):
 
 
 def rope(lib, axes=(16, 48), B=1, L=4, D=64, H=2, q=P, ids=P, id_type=0, theta=1e4, dtype=1, n=None):
-    s, i = (c_int64 * 3)(512, 256, 64), (c_int64 * 3)(8, 2, 1)
-    return lib.fluxb_rope_axes(q, P, s, s, H, P, P, s, s, H, ids, id_type, i, B, L, D, (c_int64 * len(axes))(*axes), len(axes) if n is None else n,
-                               theta, 0, dtype, None)
+    s = (512, 256, 64)
+    return lib.fluxb_rope_axes(q, *s, P, *s, H, P, *s, P, *s, H, ids, id_type, 8, 2, 1, B, L, D, (c_int64 * len(axes))(*axes),
+                               len(axes) if n is None else n, theta, 0, dtype, None)
 
 
 def test_rope_axes(lib):

@@ -7,7 +7,6 @@ PyTorch fallback.
 from __future__ import annotations
 
 import ctypes
-from contextlib import nullcontext
 from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_void_p, POINTER
 from pathlib import Path
 
@@ -16,6 +15,7 @@ import torch
 LIB_PATH = Path(__file__).resolve().parent / "libfluxb200.so"
 
 F32, BF16 = 0, 1
+DTYPE_CODES = {torch.float32: F32, torch.bfloat16: BF16}
 ID_F32, ID_I32, ID_I64 = 0, 1, 2
 EPI_NONE, EPI_GELU, EPI_GATE_RESID = 0, 1, 2
 ERR_BAD_ARG, ERR_UNSUPPORTED, ERR_CUDA, ERR_TIMEOUT = -1, -2, -3, -4
@@ -68,7 +68,7 @@ SIGNATURES = {
     "fluxb_layer_norm": (_I, [_P] * 6 + [_L] * 6 + [_F, _F, _I, _P]),
     "fluxb_layer_norm_bwd_scratch": (_L, [_L, _L, _L]),
     "fluxb_layer_norm_bwd": (_I, [_P] * 9 + [_L] * 7 + [_F, _I, _I, _P]),
-    "fluxb_rope_axes": (_I, [_P, _P, _P, _P, _L, _P, _P, _P, _P, _L, _P, _I, _P, _L, _L, _L, _P, _I, c_double, _I, _I, _P]),
+    "fluxb_rope_axes": (_I, ([_P] + [_L] * 3) * 2 + [_L] + ([_P] + [_L] * 3) * 2 + [_L, _P, _I] + [_L] * 6 + [_P, _I, c_double, _I, _I, _P]),
     "fluxb_linear_lora_scratch_bytes": (_L, [_L] * 4),
     "fluxb_linear_lora": (_I, [_P] * 8 + [_I, _P] + [_L] * 10 + [_I, _P]),
     "fluxb_peer_header_bytes": (_I, []),
@@ -128,10 +128,9 @@ def check(rc: int, launches: bool = True) -> None:
 
 
 def dtype_code(t: torch.Tensor) -> int:
-    if t.dtype == torch.bfloat16:
-        return BF16
-    if t.dtype == torch.float32:
-        return F32
+    code = DTYPE_CODES.get(t.dtype)
+    if code is not None:
+        return code
     raise NotImplementedError(f"fluxb200 kernels take float32 or bfloat16 tensors, got {t.dtype}")
 
 
@@ -147,13 +146,15 @@ def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def on_device_of(t: torch.Tensor):
-    """Context that makes t's device current for the launch: a no-op where it is already."""
-    index = t.device.index
-    return _HERE if index is None or index == torch.cuda.current_device() else torch.cuda.device(index)
-
-
-_HERE = nullcontext()
+def launch(fn, device_index: int, *args) -> None:
+    """fn(*args, stream) on the current stream of the device that the tensors are on, which is made
+    current for the call if another one is.  (The raw handle straight from torch's binding: wrapping
+    it in a Stream object first takes 3 us, as long as the launch itself.)"""
+    if device_index == torch.cuda.current_device():
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(device_index)))
+        return
+    with torch.cuda.device(device_index):
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(device_index)))
 
 
 def require_same_device(first: torch.Tensor, *others: torch.Tensor) -> None:

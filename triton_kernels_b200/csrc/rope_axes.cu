@@ -206,11 +206,12 @@ __global__ void __launch_bounds__(256) rope_axes_any_kernel(const __grid_constan
 
 using namespace fluxb;
 
-extern "C" int fluxb_rope_axes(const void* q, void* oq, const int64_t* q_strides, const int64_t* oq_strides, int64_t Hq,
-                               const void* k, void* ok, const int64_t* k_strides, const int64_t* ok_strides, int64_t Hk,
-                               const void* ids, int id_type, const int64_t* id_strides, int64_t B, int64_t L, int64_t D,
-                               const int64_t* axes_dim, int n_axes, double theta, int backward, int dtype,
-                               fluxb_stream_t stream) {
+extern "C" int fluxb_rope_axes(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sl, void* oq, int64_t oq_sb,
+                               int64_t oq_sh, int64_t oq_sl, int64_t Hq, const void* k, int64_t k_sb, int64_t k_sh,
+                               int64_t k_sl, void* ok, int64_t ok_sb, int64_t ok_sh, int64_t ok_sl, int64_t Hk,
+                               const void* ids, int id_type, int64_t id_sb, int64_t id_sl, int64_t id_sa, int64_t B,
+                               int64_t L, int64_t D, const int64_t* axes_dim, int n_axes, double theta, int backward,
+                               int dtype, fluxb_stream_t stream) {
   if (dtype != FLUXB_F32 && dtype != FLUXB_BF16) return set_error(FLUXB_ERR_UNSUPPORTED, "rope_axes: dtype %d", dtype);
   if (id_type != FLUXB_ID_F32 && id_type != FLUXB_ID_I32 && id_type != FLUXB_ID_I64)
     return set_error(FLUXB_ERR_UNSUPPORTED, "rope_axes: id type %d", id_type);
@@ -228,20 +229,16 @@ extern "C" int fluxb_rope_axes(const void* q, void* oq, const int64_t* q_strides
                                 (long long)rot, (long long)D);
   if (rot / 2 > kMaxPairs) return set_error(FLUXB_ERR_UNSUPPORTED, "rope_axes: more than %d rotated pairs", kMaxPairs);
   if (B == 0 || L == 0 || Hq + Hk == 0) return FLUXB_OK;
-  if (!ids || !id_strides || (Hq > 0 && (!q || !oq || !q_strides || !oq_strides)) ||
-      (Hk > 0 && (!k || !ok || !k_strides || !ok_strides)))
+  if (!ids || (Hq > 0 && (!q || !oq)) || (Hk > 0 && (!k || !ok)))
     return set_error(FLUXB_ERR_BAD_ARG, "rope_axes: null pointer");
   const int64_t half = (D + 1) / 2;
   if (D > (1 << 16) || Hq > (1 << 20) || Hk > (1 << 20) || B * L > INT32_MAX || (B * L * half + 255) / 256 > INT32_MAX)
     return set_error(FLUXB_ERR_UNSUPPORTED, "rope_axes: too many tokens or heads");
   RopeAxesArgs a;
-  const int64_t zero[3] = {0, 0, 0};
-  const int64_t *qs = Hq > 0 ? q_strides : zero, *qo = Hq > 0 ? oq_strides : zero;
-  const int64_t *ks = Hk > 0 ? k_strides : zero, *ko = Hk > 0 ? ok_strides : zero;
-  a.t[0] = RopeTensor{q, oq, qs[0], qs[1], qs[2], qo[0], qo[1], qo[2], (int)Hq};
-  a.t[1] = RopeTensor{k, ok, ks[0], ks[1], ks[2], ko[0], ko[1], ko[2], (int)Hk};
+  a.t[0] = RopeTensor{q, oq, q_sb, q_sh, q_sl, oq_sb, oq_sh, oq_sl, (int)Hq};
+  a.t[1] = RopeTensor{k, ok, k_sb, k_sh, k_sl, ok_sb, ok_sh, ok_sl, (int)Hk};
   a.ids = ids;
-  a.id_sb = id_strides[0]; a.id_sl = id_strides[1]; a.id_sa = id_strides[2];
+  a.id_sb = id_sb; a.id_sl = id_sl; a.id_sa = id_sa;
   a.B = B; a.L = L; a.D = (int)D;
   a.pairs = (int)(rot / 2);
   a.sign = backward ? -1.f : 1.f;

@@ -263,12 +263,9 @@ def linear_lora(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None, lora_a
     adapter = adapter.contiguous()
     lib = _lib.load()
     scratch = torch.empty(lib.fluxb_linear_lora_scratch_bytes(M, N, K, R), device=x.device, dtype=torch.uint8)
-    with _lib.on_device_of(x):
-        _lib.check(
-            lib.fluxb_linear_lora(
-                x2d.data_ptr(), w.data_ptr(), _lib.ptr(b), y.data_ptr(), lora_a.data_ptr(), lora_b.data_ptr(),
-                _lib.ptr(lora_scale), adapter.data_ptr(), int(adapter.dtype == torch.int64), scratch.data_ptr(), B, M // B, N,
-                K, R, n, x2d.stride(0), w.stride(0), N, lora_b.shape[2], _lib.EPI_GELU if activation else _lib.EPI_NONE, _lib.stream_handle(),
-            )
-        )
+    _lib.launch(
+        lib.fluxb_linear_lora, x.get_device(), x2d.data_ptr(), w.data_ptr(), _lib.ptr(b), y.data_ptr(), lora_a.data_ptr(),
+        lora_b.data_ptr(), _lib.ptr(lora_scale), adapter.data_ptr(), adapter.dtype == torch.int64, scratch.data_ptr(), B, M // B,
+        N, K, R, n, x2d.stride(0), w.stride(0), N, lora_b.shape[2], _lib.EPI_GELU if activation else _lib.EPI_NONE,
+    )
     return y

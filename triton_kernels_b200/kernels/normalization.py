@@ -33,103 +33,111 @@ def _dense16(t: torch.Tensor) -> torch.Tensor:
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
-    """x as [rows, C] with unit column stride and 16-byte aligned rows (of whole 16-byte pieces); a
-    view where the rows are evenly spaced."""
-    C = x.shape[-1]
-    if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= C and x.stride(0) % _vec(x) == 0 and x.data_ptr() % 16 == 0:
+    """x as evenly spaced rows of its last dim, 16-byte aligned (rows of whole 16-byte pieces): x
+    itself where it is contiguous or a 2-D view with a row stride, else a copy."""
+    if x.is_contiguous():
+        return x if x.data_ptr() % 16 == 0 else x.clone()
+    if (x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= x.shape[1] and x.stride(0) % _vec(x) == 0
+            and x.data_ptr() % 16 == 0):
         return x
-    return _dense16(x).view(-1, C)
+    return x.contiguous()
 
 
-def _norm_backward(dy, x2, factor2, mean, rstd, unit: float, groups: int, want_dx: bool, want_sums: bool, grads_dtype):
-    """(dx [rows, C] or None, dfactor, doffset [groups, C] or None) through fluxb_layer_norm_bwd.
-    factor2: [groups, C] view with unit column stride, or None (ones)."""
-    rows, C = x2.shape
-    dy2 = _rows(dy)
+def _row_stride(x: torch.Tensor) -> int:
+    return x.stride(0) if x.dim() == 2 else x.shape[-1]
+
+
+def _norm_backward(dy, x, factor, factor_stride: int, stats, unit: float, groups: int, want_dx: bool, df, do, grads_f32: bool):
+    """dx (or None), with the groups' gradients of factor and offset left in df and do (or None),
+    through fluxb_layer_norm_bwd.  x: as `_rows` gives it; stats: fp32, the rows' means, then their
+    reciprocal deviations."""
     lib = _lib.load()
-    dx = torch.empty((rows, C), device=x2.device, dtype=x2.dtype) if want_dx else None
-    df = do = scratch = None
-    per_group = rows // groups if groups else 0
-    if want_sums:
-        make = torch.zeros if rows == 0 else torch.empty
-        df, do = make((2, groups, C), device=x2.device, dtype=grads_dtype).unbind(0)
-        scratch = torch.empty(lib.fluxb_layer_norm_bwd_scratch(rows, C, per_group), device=x2.device, dtype=torch.float32)
-    with _lib.on_device_of(x2):
-        _lib.check(
-            lib.fluxb_layer_norm_bwd(
-                _lib.ptr(dy2), _lib.ptr(x2), _lib.ptr(factor2), _lib.ptr(mean), _lib.ptr(rstd), _lib.ptr(dx), _lib.ptr(df),
-                _lib.ptr(do), _lib.ptr(scratch), rows, C, per_group, dy2.stride(0), x2.stride(0), C,
-                factor2.stride(0) if factor2 is not None and groups > 1 else 0, unit,
-                int(grads_dtype == torch.float32), _lib.dtype_code(x2), _lib.stream_handle(),
-            )
-        )
-    return dx, df, do
-
-
-def _layer_norm_forward(x, weight, bias, eps, stats: bool):
-    """(x as rows, y, mean, rstd) of `layer_norm`; mean and rstd are None without `stats`."""
     C = x.shape[-1]
-    x2 = _rows(x)
-    rows = x2.shape[0]
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    rows = x.numel() // C
+    dy = _rows(dy)
+    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if want_dx else None
+    per_group = rows // groups if groups else 0
+    scratch = None
+    if df is not None or do is not None:
+        scratch = stats.new_empty(lib.fluxb_layer_norm_bwd_scratch(rows, C, per_group))
+    mean = stats.data_ptr()
+    _lib.launch(
+        lib.fluxb_layer_norm_bwd, x.get_device(), dy.data_ptr(), x.data_ptr(), factor.data_ptr(), mean, mean + 4 * rows,
+        _lib.ptr(dx), _lib.ptr(df), _lib.ptr(do), _lib.ptr(scratch), rows, C, per_group, _row_stride(dy), _row_stride(x), C,
+        factor_stride, unit, int(grads_f32), _lib.DTYPE_CODES[x.dtype],
+    )
+    return dx
+
+
+def _layer_norm_forward(x, weight, bias, eps, stats):
+    """y of `layer_norm` for x as `_rows` gives it; fills `stats` (see `_norm_backward`) if given."""
+    C = x.shape[-1]
+    rows = x.numel() // C
+    y = torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, device=x.device, dtype=x.dtype)
     mean = rstd = None
-    if stats:
-        mean, rstd = torch.empty((2, rows), device=x.device, dtype=torch.float32).unbind(0)
-    with _lib.on_device_of(x):
-        _lib.check(
-            _lib.load().fluxb_layer_norm(
-                _lib.ptr(x2), _lib.ptr(weight), _lib.ptr(bias), _lib.ptr(y), _lib.ptr(mean), _lib.ptr(rstd), rows, C, rows,
-                x2.stride(0), C, 0, 0.0, eps, _lib.dtype_code(x), _lib.stream_handle(),
-            )
-        )
-    return x2, y, mean, rstd
+    if stats is not None:
+        mean = stats.data_ptr()
+        rstd = mean + 4 * rows
+    _lib.launch(
+        _lib.load().fluxb_layer_norm, x.get_device(), x.data_ptr(), weight.data_ptr(), bias.data_ptr(), y.data_ptr(), mean, rstd,
+        rows, C, rows, _row_stride(x), C, 0, 0.0, eps, _lib.DTYPE_CODES[x.dtype],
+    )
+    return y
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        x2, y, mean, rstd = _layer_norm_forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x2, weight, mean, rstd)
-        ctx.shape = x.shape
+        x = _rows(x)
+        stats = x.new_empty(2 * (x.numel() // x.shape[-1]), dtype=torch.float32)
+        y = _layer_norm_forward(x, weight, bias, eps, stats)
+        ctx.save_for_backward(x, weight, stats)
         return y
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x2, weight, mean, rstd = ctx.saved_tensors
+    def _backward(ctx, dy):
+        x, weight, stats = ctx.saved_tensors
         need_x, need_w, need_b, _ = ctx.needs_input_grad
-        dx, dw, db = _norm_backward(dy, x2, weight[None], mean, rstd, 0.0, 1, need_x,
-                                    need_w or need_b, x2.dtype)
-        return dx.view(ctx.shape) if need_x else None, dw[0] if need_w else None, db[0] if need_b else None, None
+        make = torch.empty_like if x.numel() else torch.zeros_like
+        dw = make(weight) if need_w else None
+        db = make(weight) if need_b else None
+        return _norm_backward(dy, x, weight, 0, stats, 0.0, 1, need_x, dw, db, False), dw, db, None
+
+    _backward_once = once_differentiable(_backward.__func__)
+
+    @staticmethod
+    def backward(ctx, dy):
+        # the wrapper that refuses second gradients is asked for only where somebody may take them
+        return (_LayerNorm._backward_once if torch.is_grad_enabled() else _LayerNorm._backward)(ctx, dy)
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
                eps: float = 1e-5) -> torch.Tensor:
     """LayerNorm over the last dim with a learned scale and offset ([C] each, or None), for fp32 or
-    bf16 tensors of any width; weight and bias have x's dtype.  Statistics are fp32, taken as the
-    mean and then the centred variance.  Differentiable once in x, weight and bias; the scale's and
-    the offset's gradients are summed in fp32 in a fixed order.  (No counterpart in the reference,
-    whose only LayerNorm is the modulated one.)"""
+    bf16 tensors of any width; weight and bias have x's dtype.  Statistics are fp32 (rows of 2-24 KB:
+    sum and sum of squares in one pass, shifted by the row's first element; others: mean, then
+    centred variance).  Differentiable once in x, weight and bias; the scale's and the offset's
+    gradients are summed in fp32 in a fixed order.  (No counterpart in the reference, whose only
+    LayerNorm is the modulated one.)"""
     _lib.require_cuda(x, weight, bias)
     _lib.require_same_device(x, weight, bias)
-    for p in (weight, bias):
-        if p is not None:
-            assert p.shape == x.shape[-1:], "weight and bias are vectors of x's last dim"
-            assert p.dtype == x.dtype, "Incompatible dtypes"
     _lib.dtype_code(x)
     C = x.shape[-1:]
-    weight = torch.ones(C, device=x.device, dtype=x.dtype) if weight is None else _dense16(weight)
-    bias = torch.zeros(C, device=x.device, dtype=x.dtype) if bias is None else _dense16(bias)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if weight is None:
+        weight = torch.ones(C, device=x.device, dtype=x.dtype)
+    if bias is None:
+        bias = torch.zeros(C, device=x.device, dtype=x.dtype)
+    assert weight.shape == C and bias.shape == C, "weight and bias are vectors of x's last dim"
+    assert weight.dtype == bias.dtype == x.dtype, "Incompatible dtypes"
+    weight, bias = _dense16(weight), _dense16(bias)
+    if (x.requires_grad or weight.requires_grad or bias.requires_grad) and torch.is_grad_enabled():
         return _LayerNorm.apply(x, weight, bias, eps)
-    return _layer_norm_forward(x, weight, bias, eps, False)[1]
+    return _layer_norm_forward(_rows(x), weight, bias, eps, None)
 
 
-def _ln_mod_forward(x, weight, bias, eps, stats: bool):
-    """(x as rows, scale as [B, C], y, mean, rstd) of `layer_norm_modulation`; mean and rstd are
-    None without `stats`."""
+def _ln_mod_forward(x, weight, bias, eps, stats):
+    """(scale as [B, C], y) of `layer_norm_modulation` for a contiguous x; fills `stats` if given."""
     B, C = x.shape[0], x.shape[-1]
-    x = x.contiguous()
     v = _vec(x)
     w2 = weight.reshape(B, C).to(x.dtype)
     b2 = bias.reshape(B, C).to(x.dtype)
@@ -140,52 +148,58 @@ def _ln_mod_forward(x, weight, bias, eps, stats: bool):
     if not (ok(w2) and ok(b2) and (B == 1 or w2.stride(0) == b2.stride(0))):
         w2, b2 = w2.contiguous(), b2.contiguous()
     y = torch.empty_like(x)
-    x2 = x.reshape(-1, C)
-    rows = x2.shape[0]
+    rows = x.numel() // C
     per_batch = rows // B if B else 0
+    stride = w2.stride(0) if B > 1 else 0
+    lib = _lib.load()
     mean = rstd = None
-    if stats:
-        mean, rstd = torch.empty((2, rows), device=x.device, dtype=torch.float32).unbind(0)
-    with _lib.on_device_of(x):
-        if C % v or x.data_ptr() % 16:  # rows that no 16-byte piece fits: the kernels for any width
-            _lib.check(
-                _lib.load().fluxb_layer_norm(
-                    _lib.ptr(x2), _lib.ptr(w2), _lib.ptr(b2), _lib.ptr(y), _lib.ptr(mean), _lib.ptr(rstd), rows, C, per_batch,
-                    C, C, w2.stride(0) if B > 1 else 0, 1.0, eps, _lib.dtype_code(x), _lib.stream_handle(),
-                )
-            )
-        elif stats:
-            _lib.check(
-                _lib.load().fluxb_layer_norm_modulation_stats(
-                    _lib.ptr(x2), _lib.ptr(w2), _lib.ptr(b2), _lib.ptr(y), _lib.ptr(mean), _lib.ptr(rstd), rows, C, per_batch,
-                    C, C, w2.stride(0) if B > 1 else 0, eps, _lib.dtype_code(x), _lib.stream_handle(),
-                )
-            )
-        else:
-            layer_norm_modulation_into(x2, w2, b2, y.reshape(-1, C), per_batch, eps)
-    return x2, w2, y, mean, rstd
+    if stats is not None:
+        mean = stats.data_ptr()
+        rstd = mean + 4 * rows
+    args = x.data_ptr(), w2.data_ptr(), b2.data_ptr(), y.data_ptr()
+    code = _lib.dtype_code(x)
+    if C % v or x.data_ptr() % 16:  # rows that no 16-byte piece fits: the kernels for any width
+        _lib.launch(lib.fluxb_layer_norm, x.get_device(), *args, mean, rstd, rows, C, per_batch, C, C, stride, 1.0, eps, code)
+    elif stats is not None:
+        _lib.launch(lib.fluxb_layer_norm_modulation_stats, x.get_device(), *args, mean, rstd, rows, C, per_batch, C, C, stride,
+                    eps, code)
+    else:
+        _lib.launch(lib.fluxb_layer_norm_modulation, x.get_device(), *args, rows, C, per_batch, C, C, stride, eps, code)
+    return w2, y
 
 
 class _LayerNormModulation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        x2, w2, y, mean, rstd = _ln_mod_forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x2, w2, mean, rstd)
-        ctx.shapes = x.shape, weight.shape, bias.shape
-        ctx.dtypes = weight.dtype, bias.dtype
+        x = x.contiguous()
+        stats = x.new_empty(2 * (x.numel() // x.shape[-1]), dtype=torch.float32)
+        w2, y = _ln_mod_forward(x, weight, bias, eps, stats)
+        ctx.save_for_backward(x, w2, stats)
+        ctx.vectors = weight.shape, weight.dtype, bias.shape, bias.dtype
         return y
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x2, w2, mean, rstd = ctx.saved_tensors
+    def _backward(ctx, dy):
+        x, w2, stats = ctx.saved_tensors
         need_x, need_w, need_b, _ = ctx.needs_input_grad
-        # a scale kept in another type than the rows gets its gradient from the fp32 sums
-        sums = x2.dtype if ctx.dtypes == (x2.dtype, x2.dtype) else torch.float32
-        dx, dw, db = _norm_backward(dy, x2, w2, mean, rstd, 1.0, w2.shape[0], need_x, need_w or need_b, sums)
-        return (dx.view(ctx.shapes[0]) if need_x else None,
-                dw.reshape(ctx.shapes[1]).to(ctx.dtypes[0]) if need_w else None,
-                db.reshape(ctx.shapes[2]).to(ctx.dtypes[1]) if need_b else None, None)
+        w_shape, w_dtype, b_shape, b_dtype = ctx.vectors
+        # a scale or shift kept in another type than the rows gets its gradient from the fp32 sums
+        own = w_dtype == b_dtype == x.dtype
+        make = x.new_empty if x.numel() else x.new_zeros
+        dw = make(w_shape, dtype=x.dtype if own else torch.float32) if need_w else None
+        db = make(b_shape, dtype=x.dtype if own else torch.float32) if need_b else None
+        B = w2.shape[0]
+        dx = _norm_backward(dy, x, w2, w2.stride(0) if B > 1 else 0, stats, 1.0, B, need_x, dw, db,
+                            not own or x.dtype == torch.float32)
+        if not own:
+            dw, db = dw.to(w_dtype) if need_w else None, db.to(b_dtype) if need_b else None
+        return dx, dw, db, None
+
+    _backward_once = once_differentiable(_backward.__func__)
+
+    @staticmethod
+    def backward(ctx, dy):
+        return (_LayerNormModulation._backward_once if torch.is_grad_enabled() else _LayerNormModulation._backward)(ctx, dy)
 
 
 def layer_norm_modulation(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, eps: float = 1e-5) -> torch.Tensor:
@@ -198,9 +212,9 @@ def layer_norm_modulation(x: torch.Tensor, weight: torch.Tensor, bias: torch.Ten
     assert x.shape[-1] == weight.shape[-1] == bias.shape[-1]
     _lib.require_cuda(x, weight, bias)
     _lib.require_same_device(x, weight, bias)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or bias.requires_grad):
+    if (x.requires_grad or weight.requires_grad or bias.requires_grad) and torch.is_grad_enabled():
         return _LayerNormModulation.apply(x, weight, bias, eps)
-    return _ln_mod_forward(x, weight, bias, eps, False)[2]
+    return _ln_mod_forward(x.contiguous(), weight, bias, eps, None)[1]
 
 
 class _rms_norm(torch.autograd.Function):

@@ -36,32 +36,37 @@ def apply_rope(xq: torch.Tensor, xk: torch.Tensor, freqs_cis: torch.Tensor) -> t
 _ID_TYPES = {torch.float32: _lib.ID_F32, torch.int32: _lib.ID_I32, torch.int64: _lib.ID_I64}
 
 
+_NOTHING = (None, 0, 0, 0, None, 0, 0, 0, 0)
+_axes_arrays = {}  # axes_dim -> the same as a C array
+
+
 def _rope_axes(xq, xk, ids, axes_dim, theta: float, backward: bool):
     """Rotates xq and xk (either may be None); the results have the inputs' memory layout."""
-    some = xq if xq is not None else xk
-    B, _, L, D = some.shape
-    args, outs = [], []
+    args, outs, keep = (), [], []
     for x in (xq, xk):
         if x is None:
-            args += [None, None, None, None, 0]
+            args += _NOTHING
             outs.append(None)
             continue
         if x.stride(3) != 1:
             x = x.contiguous()
+            keep.append(x)
         out = torch.empty_like(x)
-        if out.stride(3) != 1:
+        if out.stride(3) != 1:  # an input that overlaps itself
             out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        args += [x.data_ptr(), out.data_ptr(), (c_int64 * 3)(*x.stride()[:3]), (c_int64 * 3)(*out.stride()[:3]), x.shape[1]]
-        outs.append((out, x))
-    id_strides = (c_int64 * 3)(ids.stride(0) if ids.shape[0] > 1 else 0, ids.stride(1), ids.stride(2))
-    with _lib.on_device_of(some):
-        _lib.check(
-            _lib.load().fluxb_rope_axes(
-                *args, ids.data_ptr(), _ID_TYPES[ids.dtype], id_strides, B, L, D, (c_int64 * len(axes_dim))(*axes_dim),
-                len(axes_dim), theta, int(backward), _lib.dtype_code(some), _lib.stream_handle(),
-            )
-        )
-    return tuple(o[0] if o is not None else None for o in outs)
+        args += (x.data_ptr(), *x.stride()[:3], out.data_ptr(), *out.stride()[:3], x.shape[1])
+        outs.append(out)
+    some = outs[0] if xq is not None else outs[1]
+    axes = _axes_arrays.get(axes_dim)
+    if axes is None:
+        axes = _axes_arrays[axes_dim] = (c_int64 * len(axes_dim))(*axes_dim)
+    i0, i1, i2 = ids.stride()
+    B, _, L, D = some.shape
+    _lib.launch(
+        _lib.load().fluxb_rope_axes, some.get_device(), *args, ids.data_ptr(), _ID_TYPES[ids.dtype],
+        i0 if ids.shape[0] > 1 else 0, i1, i2, B, L, D, axes, len(axes_dim), theta, backward, _lib.DTYPE_CODES[some.dtype],
+    )
+    return tuple(outs)
 
 
 class _RopeAxes(torch.autograd.Function):
@@ -73,12 +78,19 @@ class _RopeAxes(torch.autograd.Function):
         return _rope_axes(xq, xk, ids, axes_dim, theta, False)
 
     @staticmethod
-    @once_differentiable
+    def _backward(ctx, dq, dk):
+        need_q, need_k = ctx.needs_input_grad[:2]
+        dq, dk = dq if need_q else None, dk if need_k else None
+        if dq is not None or dk is not None:
+            dq, dk = _rope_axes(dq, dk, ctx.saved_tensors[0], *ctx.plan, True)
+        return dq, dk, None, None, None
+
+    _backward_once = once_differentiable(_backward.__func__)
+
+    @staticmethod
     def backward(ctx, dq, dk):
-        dq, dk = (d if need else None for d, need in zip((dq, dk), ctx.needs_input_grad))
-        if dq is None and dk is None:
-            return None, None, None, None, None
-        return *_rope_axes(dq, dk, ctx.saved_tensors[0], *ctx.plan, True), None, None, None
+        # the wrapper that refuses second gradients is asked for only where somebody may take them
+        return (_RopeAxes._backward_once if torch.is_grad_enabled() else _RopeAxes._backward)(ctx, dq, dk)
 
 
 def apply_rope_axes(xq: torch.Tensor, xk: torch.Tensor, ids: torch.Tensor, axes_dim, theta: float = 10000.0
@@ -94,7 +106,7 @@ def apply_rope_axes(xq: torch.Tensor, xk: torch.Tensor, ids: torch.Tensor, axes_
     Differentiable once in xq and xk."""
     _lib.require_cuda(xq, xk, ids)
     _lib.require_same_device(xq, xk, ids)
-    axes_dim = tuple(int(d) for d in axes_dim)
+    axes_dim = tuple(axes_dim)
     assert xq.dim() == xk.dim() == 4 and xq.dtype == xk.dtype
     B, _, L, D = xq.shape
     assert xk.shape[0] == B and xk.shape[2:] == xq.shape[2:], "xq and xk differ in more than the head count"
