@@ -7,6 +7,7 @@ PyTorch fallback.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_void_p, POINTER
 from pathlib import Path
 
@@ -15,7 +16,6 @@ import torch
 LIB_PATH = Path(__file__).resolve().parent / "libfluxb200.so"
 
 F32, BF16 = 0, 1
-DTYPE_CODES = {torch.float32: F32, torch.bfloat16: BF16}
 ID_F32, ID_I32, ID_I64 = 0, 1, 2
 EPI_NONE, EPI_GELU, EPI_GATE_RESID = 0, 1, 2
 ERR_BAD_ARG, ERR_UNSUPPORTED, ERR_CUDA, ERR_TIMEOUT = -1, -2, -3, -4
@@ -128,9 +128,10 @@ def check(rc: int, launches: bool = True) -> None:
 
 
 def dtype_code(t: torch.Tensor) -> int:
-    code = DTYPE_CODES.get(t.dtype)
-    if code is not None:
-        return code
+    if t.dtype == torch.bfloat16:
+        return BF16
+    if t.dtype == torch.float32:
+        return F32
     raise NotImplementedError(f"fluxb200 kernels take float32 or bfloat16 tensors, got {t.dtype}")
 
 
@@ -146,21 +147,24 @@ def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def launch(fn, device_index: int, *args) -> None:
-    """fn(*args, stream) on the current stream of the device that the tensors are on, which is made
-    current for the call if another one is.  (The raw handle straight from torch's binding: wrapping
-    it in a Stream object first takes 3 us, as long as the launch itself.)"""
-    if device_index == torch.cuda.current_device():
-        check(fn(*args, torch._C._cuda_getCurrentRawStream(device_index)))
-        return
-    with torch.cuda.device(device_index):
-        check(fn(*args, torch._C._cuda_getCurrentRawStream(device_index)))
+def binding():
+    """The module of the operators that bind through torch's C++ API (csrc/torch_binding.cpp): calls
+    so short that a Python wrapper would cost more than their kernels.  They do not pass through
+    `check`, so `kernel_calls` does not count them."""
+    global _binding
+    if _binding is None:
+        path = LIB_PATH.parent / "_binding.so"
+        if not path.exists():
+            raise ImportError(f"{path} is missing: build it with `python -m triton_kernels_b200.build`")
+        load()
+        spec = importlib.util.spec_from_file_location("triton_kernels_b200._binding", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _binding = module
+    return _binding
 
 
-def require_same_device(first: torch.Tensor, *others: torch.Tensor) -> None:
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise RuntimeError(f"fluxb200 kernels take tensors of one device; got {first.device} and {t.device}")
+_binding = None
 
 
 def stream_handle() -> int:

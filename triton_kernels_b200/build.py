@@ -1,8 +1,10 @@
-"""Builds libfluxb200.so (the C-ABI library of sm_100a kernels) in-tree with nvcc.
+"""Builds libfluxb200.so (the C-ABI library of sm_100a kernels) in-tree with nvcc, and _binding.so
+(the Python binding of the operators that bind through torch's C++ API) with the host compiler.
 
 Run as ``python -m triton_kernels_b200.build`` or call :func:`build`.  Objects are compiled
 in parallel, one per ``csrc/*.cu`` file, and linked into ``triton_kernels_b200/libfluxb200.so``.
-A source file is recompiled only when it (or a header) is newer than its object.
+A source file is recompiled only when it (or a header) is newer than its object; the binding also
+when torch's version changes.
 """
 from __future__ import annotations
 
@@ -18,6 +20,7 @@ CSRC = PKG_DIR / "csrc"
 INCLUDE = PKG_DIR.parent / "include"
 BUILD_DIR = PKG_DIR / "build"
 LIB_PATH = PKG_DIR / "libfluxb200.so"
+BINDING_PATH = PKG_DIR / "_binding.so"
 
 NVCC_FLAGS = [
     "-std=c++17",
@@ -80,7 +83,39 @@ def build(verbose: bool = False, force: bool = False) -> Path:
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("linking libfluxb200.so failed")
+    build_binding(verbose, force)
     return LIB_PATH
+
+
+def build_binding(verbose: bool = False, force: bool = False) -> Path:
+    """Compile csrc/torch_binding.cpp against the installed torch and link it to libfluxb200.so.
+    Returns its path."""
+    import sysconfig
+
+    import torch
+
+    src = CSRC / "torch_binding.cpp"
+    stamp = BUILD_DIR / "torch_binding.version"
+    version = f"{torch.__version__} {sys.version_info[:2]}"
+    current = stamp.exists() and stamp.read_text() == version
+    if not force and current and not _stale(BINDING_PATH, [src, *INCLUDE.glob("*.h")]):
+        return BINDING_PATH
+    torch_dir = Path(torch.__file__).parent
+    includes = [torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include",
+                sysconfig.get_paths()["include"], Path(_nvcc()).parent.parent / "include", INCLUDE]
+    cmd = [
+        shutil.which("g++") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_binding",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{p}" for p in includes), str(src),
+        "-o", str(BINDING_PATH), f"-L{PKG_DIR}", "-l:libfluxb200.so", f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu",
+        "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN",
+    ]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or r.returncode != 0:
+        sys.stderr.write(f"--- g++ {src.name}\n{r.stdout}{r.stderr}\n")
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {src.name}")
+    stamp.write_text(version)
+    return BINDING_PATH
 
 
 if __name__ == "__main__":

@@ -210,12 +210,6 @@ def linear(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None, activation:
     return y.reshape(*lead, N)
 
 
-def _dense16(t: torch.Tensor) -> torch.Tensor:
-    """t contiguous and 16-byte aligned; a copy where it is not."""
-    t = t.contiguous()
-    return t.clone() if t.data_ptr() % 16 else t
-
-
 def linear_lora(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None, lora_a: torch.Tensor, lora_b: torch.Tensor,
                 adapter: torch.Tensor, lora_scale: torch.Tensor | None = None, activation: str = "") -> torch.Tensor:
     """act(x @ w.T + b + scale_a * (x @ A_a.T) @ B_a.T): a projection shared by all requests plus one
@@ -227,45 +221,5 @@ def linear_lora(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None, lora_a
     values of `adapter` are read on the device: one outside [-1, n) counts as -1 and is recorded in
     the device status word (`_lib.device_status`).  R <= 256; an R that is not a multiple of 8 copies
     lora_b on every call (keep it padded with zeros instead).  activation: "" or "GELU" (tanh form)."""
-    assert x.dim() >= 2 and x.shape[-1] == w.shape[-1], "Incompatible dimensions"
-    N, K = w.shape
-    n, R = lora_a.shape[:2]
-    assert n > 0 and R > 0 and lora_a.shape == (n, R, K) and lora_b.shape == (n, N, R), (
-        f"lora_a must be [n, R, {K}] and lora_b [n, {N}, R], got {tuple(lora_a.shape)} and {tuple(lora_b.shape)}")
-    assert adapter.shape == x.shape[:1], "adapter holds one index per request (x's first dim)"
-    assert b is None or b.shape == (N,)
-    assert lora_scale is None or lora_scale.shape == (n,)
     assert activation in ("", "GELU"), f"unknown activation {activation!r}"
-    _lib.require_cuda(x, w, b, lora_a, lora_b, adapter, lora_scale)
-    _lib.require_same_device(x, w, b, lora_a, lora_b, adapter, lora_scale)
-    for t in (x, w, lora_a, lora_b):
-        if t.dtype != torch.bfloat16:
-            raise UnsupportedDtype(t.dtype)
-    if adapter.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"adapter indices are int32 or int64, got {adapter.dtype}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, lora_a, lora_b, lora_scale)):
-        raise NotImplementedError("linear_lora is forward only: call it under torch.no_grad() or detach its inputs")
-    B = x.shape[0]
-    y = torch.empty((*x.shape[:-1], N), device=x.device, dtype=x.dtype)
-    if y.numel() == 0:
-        return y
-    x2d = _as_2d(x, K)
-    M = x2d.shape[0]
-    if w.stride(1) != 1 or w.stride(0) % 8 or w.data_ptr() % 16:
-        w = _dense16(w)
-    if b is not None:
-        b = _dense16(b.to(torch.bfloat16))
-    if R % 8:  # rows of B that no 16-byte piece fits are copied into wider ones
-        lora_b = torch.nn.functional.pad(lora_b, (0, -R % 8))
-    lora_a, lora_b = _dense16(lora_a), _dense16(lora_b)
-    if lora_scale is not None:
-        lora_scale = lora_scale.to(torch.float32).contiguous()
-    adapter = adapter.contiguous()
-    lib = _lib.load()
-    scratch = torch.empty(lib.fluxb_linear_lora_scratch_bytes(M, N, K, R), device=x.device, dtype=torch.uint8)
-    _lib.launch(
-        lib.fluxb_linear_lora, x.get_device(), x2d.data_ptr(), w.data_ptr(), _lib.ptr(b), y.data_ptr(), lora_a.data_ptr(),
-        lora_b.data_ptr(), _lib.ptr(lora_scale), adapter.data_ptr(), adapter.dtype == torch.int64, scratch.data_ptr(), B, M // B,
-        N, K, R, n, x2d.stride(0), w.stride(0), N, lora_b.shape[2], _lib.EPI_GELU if activation else _lib.EPI_NONE,
-    )
-    return y
+    return _lib.binding().linear_lora(x, w, b, lora_a, lora_b, adapter, lora_scale, activation == "GELU")
