@@ -352,14 +352,14 @@ __device__ __forceinline__ int find_problem(const G& g, int tile) {
   return i;
 }
 
-// The adapters of a tile's W x 32 rows, one warp.  fetch() asks for the indices, which next() looks at only behind the
-// tile's K loop, so that nobody waits for them (waiting at the head of each tile cost 5 % of the joint q|k|v
-// projection).  next() gives the adapter of the first row that is left, with the mask of the rows that do NOT use it
-// (bit set: row left alone), or -1.  A tile inside one request, the ordinary case of long requests, is one index and
-// an empty mask; else lane l holds rows l, 32 + l, ...
+// The adapters of a tile's W x 32 rows, as the producer warp finds them.  fetch() asks for the indices, well ahead of
+// begin() and next(), so that nobody waits for them.  next() gives the adapter of the first row that is left, with the
+// mask of the rows that do NOT use it (bit set: row left alone), or -1.  A tile inside one request, the ordinary case of
+// long requests, is one index and an empty mask; else lane l holds rows l, 32 + l, ...
 template <int W>
 struct TileAdapters {
   int64_t raw[W];
+  int a[W];
   int n_adapters;
   bool single;
   __device__ __forceinline__ void fetch(const RequestAdapters& req, int row0, int rows, int lane) {
@@ -376,30 +376,43 @@ struct TileAdapters {
       raw[i] = row < rows ? req.raw(row / req.length) : -1;
     }
   }
-  __device__ __forceinline__ bool valid(int64_t a) const { return a >= 0 && a < n_adapters; }
+  // What next() walks over, behind the K loop: the indices as 32-bit numbers, -1 for none.
+  __device__ __forceinline__ void begin() {
+#pragma unroll
+    for (int i = 0; i < W; ++i) a[i] = raw[i] >= 0 && raw[i] < n_adapters ? (int)raw[i] : -1;
+  }
   __device__ __forceinline__ int next(uint32_t (&off)[W]) {
-    int cur = -1;
     if (single) {
-      if (valid(raw[0])) cur = (int)raw[0];
-      raw[0] = -1;
+      const int cur = a[0];
+      a[0] = -1;
 #pragma unroll
       for (int i = 0; i < W; ++i) off[i] = 0;
       return cur;
     }
+    uint32_t left = 0;
+    int mine = -1;
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-      const uint32_t left = __ballot_sync(0xffffffffu, valid(raw[i]));
-      const int first = __shfl_sync(0xffffffffu, (int)raw[i], left != 0 ? __ffs(left) - 1 : 0);
-      if (cur < 0 && left != 0) cur = first;
+    for (int i = W - 1; i >= 0; --i) {
+      const uint32_t here = __ballot_sync(0xffffffffu, a[i] >= 0);
+      if (here != 0) { left = here; mine = a[i]; }  // (the same word for all lanes)
     }
-    if (cur < 0) return cur;
+    if (left == 0) return -1;
+    const int cur = __shfl_sync(0xffffffffu, mine, __ffs(left) - 1);
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-      off[i] = ~__ballot_sync(0xffffffffu, raw[i] == cur);
-      if (raw[i] == cur) raw[i] = -1;
+      off[i] = ~__ballot_sync(0xffffffffu, a[i] == cur);
+      if (a[i] == cur) a[i] = -1;
     }
     return cur;
   }
+};
+// What the producer leaves beside a ring slot for the MMA warp: of an adapter's slot the mask of the rows that it leaves
+// alone, and of the last slot of a K loop and of every adapter's whether another adapter's slot follows.  The MMA warp
+// reads it behind its wait for the slot (the producer's arrival there releases it) and so has nothing to find out.
+template <int W>
+struct SlotNote {
+  uint32_t off[W];
+  uint32_t more;
 };
 // A ring slot of the adapters: a line of t and a group of B; a group of 64 takes two (high parts, low parts).
 __device__ __forceinline__ int lora_slots(const LowRank& low) { return low.group == 64 ? 2 * low.groups : low.groups; }
@@ -582,6 +595,7 @@ gemm_pair_kernel(const __grid_constant__ G g) {
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
+  __shared__ SlotNote<8> notes[kMode == 3 ? STAGES : 1];  // (kMode 3 alone uses it)
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -628,48 +642,70 @@ gemm_pair_kernel(const __grid_constant__ G g) {
       const Problem& pr = g.prob[0];
       const Params& p = pr.p;
       const int num_kb = (p.K + BK - 1) / BK;
+      // The next tile's coordinates and indices are taken while the current one's loads are under way: between tiles the
+      // ring drains (0.6 us per tile of the joint q|k|v projection, 3 %).
+      int m_blk = 0, n_blk = 0, next_m = 0, next_n = 0;
+      TileAdapters<8> rows, next_rows;
+      tile_coords(p, pair_id, pr.tiles_m, next_m, next_n);
+      next_rows.fetch(g.req, next_m * 2 * BM, p.M, lane);
       for (int tile = pair_id; ok && tile < num_tiles; tile += num_pairs) {
-        int m_blk, n_blk;
-        tile_coords(p, tile, pr.tiles_m, m_blk, n_blk);
+        m_blk = next_m;
+        n_blk = next_n;
+        rows = next_rows;
         const int row0 = m_blk * 2 * BM + (int)rank * BM;
         const int col0 = n_blk * BN + (int)rank * BNH;
-        TileAdapters<8> rows;
-        rows.fetch(g.req, m_blk * 2 * BM, p.M, lane);
-        if (lane == 0) {
-          for (int kb = 0; kb < num_kb; ++kb) {
+        uint32_t off[8], next_off[8];
+        int cur = -1;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (kb == num_kb - 1) {
+            rows.begin();
+            cur = rows.next(off);
+          }
+          if (ok && lane == 0) {
             ok = mbar_wait_cluster(&empty_bar[stage], phase ^ 1, abort_flag, status, 41);
-            if (!ok) break;
-            if (leader) mbar_expect_tx(&full_bar[stage], 2 * STAGE_BYTES);
-            const uint32_t full_addr = map_to_cta(smem_u32(&full_bar[stage]), 0);
-            uint8_t* a_dst = smem + stage * STAGE_BYTES;
-            tma_load_2d_pair(a_dst, &pr.tm_a, full_addr, kb * BK, row0);
-            tma_load_2d_pair(a_dst + A_BYTES, &pr.tm_b, full_addr, kb * BK, col0);
-            if (++stage == g.pair_stages) { stage = 0; phase ^= 1; }
+            if (ok) {
+              if (kb == num_kb - 1) notes[stage].more = cur >= 0;
+              if (leader) mbar_expect_tx(&full_bar[stage], 2 * STAGE_BYTES);
+              const uint32_t full_addr = map_to_cta(smem_u32(&full_bar[stage]), 0);
+              uint8_t* a_dst = smem + stage * STAGE_BYTES;
+              tma_load_2d_pair(a_dst, &pr.tm_a, full_addr, kb * BK, row0);
+              tma_load_2d_pair(a_dst + A_BYTES, &pr.tm_b, full_addr, kb * BK, col0);
+              if (++stage == g.pair_stages) { stage = 0; phase ^= 1; }
+            }
+          }
+          if (kb == num_kb / 2 && tile + num_pairs < num_tiles) {
+            tile_coords(p, tile + num_pairs, pr.tiles_m, next_m, next_n);
+            next_rows.fetch(g.req, next_m * 2 * BM, p.M, lane);
           }
         }
         __syncwarp();
-        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-        stage = __shfl_sync(0xffffffffu, stage, 0);
-        phase = __shfl_sync(0xffffffffu, phase, 0);
         if (tile == pair_id) pdl_wait();  // t is complete; every CTA passes here, with adapters or without
-        uint32_t off[8];
-        for (int cur; ok && (cur = rows.next(off)) >= 0;) {
-          for (int q = 0; q < lora_slots(g.low); ++q) {
-            if (ok && lane == 0) {
+        // (lane 0 alone knows the ring's position and whether a wait gave up; the others only help to find the adapters)
+        while (cur >= 0) {
+          const int next = rows.next(next_off);
+          if (lane == 0) {
+            const int slots = lora_slots(g.low);
+            for (int q = 0; ok && q < slots; ++q) {
               ok = mbar_wait_cluster(&empty_bar[stage], phase ^ 1, abort_flag, status, 46);
-              if (ok) {
-                const int line = g.low.group == 16 ? 32 : 64;
-                if (leader) mbar_expect_tx(&full_bar[stage], 2 * (BM * line * 2 + BNH * g.low.group * 2));
-                const uint32_t full_addr = map_to_cta(smem_u32(&full_bar[stage]), 0);
-                uint8_t* a_dst = smem + stage * STAGE_BYTES;
-                tma_load_2d_pair(a_dst, &g.tm_t, full_addr, q * line, row0);
-                tma_load_3d_pair(a_dst + A_BYTES, &g.tm_b, full_addr, (g.low.group == 64 ? q >> 1 : q) * g.low.group, col0, cur);
-              }
+              if (!ok) break;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) notes[stage].off[i] = off[i];
+              notes[stage].more = q + 1 < slots || next >= 0;
+              const int line = g.low.group == 16 ? 32 : 64;
+              if (leader) mbar_expect_tx(&full_bar[stage], 2 * (BM * line * 2 + BNH * g.low.group * 2));
+              const uint32_t full_addr = map_to_cta(smem_u32(&full_bar[stage]), 0);
+              uint8_t* a_dst = smem + stage * STAGE_BYTES;
+              tma_load_2d_pair(a_dst, &g.tm_t, full_addr, q * line, row0);
+              tma_load_3d_pair(a_dst + A_BYTES, &g.tm_b, full_addr, (g.low.group == 64 ? q >> 1 : q) * g.low.group, col0, cur);
+              if (++stage == g.pair_stages) { stage = 0; phase ^= 1; }
             }
-            if (++stage == g.pair_stages) { stage = 0; phase ^= 1; }
           }
-          ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+          __syncwarp();
+          cur = next;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) off[i] = next_off[i];
         }
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
       }
     }
     __syncwarp();
@@ -709,7 +745,7 @@ gemm_pair_kernel(const __grid_constant__ G g) {
       int local = 0;
       for (int tile = pair_id; ok && tile < num_tiles; tile += num_pairs, ++local) {
         const int num_kb = (g.prob[find_problem(g, tile)].p.K + BK - 1) / BK;
-        TileAdapters<8> rows;
+        uint32_t more = 0;
         const int acc = local & 1;
         const uint32_t acc_phase = (local >> 1) & 1;
         if (!__all_sync(0xffffffffu, mbar_wait_cluster(&acc_empty[acc], acc_phase ^ 1, abort_flag, status, 43))) { ok = false; break; }
@@ -718,6 +754,9 @@ gemm_pair_kernel(const __grid_constant__ G g) {
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!__all_sync(0xffffffffu, mbar_wait_cluster(&full_bar[stage], phase, abort_flag, status, 44))) { ok = false; break; }
           tc_fence_after_sync();
+          if constexpr (kMode == 3) {
+            if (kb == num_kb - 1) more = notes[stage].more;  // before the slot is given back
+          }
           const uint32_t a_addr = smem_u32(smem + stage * STAGE_BYTES);
           const uint64_t adesc = make_smem_desc(a_addr, 16, 1024);
           const uint64_t bdesc = make_smem_desc(a_addr + A_BYTES, 16, 1024);
@@ -728,37 +767,30 @@ gemm_pair_kernel(const __grid_constant__ G g) {
             umma_commit_pair_both(&empty_bar[stage]);
           }
           if (++stage == g.pair_stages) { stage = 0; phase ^= 1; }
-          if constexpr (kMode == 3) {
-            if (kb == 0) {  // with MMAs under way
-              int m_blk, n_blk;
-              tile_coords(g.prob[0].p, tile, g.prob[0].tiles_m, m_blk, n_blk);
-              rows.fetch(g.req, m_blk * 2 * BM, g.prob[0].p.M, lane);
-            }
-          }
         }
         if constexpr (kMode == 3) {
-          uint32_t off[8];
-          for (int cur; ok && (cur = rows.next(off)) >= 0;) {
-            for (int q = 0; ok && q < lora_slots(g.low); ++q) {
-              ok = __all_sync(0xffffffffu, mbar_wait_cluster(&full_bar[stage], phase, abort_flag, status, 47));
-              if (!ok) break;
-              tc_fence_after_sync();
-              const uint32_t a_addr = smem_u32(smem + stage * STAGE_BYTES);
-              const uint64_t adesc = g.low.desc(a_addr);
-              const uint64_t bdesc = g.low.group == 64   ? make_smem_desc(a_addr + A_BYTES, 16, 1024)
-                                     : g.low.group == 32 ? make_smem_desc(a_addr + A_BYTES, 16, 512, 4)
-                                                         : make_smem_desc(a_addr + A_BYTES, 16, 256, 6);
-              const int first = (g.low.group == 64 ? q >> 1 : q) * (g.low.group / 16);
-              const int n_units = min(g.low.group / 16, g.low.units - first);
-              if (elect_one()) {
-                for (int i = 0; i < n_units; ++i) {
-                  umma_ss_pair_masked(d_tmem, adesc + 2 * i, bdesc + 2 * i, idesc, off);
-                  if (g.low.group < 64) umma_ss_pair_masked(d_tmem, adesc + g.low.low(i), bdesc + 2 * i, idesc, off);
-                }
-                umma_commit_pair_both(&empty_bar[stage]);
+          for (int q = 0; ok && more != 0; ++q) {
+            ok = __all_sync(0xffffffffu, mbar_wait_cluster(&full_bar[stage], phase, abort_flag, status, 47));
+            if (!ok) break;
+            tc_fence_after_sync();
+            const SlotNote<8> note = notes[stage];
+            more = note.more;
+            const uint32_t a_addr = smem_u32(smem + stage * STAGE_BYTES);
+            const uint64_t adesc = g.low.desc(a_addr);
+            const uint64_t bdesc = g.low.group == 64   ? make_smem_desc(a_addr + A_BYTES, 16, 1024)
+                                   : g.low.group == 32 ? make_smem_desc(a_addr + A_BYTES, 16, 512, 4)
+                                                       : make_smem_desc(a_addr + A_BYTES, 16, 256, 6);
+            // which of the adapter's slots: of a group of 64 two, of a smaller one one
+            const int first = g.low.group == 64 ? (q % (2 * g.low.groups) >> 1) * 4 : 0;
+            const int n_units = min(g.low.group / 16, g.low.units - first);
+            if (elect_one()) {
+              for (int i = 0; i < n_units; ++i) {
+                umma_ss_pair_masked(d_tmem, adesc + 2 * i, bdesc + 2 * i, idesc, note.off);
+                if (g.low.group < 64) umma_ss_pair_masked(d_tmem, adesc + g.low.low(i), bdesc + 2 * i, idesc, note.off);
               }
-              if (++stage == g.pair_stages) { stage = 0; phase ^= 1; }
+              umma_commit_pair_both(&empty_bar[stage]);
             }
+            if (++stage == g.pair_stages) { stage = 0; phase ^= 1; }
           }
         }
         if (ok && elect_one()) umma_commit_pair_both(&acc_full[acc]);
@@ -866,6 +898,7 @@ using gemm::BK;
 using gemm::BM;
 using gemm::Params;
 using gemm::epilogue_chunk;
+using gemm2::SlotNote;
 using gemm2::TileAdapters;
 constexpr int THREADS = 192;
 constexpr int MAX_STAGES = 16;
@@ -886,6 +919,7 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
   const int A_BYTES = g.a_rows * BK * 2, STAGE_BYTES = A_BYTES + BN * BK * 2;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], acc_full[2], acc_empty[2], t_full, t_empty;
+  __shared__ SlotNote<4> notes[MAX_STAGES];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   uint8_t* t_smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -932,26 +966,32 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
       const int row0 = tile % p.tiles_m * BM, col0 = tile / p.tiles_m * BN;
       TileAdapters<4> rows;
       rows.fetch(g.req, row0, p.M, lane);
-      if (lane == 0) {
-        for (int kb = 0; kb < num_kb; ++kb) {
+      uint32_t off[4], next_off[4];
+      int cur = -1;
+      for (int kb = 0; kb < num_kb; ++kb) {
+        if (kb == num_kb - 1) {
+          rows.begin();
+          cur = rows.next(off);
+        }
+        if (ok && lane == 0) {
           ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, 91);
-          if (!ok) break;
-          uint8_t* dst = smem + stage * STAGE_BYTES;
-          mbar_expect_tx(&full_bar[stage], STAGE_BYTES);
-          tma_load_2d(dst, &g.tm_a, &full_bar[stage], kb * BK, row0);
-          tma_load_2d(dst + A_BYTES, &g.tm_b, &full_bar[stage], kb * BK, col0);
-          if (++stage == g.stages) { stage = 0; phase ^= 1; }
+          if (ok) {
+            if (kb == num_kb - 1) notes[stage].more = cur >= 0;
+            uint8_t* dst = smem + stage * STAGE_BYTES;
+            mbar_expect_tx(&full_bar[stage], STAGE_BYTES);
+            tma_load_2d(dst, &g.tm_a, &full_bar[stage], kb * BK, row0);
+            tma_load_2d(dst + A_BYTES, &g.tm_b, &full_bar[stage], kb * BK, col0);
+            if (++stage == g.stages) { stage = 0; phase ^= 1; }
+          }
         }
       }
       __syncwarp();
-      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-      stage = __shfl_sync(0xffffffffu, stage, 0);
-      phase = __shfl_sync(0xffffffffu, phase, 0);
       if (tile == (int)blockIdx.x) pdl_wait();  // t is complete
-      uint32_t off[4];
       bool first = true;
-      for (int cur; ok && (cur = rows.next(off)) >= 0;) {
-        if (lane == 0) {
+      // (lane 0 alone knows the ring's position and whether a wait gave up; the others only help to find the adapters)
+      while (cur >= 0) {
+        const int next = rows.next(next_off);
+        if (ok && lane == 0) {
           if (first) {
             ok = mbar_wait(&t_empty, t_phase ^ 1, abort_flag, p.status, 92);
             if (ok) {
@@ -963,6 +1003,9 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
           for (int q = 0; ok && q < slots; ++q) {
             ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, 93);
             if (!ok) break;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) notes[stage].off[i] = off[i];
+            notes[stage].more = q + 1 < slots || next >= 0;
             mbar_expect_tx(&full_bar[stage], BN * BK * 2);
             tma_load_3d(smem + stage * STAGE_BYTES + A_BYTES, &g.tm_lb, &full_bar[stage], q * 64, col0, cur);
             if (++stage == g.stages) { stage = 0; phase ^= 1; }
@@ -970,11 +1013,11 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
         }
         if (first) t_phase ^= 1;
         first = false;
-        __syncwarp();
-        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-        stage = __shfl_sync(0xffffffffu, stage, 0);
-        phase = __shfl_sync(0xffffffffu, phase, 0);
+        cur = next;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) off[i] = next_off[i];
       }
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -984,18 +1027,18 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
     bool ok = true;
     int local = 0;
     for (int tile = blockIdx.x; ok && tile < p.num_tiles; tile += gridDim.x, ++local) {
-      TileAdapters<4> rows;
-      rows.fetch(g.req, tile % p.tiles_m * BM, p.M, lane);
       const int acc = local & 1;
       const uint32_t acc_phase = (local >> 1) & 1;
       ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[acc], acc_phase ^ 1, abort_flag, p.status, 94));
       if (!ok) break;
       tc_fence_after_sync();
       const uint32_t d_tmem = tmem_base + acc * BN;
+      uint32_t more = 0;
       for (int kb = 0; kb < num_kb; ++kb) {
         ok = __all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, abort_flag, p.status, 95));
         if (!ok) break;
         tc_fence_after_sync();
+        if (kb == num_kb - 1) more = notes[stage].more;  // before the slot is given back
         const uint32_t a_addr = smem_u32(smem + stage * STAGE_BYTES);
         const uint64_t adesc = make_smem_desc(a_addr, 16, 1024), bdesc = make_smem_desc(a_addr + A_BYTES, 16, 1024);
         if (elect_one()) {
@@ -1005,32 +1048,33 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
         }
         if (++stage == g.stages) { stage = 0; phase ^= 1; }
       }
-      uint32_t off[4];
-      bool first = true;
-      for (int cur; ok && (cur = rows.next(off)) >= 0;) {
-        if (first) ok = __all_sync(0xffffffffu, mbar_wait(&t_full, t_phase, abort_flag, p.status, 96));
-        for (int q = 0; ok && q < slots; ++q) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, abort_flag, p.status, 97));
-          if (!ok) break;
-          tc_fence_after_sync();
-          // (more than 64 ranks: groups of 64, one per slot; up to 64 there is one group and one slot)
-          const uint64_t adesc = g.low.desc(smem_u32(t_smem + q * g.low.tile_bytes()));
-          const uint64_t bdesc = make_smem_desc(smem_u32(smem + stage * STAGE_BYTES) + A_BYTES, 16, 1024);
-          const int n_units = min(4, g.low.units - q * 4);
-          if (elect_one()) {
-            for (int i = 0; i < n_units; ++i) {
-              umma_ss_masked(d_tmem, adesc + g.low.high(i), bdesc + 2 * i, idesc, off);
-              umma_ss_masked(d_tmem, adesc + g.low.low(i), bdesc + 2 * i, idesc, off);
-            }
-            umma_commit(&empty_bar[stage]);
+      const bool any = more != 0;
+      if (ok && any) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&t_full, t_phase, abort_flag, p.status, 96));
+        t_phase ^= 1;
+      }
+      for (int q = 0; ok && more != 0;) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, abort_flag, p.status, 97));
+        if (!ok) break;
+        tc_fence_after_sync();
+        const SlotNote<4> note = notes[stage];
+        more = note.more;
+        // (more than 64 ranks: groups of 64, one per slot; up to 64 there is one group and one slot)
+        const uint64_t adesc = g.low.desc(smem_u32(t_smem + q * g.low.tile_bytes()));
+        const uint64_t bdesc = make_smem_desc(smem_u32(smem + stage * STAGE_BYTES) + A_BYTES, 16, 1024);
+        const int n_units = min(4, g.low.units - q * 4);
+        if (elect_one()) {
+          for (int i = 0; i < n_units; ++i) {
+            umma_ss_masked(d_tmem, adesc + g.low.high(i), bdesc + 2 * i, idesc, note.off);
+            umma_ss_masked(d_tmem, adesc + g.low.low(i), bdesc + 2 * i, idesc, note.off);
           }
-          if (++stage == g.stages) { stage = 0; phase ^= 1; }
+          umma_commit(&empty_bar[stage]);
         }
-        if (first) t_phase ^= 1;
-        first = false;
+        if (++q == slots) q = 0;
+        if (++stage == g.stages) { stage = 0; phase ^= 1; }
       }
       if (ok && elect_one()) {
-        if (!first) umma_commit(&t_empty);
+        if (any) umma_commit(&t_empty);
         umma_commit(&acc_full[acc]);
       }
     }

@@ -28,9 +28,9 @@ struct Params {
   DeviceStatus* status;
 };
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
   return v;
 }
 
@@ -119,7 +119,10 @@ __global__ void __launch_bounds__(THREADS, 1) lora_shrink_kernel(const __grid_co
     if (ok && elect_one()) umma_commit(&acc_full);
     __syncwarp();
   }
-  float* part = reinterpret_cast<float*>(smem);  // [rpad][128]: the ring's memory, free once the last MMA is done
+  // [128][rpad + 4], the ring's memory, free once the last MMA is done; the four floats behind each row spread the rows
+  // over the banks
+  float* part = reinterpret_cast<float*>(smem);
+  const int pitch = p.rpad + 4;
   bool ok = true;
   if (warp >= 2) {
     const int quad = warp & 3;
@@ -133,7 +136,8 @@ __global__ void __launch_bounds__(THREADS, 1) lora_shrink_kernel(const __grid_co
         tmem_ld_x16(t_addr + c, r);
         tmem_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) part[(c + e) * BM + quad * 32 + lane] = __uint_as_float(r[e]);
+        for (int e = 0; e < 16; e += 4)
+          *reinterpret_cast<uint4*>(part + (quad * 32 + lane) * pitch + c + e) = make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
       }
     }
   }
@@ -146,14 +150,25 @@ __global__ void __launch_bounds__(THREADS, 1) lora_shrink_kernel(const __grid_co
   cluster_sync_all();
   const float scale = p.scale != nullptr ? p.scale[adapter] : 1.f;
   const int t_ld = p.low.ld();
-  for (int i = rank * THREADS + threadIdx.x; i < p.rpad / 8 * BM; i += p.ksplit * THREADS) {
-    const int row = i & (BM - 1), c8 = i / BM * 8;
-    if (row >= rows) continue;
-    float v[8] = {};
-    for (int s = 0; s < p.ksplit; ++s) {
-      const uint32_t src = map_to_cta(smem_u32(part + c8 * BM + row), (uint32_t)s);
+  const int eights = p.rpad / 8;
+  for (int i = rank * THREADS + threadIdx.x; i < eights * rows; i += p.ksplit * THREADS) {
+    const int row = i / eights, c8 = (i - row * eights) * 8;
+    float4 lo4[8], hi4[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += ld_cluster_f32(src + e * BM * 4);
+    for (int s = 0; s < 8; ++s) {
+      if (s < p.ksplit) {
+        const uint32_t src = map_to_cta(smem_u32(part + row * pitch + c8), (uint32_t)s);
+        lo4[s] = ld_cluster_f32x4(src);
+        hi4[s] = ld_cluster_f32x4(src + 16);
+      }
+    }
+    float v[8] = {};
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      if (s < p.ksplit) {
+        v[0] += lo4[s].x; v[1] += lo4[s].y; v[2] += lo4[s].z; v[3] += lo4[s].w;
+        v[4] += hi4[s].x; v[5] += hi4[s].y; v[6] += hi4[s].z; v[7] += hi4[s].w;
+      }
     }
     uint32_t hi[4], lo[4];
 #pragma unroll
@@ -197,7 +212,7 @@ static int launch_shrink(const void* x, int64_t ldx, const void* lora_a, const f
   p.stages = MAX_SMEM / stage_bytes < MAX_STAGES ? MAX_SMEM / stage_bytes : MAX_STAGES;
   if (p.stages > steps) p.stages = steps;
   int smem = p.stages * stage_bytes;
-  if (smem < p.rpad * BM * 4) smem = p.rpad * BM * 4;
+  if (smem < (p.rpad + 4) * BM * 4) smem = (p.rpad + 4) * BM * 4;
   smem += 1024;
   p.tmem_cols = 32;
   while (p.tmem_cols < p.rpad) p.tmem_cols *= 2;
@@ -259,6 +274,7 @@ __global__ void __launch_bounds__(128) lora_shrink_short_kernel(const ShortParam
   const int ranks = p.low.units * 16;  // the ranks behind R are zeros: the tensor cores multiply them, too
   const int request = blockIdx.x / (ranks / kRanks), j0 = (blockIdx.x - request * (ranks / kRanks)) * kRanks;
   const int L = p.req.length, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_release();  // (its stream of W does not get in front: the loads here are all on their way within the launch)
   const int adapter = p.req.of_request(request);
   if (adapter < 0) {
     if (j0 == 0 && threadIdx.x == 0 && p.req.raw(request) != -1) report_error(p.status, FLUXB_ERR_BAD_ARG, 81);
@@ -295,7 +311,6 @@ __global__ void __launch_bounds__(128) lora_shrink_short_kernel(const ShortParam
       }
     }
   }
-  pdl_release();  // behind the loads: the projection's stream of W would get in front of them
 #pragma unroll
   for (int l = 0; l < SHORT; ++l) {
     if (l < L) {
