@@ -661,17 +661,17 @@ gemm_pair_kernel(const __grid_constant__ G g) {
             rows.begin();
             cur = rows.next(off);
           }
-          if (ok && lane == 0) {
-            ok = mbar_wait_cluster(&empty_bar[stage], phase ^ 1, abort_flag, status, 41);
-            if (ok) {
+          ok = ok && __all_sync(0xffffffffu, mbar_wait_cluster(&empty_bar[stage], phase ^ 1, abort_flag, status, 41));
+          if (ok) {
+            const uint32_t full_addr = map_to_cta(smem_u32(&full_bar[stage]), 0);
+            uint8_t* a_dst = smem + stage * STAGE_BYTES;
+            if (elect_one()) {
               if (kb == num_kb - 1) notes[stage].more = cur >= 0;
               if (leader) mbar_expect_tx(&full_bar[stage], 2 * STAGE_BYTES);
-              const uint32_t full_addr = map_to_cta(smem_u32(&full_bar[stage]), 0);
-              uint8_t* a_dst = smem + stage * STAGE_BYTES;
               tma_load_2d_pair(a_dst, &pr.tm_a, full_addr, kb * BK, row0);
               tma_load_2d_pair(a_dst + A_BYTES, &pr.tm_b, full_addr, kb * BK, col0);
-              if (++stage == g.pair_stages) { stage = 0; phase ^= 1; }
             }
+            if (++stage == g.pair_stages) { stage = 0; phase ^= 1; }
           }
           if (kb == num_kb / 2 && tile + num_pairs < num_tiles) {
             tile_coords(p, tile + num_pairs, pr.tiles_m, next_m, next_n);
@@ -680,32 +680,28 @@ gemm_pair_kernel(const __grid_constant__ G g) {
         }
         __syncwarp();
         if (tile == pair_id) pdl_wait();  // t is complete; every CTA passes here, with adapters or without
-        // (lane 0 alone knows the ring's position and whether a wait gave up; the others only help to find the adapters)
+        const int slots = lora_slots(g.low), line = g.low.group == 16 ? 32 : 64;
         while (cur >= 0) {
           const int next = rows.next(next_off);
-          if (lane == 0) {
-            const int slots = lora_slots(g.low);
-            for (int q = 0; ok && q < slots; ++q) {
-              ok = mbar_wait_cluster(&empty_bar[stage], phase ^ 1, abort_flag, status, 46);
-              if (!ok) break;
+          for (int q = 0; ok && q < slots; ++q) {
+            ok = __all_sync(0xffffffffu, mbar_wait_cluster(&empty_bar[stage], phase ^ 1, abort_flag, status, 46));
+            if (!ok) break;
+            const uint32_t full_addr = map_to_cta(smem_u32(&full_bar[stage]), 0);
+            uint8_t* a_dst = smem + stage * STAGE_BYTES;
+            if (elect_one()) {
 #pragma unroll
               for (int i = 0; i < 8; ++i) notes[stage].off[i] = off[i];
               notes[stage].more = q + 1 < slots || next >= 0;
-              const int line = g.low.group == 16 ? 32 : 64;
               if (leader) mbar_expect_tx(&full_bar[stage], 2 * (BM * line * 2 + BNH * g.low.group * 2));
-              const uint32_t full_addr = map_to_cta(smem_u32(&full_bar[stage]), 0);
-              uint8_t* a_dst = smem + stage * STAGE_BYTES;
               tma_load_2d_pair(a_dst, &g.tm_t, full_addr, q * line, row0);
               tma_load_3d_pair(a_dst + A_BYTES, &g.tm_b, full_addr, (g.low.group == 64 ? q >> 1 : q) * g.low.group, col0, cur);
-              if (++stage == g.pair_stages) { stage = 0; phase ^= 1; }
             }
+            if (++stage == g.pair_stages) { stage = 0; phase ^= 1; }
           }
-          __syncwarp();
           cur = next;
 #pragma unroll
           for (int i = 0; i < 8; ++i) off[i] = next_off[i];
         }
-        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
       }
     }
     __syncwarp();
@@ -973,43 +969,42 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
           rows.begin();
           cur = rows.next(off);
         }
-        if (ok && lane == 0) {
-          ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, 91);
-          if (ok) {
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, 91));
+        if (ok) {
+          uint8_t* dst = smem + stage * STAGE_BYTES;
+          if (elect_one()) {
             if (kb == num_kb - 1) notes[stage].more = cur >= 0;
-            uint8_t* dst = smem + stage * STAGE_BYTES;
             mbar_expect_tx(&full_bar[stage], STAGE_BYTES);
             tma_load_2d(dst, &g.tm_a, &full_bar[stage], kb * BK, row0);
             tma_load_2d(dst + A_BYTES, &g.tm_b, &full_bar[stage], kb * BK, col0);
-            if (++stage == g.stages) { stage = 0; phase ^= 1; }
           }
+          if (++stage == g.stages) { stage = 0; phase ^= 1; }
         }
       }
       __syncwarp();
       if (tile == (int)blockIdx.x) pdl_wait();  // t is complete
       bool first = true;
-      // (lane 0 alone knows the ring's position and whether a wait gave up; the others only help to find the adapters)
       while (cur >= 0) {
         const int next = rows.next(next_off);
-        if (ok && lane == 0) {
-          if (first) {
-            ok = mbar_wait(&t_empty, t_phase ^ 1, abort_flag, p.status, 92);
-            if (ok) {
-              const int line = g.low.group == 16 ? 32 : 64;
-              mbar_expect_tx(&t_full, T_BYTES);
-              for (int c = 0; c < g.low.ld(); c += line) tma_load_2d(t_smem + c * BM * 2, &g.tm_t, &t_full, c, row0);
-            }
+        if (first) {
+          ok = ok && __all_sync(0xffffffffu, mbar_wait(&t_empty, t_phase ^ 1, abort_flag, p.status, 92));
+          if (ok && elect_one()) {
+            const int line = g.low.group == 16 ? 32 : 64;
+            mbar_expect_tx(&t_full, T_BYTES);
+            for (int c = 0; c < g.low.ld(); c += line) tma_load_2d(t_smem + c * BM * 2, &g.tm_t, &t_full, c, row0);
           }
-          for (int q = 0; ok && q < slots; ++q) {
-            ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, 93);
-            if (!ok) break;
+        }
+        for (int q = 0; ok && q < slots; ++q) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, 93));
+          if (!ok) break;
+          if (elect_one()) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) notes[stage].off[i] = off[i];
             notes[stage].more = q + 1 < slots || next >= 0;
             mbar_expect_tx(&full_bar[stage], BN * BK * 2);
             tma_load_3d(smem + stage * STAGE_BYTES + A_BYTES, &g.tm_lb, &full_bar[stage], q * 64, col0, cur);
-            if (++stage == g.stages) { stage = 0; phase ^= 1; }
           }
+          if (++stage == g.stages) { stage = 0; phase ^= 1; }
         }
         if (first) t_phase ^= 1;
         first = false;
@@ -1017,7 +1012,6 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
 #pragma unroll
         for (int i = 0; i < 4; ++i) off[i] = next_off[i];
       }
-      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
     }
     __syncwarp();
   } else if (warp == 1) {

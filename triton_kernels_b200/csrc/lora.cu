@@ -81,19 +81,21 @@ __global__ void __launch_bounds__(THREADS, 1) lora_shrink_kernel(const __grid_co
   pdl_release();  // behind the TMEM allocation: the projection's blocks take all of an SM's TMEM
 
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      const uint32_t bytes = (uint32_t)(p.box_rows + p.rpad) * BK * 2;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, 82)) break;
-        uint8_t* dst = smem + stage * stage_bytes;
+    // (the whole warp walks the ring and an elected lane issues: with one lane on its own in the loop the copies' operands
+    // are not known to be uniform, and issuing a slot took 440 cycles)
+    int stage = 0;
+    uint32_t phase = 0;
+    const uint32_t bytes = (uint32_t)(p.box_rows + p.rpad) * BK * 2;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, 82))) break;
+      uint8_t* dst = smem + stage * stage_bytes;
+      if (elect_one()) {
         mbar_expect_tx(&full_bar[stage], bytes);
         // rows behind the request are loaded and never stored; rows of the tile that no box covers are never read out
         tma_load_2d(dst, &p.tm_x, &full_bar[stage], kb * BK, row0);
         tma_load_3d(dst + BM * BK * 2, &p.tm_a, &full_bar[stage], kb * BK, 0, adapter);
-        if (++stage == p.stages) { stage = 0; phase ^= 1; }
       }
+      if (++stage == p.stages) { stage = 0; phase ^= 1; }
     }
     __syncwarp();
   } else if (warp == 1) {
