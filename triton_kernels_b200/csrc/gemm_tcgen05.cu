@@ -906,13 +906,15 @@ struct Tiles {
   RequestAdapters req;
   LowRank low;
   int stages;
+  int subs;    // 64-wide K steps per ring slot
   int a_rows;  // rows of x per box: fewer than 128 when there are fewer; the MMAs then read what lies behind them in
                // shared memory as the other rows, whose results are never stored
 };
 
 template <int BN>
 __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_constant__ Tiles g) {
-  const int A_BYTES = g.a_rows * BK * 2, STAGE_BYTES = A_BYTES + BN * BK * 2;
+  constexpr int B_BYTES = BN * BK * 2;
+  const int A_BYTES = g.a_rows * BK * 2, SLOT_A = g.subs * A_BYTES, STAGE_BYTES = SLOT_A + g.subs * B_BYTES;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], acc_full[2], acc_empty[2], t_full, t_empty;
   __shared__ SlotNote<4> notes[MAX_STAGES];
@@ -964,8 +966,10 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
       rows.fetch(g.req, row0, p.M, lane);
       uint32_t off[4], next_off[4];
       int cur = -1;
-      for (int kb = 0; kb < num_kb; ++kb) {
-        if (kb == num_kb - 1) {
+      for (int kb = 0; kb < num_kb; kb += g.subs) {
+        const int subs = min(g.subs, num_kb - kb);
+        const bool last = kb + g.subs >= num_kb;
+        if (last) {
           rows.begin();
           cur = rows.next(off);
         }
@@ -973,10 +977,12 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
         if (ok) {
           uint8_t* dst = smem + stage * STAGE_BYTES;
           if (elect_one()) {
-            if (kb == num_kb - 1) notes[stage].more = cur >= 0;
-            mbar_expect_tx(&full_bar[stage], STAGE_BYTES);
-            tma_load_2d(dst, &g.tm_a, &full_bar[stage], kb * BK, row0);
-            tma_load_2d(dst + A_BYTES, &g.tm_b, &full_bar[stage], kb * BK, col0);
+            if (last) notes[stage].more = cur >= 0;
+            mbar_expect_tx(&full_bar[stage], subs * (A_BYTES + B_BYTES));
+            for (int i = 0; i < subs; ++i) {
+              tma_load_2d(dst + i * A_BYTES, &g.tm_a, &full_bar[stage], (kb + i) * BK, row0);
+              tma_load_2d(dst + SLOT_A + i * B_BYTES, &g.tm_b, &full_bar[stage], (kb + i) * BK, col0);
+            }
           }
           if (++stage == g.stages) { stage = 0; phase ^= 1; }
         }
@@ -1001,8 +1007,8 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
 #pragma unroll
             for (int i = 0; i < 4; ++i) notes[stage].off[i] = off[i];
             notes[stage].more = q + 1 < slots || next >= 0;
-            mbar_expect_tx(&full_bar[stage], BN * BK * 2);
-            tma_load_3d(smem + stage * STAGE_BYTES + A_BYTES, &g.tm_lb, &full_bar[stage], q * 64, col0, cur);
+            mbar_expect_tx(&full_bar[stage], B_BYTES);
+            tma_load_3d(smem + stage * STAGE_BYTES + SLOT_A, &g.tm_lb, &full_bar[stage], q * 64, col0, cur);
           }
           if (++stage == g.stages) { stage = 0; phase ^= 1; }
         }
@@ -1028,16 +1034,20 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
       tc_fence_after_sync();
       const uint32_t d_tmem = tmem_base + acc * BN;
       uint32_t more = 0;
-      for (int kb = 0; kb < num_kb; ++kb) {
+      for (int kb = 0; kb < num_kb; kb += g.subs) {
         ok = __all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, abort_flag, p.status, 95));
         if (!ok) break;
         tc_fence_after_sync();
-        if (kb == num_kb - 1) more = notes[stage].more;  // before the slot is given back
+        if (kb + g.subs >= num_kb) more = notes[stage].more;  // before the slot is given back
+        const int subs = min(g.subs, num_kb - kb);
         const uint32_t a_addr = smem_u32(smem + stage * STAGE_BYTES);
-        const uint64_t adesc = make_smem_desc(a_addr, 16, 1024), bdesc = make_smem_desc(a_addr + A_BYTES, 16, 1024);
+        const uint64_t adesc = make_smem_desc(a_addr, 16, 1024), bdesc = make_smem_desc(a_addr + SLOT_A, 16, 1024);
         if (elect_one()) {
+          for (int i = 0; i < subs; ++i) {
+            const uint64_t ad = adesc + i * (A_BYTES >> 4), bd = bdesc + i * (B_BYTES >> 4);
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k) umma_ss(d_tmem, adesc + 2 * k, bdesc + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
+            for (int k = 0; k < BK / 16; ++k) umma_ss(d_tmem, ad + 2 * k, bd + 2 * k, idesc, (kb | i | k) != 0 ? 1u : 0u);
+          }
           umma_commit(&empty_bar[stage]);
         }
         if (++stage == g.stages) { stage = 0; phase ^= 1; }
@@ -1055,7 +1065,7 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
         more = note.more;
         // (more than 64 ranks: groups of 64, one per slot; up to 64 there is one group and one slot)
         const uint64_t adesc = g.low.desc(smem_u32(t_smem + q * g.low.tile_bytes()));
-        const uint64_t bdesc = make_smem_desc(smem_u32(smem + stage * STAGE_BYTES) + A_BYTES, 16, 1024);
+        const uint64_t bdesc = make_smem_desc(smem_u32(smem + stage * STAGE_BYTES) + SLOT_A, 16, 1024);
         const int n_units = min(4, g.low.units - q * 4);
         if (elect_one()) {
           for (int i = 0; i < n_units; ++i) {
@@ -1123,9 +1133,14 @@ static int launch_tiles(Tiles& g, const fluxb_linear_problem& a, int64_t N, int6
     int rc = encode_tmap_bf16(&g.tm_lb, lora_b, 3, dims, strides, box);
     if (rc != FLUXB_OK) return rc;
   }
-  const int stage_bytes = g.a_rows * BK * 2 + BN * BK * 2, behind = (BM - g.a_rows) * BK * 2;
-  const int t_bytes = g.low.groups * g.low.group * 512;
-  g.stages = (MAX_SMEM - 1024 - 512 - t_bytes - behind) / stage_bytes;
+  const int step_bytes = g.a_rows * BK * 2 + BN * BK * 2, behind = (BM - g.a_rows) * BK * 2;
+  const int t_bytes = g.low.groups * g.low.group * 512, room = MAX_SMEM - 1024 - 1024 - t_bytes - behind;
+  // Several K steps per slot, as long as three slots fit: a slot costs the producer and the MMA warp some 500 cycles
+  // each (wait, vote, election, issue), which a step of a narrow tile does not cover (16 x 4096 -> 4096: 22.6 us with
+  // one step per slot).
+  g.subs = room / step_bytes >= 12 ? 4 : (room / step_bytes >= 6 ? 2 : 1);
+  const int stage_bytes = g.subs * step_bytes;
+  g.stages = room / stage_bytes;
   if (g.stages > MAX_STAGES) g.stages = MAX_STAGES;
   g.p.tiles_n = (int)((N + BN - 1) / BN);
   g.p.num_tiles = g.p.tiles_m * g.p.tiles_n;

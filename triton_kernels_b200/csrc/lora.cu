@@ -24,7 +24,7 @@ struct Params {
   __nv_bfloat16* t;    // [M, low.ld()]
   LowRank low;
   int L, tiles_per_request, box_rows;
-  int num_kb, ksplit, rpad, stages, tmem_cols;
+  int num_kb, ksplit, rpad, stages, subs, tmem_cols;  // subs: 64-wide K steps per ring slot
   DeviceStatus* status;
 };
 
@@ -56,7 +56,8 @@ __global__ void __launch_bounds__(THREADS, 1) lora_shrink_kernel(const __grid_co
     if (threadIdx.x == 0 && rank == 0 && l0 == 0 && p.req.raw(request) != -1) report_error(p.status, FLUXB_ERR_BAD_ARG, 81);
     return;
   }
-  const int stage_bytes = BM * BK * 2 + p.rpad * BK * 2;
+  constexpr int x_bytes = BM * BK * 2;
+  const int a_bytes = p.rpad * BK * 2, slot_x = p.subs * x_bytes, stage_bytes = slot_x + p.subs * a_bytes;
   const int kb0 = rank * p.num_kb / p.ksplit, kb1 = (rank + 1) * p.num_kb / p.ksplit;
 
   if (threadIdx.x == 0) {
@@ -86,14 +87,17 @@ __global__ void __launch_bounds__(THREADS, 1) lora_shrink_kernel(const __grid_co
     int stage = 0;
     uint32_t phase = 0;
     const uint32_t bytes = (uint32_t)(p.box_rows + p.rpad) * BK * 2;
-    for (int kb = kb0; kb < kb1; ++kb) {
+    for (int kb = kb0; kb < kb1; kb += p.subs) {
+      const int subs = min(p.subs, kb1 - kb);
       if (!__all_sync(0xffffffffu, mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, 82))) break;
       uint8_t* dst = smem + stage * stage_bytes;
       if (elect_one()) {
-        mbar_expect_tx(&full_bar[stage], bytes);
+        mbar_expect_tx(&full_bar[stage], subs * bytes);
         // rows behind the request are loaded and never stored; rows of the tile that no box covers are never read out
-        tma_load_2d(dst, &p.tm_x, &full_bar[stage], kb * BK, row0);
-        tma_load_3d(dst + BM * BK * 2, &p.tm_a, &full_bar[stage], kb * BK, 0, adapter);
+        for (int i = 0; i < subs; ++i) {
+          tma_load_2d(dst + i * x_bytes, &p.tm_x, &full_bar[stage], (kb + i) * BK, row0);
+          tma_load_3d(dst + slot_x + i * a_bytes, &p.tm_a, &full_bar[stage], (kb + i) * BK, 0, adapter);
+        }
       }
       if (++stage == p.stages) { stage = 0; phase ^= 1; }
     }
@@ -103,17 +107,21 @@ __global__ void __launch_bounds__(THREADS, 1) lora_shrink_kernel(const __grid_co
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int kb = kb0; kb < kb1; ++kb) {
+    for (int kb = kb0; kb < kb1; kb += p.subs) {
+      const int subs = min(p.subs, kb1 - kb);
       ok = __all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, abort_flag, p.status, 83));
       if (!ok) break;
       tc_fence_after_sync();
       const uint32_t a_addr = smem_u32(smem + stage * stage_bytes);
       const uint64_t adesc = make_smem_desc(a_addr, 16, 1024);
-      const uint64_t bdesc = make_smem_desc(a_addr + BM * BK * 2, 16, 1024);
+      const uint64_t bdesc = make_smem_desc(a_addr + slot_x, 16, 1024);
       if (elect_one()) {
+        for (int i = 0; i < subs; ++i) {
+          const uint64_t ad = adesc + i * (x_bytes >> 4), bd = bdesc + i * (a_bytes >> 4);
 #pragma unroll
-        for (int k = 0; k < BK / 16; ++k)
-          umma_ss(tmem_base, adesc + 2 * k, bdesc + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+          for (int k = 0; k < BK / 16; ++k)
+            umma_ss(tmem_base, ad + 2 * k, bd + 2 * k, idesc, (kb > kb0 || i > 0 || k > 0) ? 1u : 0u);
+        }
         umma_commit(&empty_bar[stage]);
       }
       if (++stage == p.stages) { stage = 0; phase ^= 1; }
@@ -209,8 +217,11 @@ static int launch_shrink(const void* x, int64_t ldx, const void* lora_a, const f
   // not all find a place at once from 16 on (2048 rows, K 3072: 16.7 us with eight, 9.9 with four, 12.0 with two).
   p.ksplit = 1;
   while (p.ksplit < (tiles < 12 ? 8 : 4) && tiles * p.ksplit * 2 <= sm_count() && p.num_kb >= p.ksplit * 2 * 4) p.ksplit *= 2;
-  const int steps = (p.num_kb + p.ksplit - 1) / p.ksplit;
-  const int stage_bytes = BM * BK * 2 + p.rpad * BK * 2;
+  const int step_bytes = BM * BK * 2 + p.rpad * BK * 2;
+  // two K steps per slot where three slots fit: a slot costs its warps some 500 cycles each
+  p.subs = MAX_SMEM / step_bytes >= 6 ? 2 : 1;
+  const int stage_bytes = p.subs * step_bytes;
+  const int steps = ((p.num_kb + p.ksplit - 1) / p.ksplit + p.subs - 1) / p.subs;
   p.stages = MAX_SMEM / stage_bytes < MAX_STAGES ? MAX_SMEM / stage_bytes : MAX_STAGES;
   if (p.stages > steps) p.stages = steps;
   int smem = p.stages * stage_bytes;
