@@ -406,6 +406,27 @@ struct TileAdapters {
     return cur;
   }
 };
+// 32 accumulator columns of one row through bias and activation, packed to four 16-byte pieces.  The bias comes from
+// shared memory, staged once per tile while the tile is still being multiplied: asked for eight columns at a time in the
+// epilogue itself, each of those loads is waited for (8370 x 176 -> 5496, all epilogue: 75 us instead of 50).
+__device__ __forceinline__ void finish32(const uint32_t (&acc)[32], const float* bias, int epi, uint4 (&out)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float4 b0 = *reinterpret_cast<const float4*>(bias + j * 8), b1 = *reinterpret_cast<const float4*>(bias + j * 8 + 4);
+    float v[8] = {__uint_as_float(acc[j * 8]) + b0.x,     __uint_as_float(acc[j * 8 + 1]) + b0.y,
+                  __uint_as_float(acc[j * 8 + 2]) + b0.z, __uint_as_float(acc[j * 8 + 3]) + b0.w,
+                  __uint_as_float(acc[j * 8 + 4]) + b1.x, __uint_as_float(acc[j * 8 + 5]) + b1.y,
+                  __uint_as_float(acc[j * 8 + 6]) + b1.z, __uint_as_float(acc[j * 8 + 7]) + b1.w};
+    if (epi == FLUXB_EPI_GELU) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = gelu_tanh(v[e]);
+    }
+    out[j] = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+  }
+}
+__device__ __forceinline__ float bias_at(const Params& p, int col) {
+  return p.bias != nullptr && col < p.N ? __bfloat162float(p.bias[col]) : 0.f;
+}
 // What the producer leaves beside a ring slot for the MMA warp: of an adapter's slot the mask of the rows that it leaves
 // alone, and of the last slot of a K loop and of every adapter's whether another adapter's slot follows.  The MMA warp
 // reads it behind its wait for the slot (the producer's arrival there releases it) and so has nothing to find out.
@@ -595,7 +616,8 @@ gemm_pair_kernel(const __grid_constant__ G g) {
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  __shared__ SlotNote<8> notes[kMode == 3 ? STAGES : 1];  // (kMode 3 alone uses it)
+  __shared__ SlotNote<8> notes[kMode == 3 ? STAGES : 1];  // (kMode 3 alone uses these two)
+  __shared__ __align__(16) float bias_s[2][kMode == 3 ? BN : 4];
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -819,6 +841,11 @@ gemm_pair_kernel(const __grid_constant__ G g) {
       const int row = row0 + r_local;
       const int n0 = n_blk * BN;
       const bool second = n0 >= p.split;
+      if constexpr (kMode == 3) {
+        // (a tile's bias is overwritten two tiles later, behind the barrier of the tile between)
+        bias_s[acc][threadIdx.x - 64] = bias_at(p, n0 + (int)threadIdx.x - 64);
+        asm volatile("bar.sync 3, 256;" ::: "memory");
+      }
       if (!mbar_wait_cluster(&acc_full[acc], acc_phase, abort_flag, status, 45)) { ok = false; break; }
       tc_fence_after_sync();
       const CUtensorMap* tm_out = second ? &pr.tm_y2 : &pr.tm_y;
@@ -852,8 +879,19 @@ gemm_pair_kernel(const __grid_constant__ G g) {
           // this group's previous store must have read the staging tile out
           if (store_issuer) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
           asm volatile("bar.sync %0, 128;" ::"r"(bar_id) : "memory");
-          epilogue_chunk(p, r0, row, n0 + c * OUT_CHUNK_COLS, second, line, 0, r_local & 7);
-          epilogue_chunk(p, r1, row, n0 + c * OUT_CHUNK_COLS + 32, second, line, 4, r_local & 7);
+          if constexpr (kMode == 3) {
+            uint4 o0[4], o1[4];
+            finish32(r0, &bias_s[acc][c * OUT_CHUNK_COLS], p.epi, o0);
+            finish32(r1, &bias_s[acc][c * OUT_CHUNK_COLS + 32], p.epi, o1);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              *reinterpret_cast<uint4*>(line + ((j ^ (r_local & 7)) << 4)) = o0[j];
+              *reinterpret_cast<uint4*>(line + (((4 + j) ^ (r_local & 7)) << 4)) = o1[j];
+            }
+          } else {
+            epilogue_chunk(p, r0, row, n0 + c * OUT_CHUNK_COLS, second, line, 0, r_local & 7);
+            epilogue_chunk(p, r1, row, n0 + c * OUT_CHUNK_COLS + 32, second, line, 4, r_local & 7);
+          }
           fence_proxy_async_smem();
           asm volatile("bar.sync %0, 128;" ::"r"(bar_id) : "memory");
           if (store_issuer) {
@@ -893,9 +931,10 @@ namespace gemm3 {
 using gemm::BK;
 using gemm::BM;
 using gemm::Params;
-using gemm::epilogue_chunk;
 using gemm2::SlotNote;
 using gemm2::TileAdapters;
+using gemm2::bias_at;
+using gemm2::finish32;
 constexpr int THREADS = 192;
 constexpr int MAX_STAGES = 16;
 constexpr int MAX_SMEM = 224 * 1024;
@@ -918,6 +957,7 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], acc_full[2], acc_empty[2], t_full, t_empty;
   __shared__ SlotNote<4> notes[MAX_STAGES];
+  __shared__ __align__(16) float bias_s[2][BN];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   uint8_t* t_smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -1089,10 +1129,13 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
     for (int tile = blockIdx.x; tile < p.num_tiles; tile += gridDim.x, ++local) {
       const int acc = local & 1;
       const uint32_t acc_phase = (local >> 1) & 1;
+      const int row0 = tile % p.tiles_m * BM, n0 = tile / p.tiles_m * BN;
+      // (a tile's bias is overwritten two tiles later, behind the barrier of the tile between)
+      if ((int)threadIdx.x - 64 < BN) bias_s[acc][threadIdx.x - 64] = bias_at(p, n0 + (int)threadIdx.x - 64);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
       if (!mbar_wait(&acc_full[acc], acc_phase, abort_flag, p.status, 98)) break;
       __syncwarp();
       tc_fence_after_sync();
-      const int row0 = tile % p.tiles_m * BM, n0 = tile / p.tiles_m * BN;
       const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * BN;
       if (row0 + quad * 32 < p.M) {
 #pragma unroll 1
@@ -1101,7 +1144,15 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
           uint32_t r[32];
           tmem_ld_x32(t_addr + c * 32, r);
           tmem_wait_ld();
-          epilogue_chunk(p, r, row0 + quad * 32 + lane, n0 + c * 32, false);
+          uint4 o[4];
+          finish32(r, &bias_s[acc][c * 32], p.epi, o);
+          const int row = row0 + quad * 32 + lane;
+          if (row < p.M) {
+            __nv_bfloat16* out = p.y + (int64_t)row * p.ldy + n0 + c * 32;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (n0 + c * 32 + j * 8 < p.N) *reinterpret_cast<uint4*>(out + j * 8) = o[j];
+          }
         }
       }
       tc_fence_before_sync();
@@ -1455,17 +1506,20 @@ static int encode_low_rank(CUtensorMap* out, const void* t_rows, int64_t M, cons
 // The projection of fluxb_linear_lora for more rows than the row-streaming kernel takes; t as lora.cu leaves it.
 int fluxb::launch_lora_gemm(const fluxb_linear_problem& a, int64_t N, int64_t K, int epi, const void* t_rows,
                             const void* lora_b, const LowRank& low, int64_t ldb, const RequestAdapters& req, cudaStream_t st) {
-  // Which tiles: cycles per 64-wide K step are 512 for a 256 x 256 tile of a CTA pair (its MMAs), and 64 bytes a cycle of
-  // operands for a 128 x BN tile of one CTA; on top of the K loop the last tile's epilogue shows, 20 000 cycles of the
-  // pair kernel's and about 40 per column of the other's.
+  // Which tiles, by an estimate in cycles fitted to both kernels over 20 problems (9 to 31131 rows, K 96 to 4696, N 72 to
+  // 5496; it is within a fifth of each time and picks the faster kernel or one within 5 %).  A 256 x 256 tile of a CTA
+  // pair takes 700 per 64-wide K step, and at least the 7500 of its epilogue; a 128 x BN tile of one CTA takes two per
+  // operand row and step, and at least its own epilogue.  For example 1024 x 2048 -> 2048: pairs 19.2 us, BN 128 15.5,
+  // 64 21.6, 32 34.4; 128 x 1024 -> 4096: 13.8, 10.4, 9.7, 9.2; 4096 x 4096 -> 4096: 97.5, 129, 209, 385.
   const int64_t kb = (K + 63) / 64, sms = sm_count();
-  const int64_t pair_tiles = ((a.M + 255) / 256) * ((N + 255) / 256);
-  int64_t best = (pair_tiles + sms / 2 - 1) / (sms / 2) * 512 * kb + 20000;
   const int64_t a_rows = a.M < 128 ? (a.M + 7) / 8 * 8 : 128;
+  const int64_t pair_tiles = ((a.M + 255) / 256) * ((N + 255) / 256);
+  int64_t best = (pair_tiles + sms / 2 - 1) / (sms / 2) * (700 * kb > 7500 ? 700 * kb : 7500) + 13000;
   int bn = 256;
   for (int c = 128; c >= 32; c /= 2) {
     const int64_t tiles = ((a.M + 127) / 128) * ((N + c - 1) / c);
-    const int64_t t = (tiles + sms - 1) / sms * ((a_rows + c) * 2 * kb + 40 * c);
+    const int64_t steps = ((a_rows + c) * 2 + 100) * kb, epilogue = 1100 + 30 * c;
+    const int64_t t = (tiles + sms - 1) / sms * ((steps > epilogue ? steps : epilogue) + 1000) + 7000;
     if (t < best) { best = t; bn = c; }
   }
   if (bn < 256) {
