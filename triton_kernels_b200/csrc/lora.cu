@@ -363,19 +363,21 @@ static int launch_shrink_short(const void* x, int64_t ldx, const void* lora_a, c
 
 // ----------------------------------------------------------------------------------------
 // One to eight rows: the projection is a stream of W.  A block takes 16 output columns at a time; the 16 rows of W
-// come through a ring in shared memory by bulk copies (2 KB of a row each, 200 KB in flight per SM: the block keeps
+// come through a ring in shared memory by bulk copies (a row of up to 6 KB each, 200 KB in flight per SM: the block keeps
 // asking while it computes), and its eight warps share a piece's columns.  The products run as mma.m16n8k16 with W's
 // rows on the M side and the rows of x on the N side; a lane reads 16 consecutive bytes of two W rows and uses them as
 // its A fragments of two MMAs, with x's fragment taken from the same k positions: the order of k does not matter as
 // long as both sides agree.  x's fragments stay in registers for all tiles (kPieces pieces of W; 0: read each time).
 // The adapters are R more products per output, from t's two parts widened to fp32.
-// (With W loaded straight to registers, 98 KB in flight per SM: 27 us for 18432 x 3072 instead.)
+// 18432 x 3072, eight rows: 23.9 us with the low-rank rows.  (With W loaded straight to registers, 98 KB in flight per SM: 27 us; with 2 KB
+// copies: 25 us.)
 // ----------------------------------------------------------------------------------------
 namespace rows {
 constexpr int WARPS = 8;
 constexpr int THREADS = WARPS * 32 + 32 + 128;  // and a warp that issues the copies, and four that finish the outputs
-constexpr int AHEAD = 4;                  // eights of ranks whose loads leave ahead of a tile's sums
-constexpr int PIECE = 1024;               // most columns of W per ring slot
+constexpr int AHEAD = 8;                  // eights of ranks that are asked for a tile ahead
+constexpr int WHOLE = 3072;               // rows of up to so many columns are one piece ...
+constexpr int PIECE = 1536;               // ... longer ones are cut into pieces of so many
 constexpr int MAX_SLOTS = 12;
 constexpr int RING_BYTES = 200 * 1024;
 
@@ -403,7 +405,8 @@ __device__ __forceinline__ float dot8(const uint4& b, const float* t, float acc)
   return acc;
 }
 
-template <int kPieces>
+// kPieces: pieces per row whose fragments of x are kept (0: read each time); kSteps: most 32-column steps of a warp per piece.
+template <int kPieces, int kSteps>
 __global__ void __launch_bounds__(THREADS, 1) lora_rows_kernel(const Params p) {
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ uint64_t full_bar[MAX_SLOTS], empty_bar[MAX_SLOTS], red_full[2], red_empty[2];
@@ -455,7 +458,7 @@ __global__ void __launch_bounds__(THREADS, 1) lora_rows_kernel(const Params p) {
   }
   if (warp > WARPS) {
     // One thread per output of a tile: sums the eight warps' shares and adds bias and adapter.  Warps of their own,
-    // which ask for their rows of B before they wait, because a tile's finish is all latency: done by the streaming
+    // which ask for their rows of B a tile ahead, because a tile's finish is all latency: done by the streaming
     // warps it cost a third of the time (29.8 us).
     const int e = threadIdx.x - (WARPS + 1) * 32;
     const int m = e >> 4, nl = e & 15;
@@ -463,15 +466,22 @@ __global__ void __launch_bounds__(THREADS, 1) lora_rows_kernel(const Params p) {
     const int ahead = min(p.low.R / 8, AHEAD);
     int parity = 0;
     uint32_t red_phase = 0;
+    uint4 bv[AHEAD];
+    float bias = 0.f;
+    auto row_of_b = [&](int n) { return p.lora_b + ((int64_t)adapter * p.N + n) * p.ldb; };
+    auto ask = [&](int tile) {
+      const int n = tile * 16 + nl;
+      if (m >= p.M || n >= p.N) return;
+      if (p.bias != nullptr) bias = __bfloat162float(p.bias[n]);
+      if (adapter < 0) return;
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        if (i < ahead) bv[i] = __ldg(reinterpret_cast<const uint4*>(row_of_b(n) + i * 8));
+    };
+    ask(blockIdx.x);
     for (int tile = blockIdx.x; tile < p.tiles; tile += gridDim.x) {
       const int n = tile * 16 + nl;
       const bool mine = m < p.M && n < p.N;
-      const __nv_bfloat16* b = p.lora_b + ((int64_t)adapter * p.N + n) * p.ldb;
-      uint4 bv[AHEAD];
-#pragma unroll
-      for (int i = 0; i < AHEAD; ++i)
-        if (mine && adapter >= 0 && i < ahead) bv[i] = __ldg(reinterpret_cast<const uint4*>(b + i * 8));
-      float v = mine && p.bias != nullptr ? __bfloat162float(p.bias[n]) : 0.f;
       if (tile == (int)blockIdx.x) {  // t of the requests that have an adapter, widened
         pdl_wait();
         for (int i = e; i < p.M * p.low.R; i += 128) {
@@ -485,8 +495,9 @@ __global__ void __launch_bounds__(THREADS, 1) lora_rows_kernel(const Params p) {
         }
         asm volatile("bar.sync 1, 128;" ::: "memory");
       }
-      float s = 0.f;
+      float v = bias, s = 0.f;
       if (mine && adapter >= 0) {
+        const __nv_bfloat16* b = row_of_b(n);
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i)
           if (i < ahead) s = dot8(bv[i], &t_s[m][i * 8], s);
@@ -495,6 +506,7 @@ __global__ void __launch_bounds__(THREADS, 1) lora_rows_kernel(const Params p) {
         for (; j + 8 <= p.low.R; j += 8) s = dot8(__ldg(reinterpret_cast<const uint4*>(b + j)), &t_s[m][j], s);
         for (; j < p.low.R; ++j) s = fmaf(__bfloat162float(b[j]), t_s[m][j], s);
       }
+      if (tile + (int)gridDim.x < p.tiles) ask(tile + gridDim.x);
       __syncwarp();
       if (!__all_sync(0xffffffffu, mbar_wait(&red_full[parity], red_phase, abort_flag, p.status, 88))) return;
 #pragma unroll
@@ -509,30 +521,30 @@ __global__ void __launch_bounds__(THREADS, 1) lora_rows_kernel(const Params p) {
     return;
   }
   const int g = lane >> 2, t4 = lane & 3;
-  const int steps = p.piece / (WARPS * 32);  // of 32 columns per warp and piece, at most four
+  const int steps = p.piece / (WARPS * 32);  // of 32 columns per warp and piece
   const int col = warp * (p.piece / WARPS) + t4 * 8;
   const __nv_bfloat16* xr = p.x + g * p.ldx;
   auto load_x = [&](int piece, int s) {
     const int k = piece * p.piece + col + s * 32;
     return g < p.M && s < steps && k < p.K ? __ldg(reinterpret_cast<const uint4*>(xr + k)) : make_uint4(0, 0, 0, 0);
   };
-  uint4 bx[kPieces > 0 ? kPieces : 1][4];
+  uint4 bx[kPieces > 0 ? kPieces : 1][kSteps];
   if (kPieces > 0) {
 #pragma unroll
     for (int q = 0; q < kPieces; ++q)
 #pragma unroll
-      for (int s = 0; s < 4; ++s) bx[q][s] = load_x(q, s);
+      for (int s = 0; s < kSteps; ++s) bx[q][s] = load_x(q, s);
   }
   int parity = 0;
   uint32_t red_phase = 0;
   for (int tile = blockIdx.x; tile < p.tiles; tile += gridDim.x) {
     float c[4] = {};
-    auto work = [&](int piece, const uint4 (&b)[4]) -> bool {
+    auto work = [&](int piece, const uint4 (&b)[kSteps]) -> bool {
       if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[slot], phase, abort_flag, p.status, 86))) return false;
       const uint8_t* base = ring + slot * slot_bytes + g * pitch + col * 2;
       const bool whole = (piece + 1) * p.piece <= p.K;
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
+      for (int s = 0; s < kSteps; ++s) {
         if (s < steps) {
           uint4 a0 = *reinterpret_cast<const uint4*>(base + s * 64);
           uint4 a1 = *reinterpret_cast<const uint4*>(base + 8 * pitch + s * 64);
@@ -553,7 +565,7 @@ __global__ void __launch_bounds__(THREADS, 1) lora_rows_kernel(const Params p) {
     } else {
       for (int q = 0; ok && q < p.pieces; ++q) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) bx[0][s] = load_x(q, s);
+        for (int s = 0; s < kSteps; ++s) bx[0][s] = load_x(q, s);
         ok = work(q, bx[0]);
       }
     }
@@ -584,7 +596,7 @@ static int launch_rows(const fluxb_linear_problem& a, int64_t N, int64_t K, int 
   p.ldx = a.ldx; p.ldw = a.ldw; p.ldy = a.ldy; p.ldb = ldb;
   p.M = (int)a.M; p.N = (int)N; p.K = (int)K; p.epi = epi;
   p.tiles = (int)((N + 15) / 16);
-  p.piece = K < PIECE ? (int)((K + 255) / 256 * 256) : PIECE;
+  p.piece = K <= WHOLE ? (int)((K + 255) / 256 * 256) : PIECE;
   p.pieces = (int)((K + p.piece - 1) / p.piece);
   p.status = device_status_ptr();
   const int slot_bytes = 16 * (p.piece * 2 + 64);
@@ -594,11 +606,9 @@ static int launch_rows(const fluxb_linear_problem& a, int64_t N, int64_t K, int 
   p.slots = RING_BYTES / slot_bytes;
   if (p.slots > MAX_SLOTS) p.slots = MAX_SLOTS;
   if (p.slots > per * p.pieces) p.slots = per * p.pieces;
-  auto kern = p.pieces == 1   ? lora_rows_kernel<1>
-              : p.pieces == 2 ? lora_rows_kernel<2>
-              : p.pieces == 3 ? lora_rows_kernel<3>
-              : p.pieces == 4 ? lora_rows_kernel<4>
-                              : lora_rows_kernel<0>;  // (the fragments of more pieces spill)
+  auto kern = p.pieces == 1   ? (p.piece <= 1024 ? lora_rows_kernel<1, 4> : lora_rows_kernel<1, 12>)
+              : p.pieces == 3 ? lora_rows_kernel<3, 6>
+                              : lora_rows_kernel<0, 6>;  // (the fragments of more pieces spill)
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES);
   if (e != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "linear_lora: cannot set shared memory size: %s", cudaGetErrorString(e));
   e = launch_after(kern, grid, THREADS, (size_t)p.slots * slot_bytes, st, p);
