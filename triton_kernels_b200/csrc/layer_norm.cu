@@ -56,7 +56,7 @@ struct LnBwdArgs {
 constexpr int kMaxTeamSlots = 64;
 
 
-// ---- any width, any alignment: one block per row, elements one at a time -----------------------------------
+// ---- any width, any alignment: one block per row, elements one at a time (more than 8192 columns, or 12288 aligned)
 template <typename T>
 __global__ void __launch_bounds__(256) ln_fwd_any_kernel(const LnArgs a) {
   __shared__ float slot[8];
@@ -134,6 +134,168 @@ __global__ void __launch_bounds__(256) ln_bwd_cols_any_kernel(const LnBwdArgs a)
     for (int i = 0; i < 8; ++i) s += acc[which][i][threadIdx.x & 31];
     if (cc < a.cols) a.partial[(part * 2 + which) * a.cols + cc] = s;
   }
+}
+
+// ---- any alignment, up to 8192 columns: one block per row, kE elements per thread in registers, 512 apart (so a warp's
+// loads are neighbours whatever the row starts at) -------------------------------------------------------------
+constexpr int kWide = 512;  // threads
+
+template <typename T, int kE>
+__global__ void __launch_bounds__(kWide) ln_fwd_elements_kernel(const LnArgs a) {
+  __shared__ float slot[2][16];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t row = blockIdx.x;
+  const T* x = static_cast<const T*>(a.x) + row * a.x_ld;
+  float v[kE];
+#pragma unroll
+  for (int i = 0; i < kE; ++i) v[i] = tid + i * kWide < a.cols ? to_f(x[tid + i * kWide]) : 0.f;
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < kE; ++i) s += v[i];
+  s = warp_sum(s);
+  if (lane == 0) slot[0][warp] = s;
+  __syncthreads();
+  float mean = 0.f;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) mean += slot[0][w];
+  mean /= a.cols;
+  float q = 0.f;
+#pragma unroll
+  for (int i = 0; i < kE; ++i) {
+    const float d = tid + i * kWide < a.cols ? v[i] - mean : 0.f;
+    q = fmaf(d, d, q);
+  }
+  q = warp_sum(q);
+  if (lane == 0) slot[1][warp] = q;
+  __syncthreads();
+  q = 0.f;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) q += slot[1][w];
+  const float rstd = rsqrtf(q / a.cols + a.eps);
+  if (a.mean != nullptr && tid == 0) { a.mean[row] = mean; a.rstd[row] = rstd; }
+  const int64_t vec = row / a.rows_per_group * a.vec_stride;
+  const T* f = a.factor != nullptr ? static_cast<const T*>(a.factor) + vec : nullptr;
+  const T* o = a.offset != nullptr ? static_cast<const T*>(a.offset) + vec : nullptr;
+  T* y = static_cast<T*>(a.y) + row * a.y_ld;
+#pragma unroll
+  for (int i = 0; i < kE; ++i) {
+    const int c = tid + i * kWide;
+    if (c < a.cols) {
+      const float h = __fmul_rn(v[i] - mean, rstd);
+      y[c] = static_cast<T>(fmaf(h, f != nullptr ? a.unit + to_f(f[c]) : 1.f, o != nullptr ? to_f(o[c]) : 0.f));
+    }
+  }
+}
+
+// Up to 1024 columns: a warp per row, kE elements per lane.
+template <typename T, int kE>
+__global__ void __launch_bounds__(256) ln_fwd_narrow_kernel(const LnArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= a.rows) return;
+  const T* x = static_cast<const T*>(a.x) + row * a.x_ld;
+  float v[kE], s = 0.f, q = 0.f;
+#pragma unroll
+  for (int i = 0; i < kE; ++i) v[i] = lane + i * 32 < a.cols ? to_f(x[lane + i * 32]) : 0.f;
+#pragma unroll
+  for (int i = 0; i < kE; ++i) s += v[i];
+  const float mean = warp_sum(s) / a.cols;
+#pragma unroll
+  for (int i = 0; i < kE; ++i) {
+    const float d = lane + i * 32 < a.cols ? v[i] - mean : 0.f;
+    q = fmaf(d, d, q);
+  }
+  const float rstd = rsqrtf(warp_sum(q) / a.cols + a.eps);
+  if (a.mean != nullptr && lane == 0) { a.mean[row] = mean; a.rstd[row] = rstd; }
+  const int64_t vec = row / a.rows_per_group * a.vec_stride;
+  const T* f = a.factor != nullptr ? static_cast<const T*>(a.factor) + vec : nullptr;
+  const T* o = a.offset != nullptr ? static_cast<const T*>(a.offset) + vec : nullptr;
+  T* y = static_cast<T*>(a.y) + row * a.y_ld;
+#pragma unroll
+  for (int i = 0; i < kE; ++i) {
+    const int c = lane + i * 32;
+    if (c < a.cols) {
+      const float h = __fmul_rn(v[i] - mean, rstd);
+      y[c] = static_cast<T>(fmaf(h, f != nullptr ? a.unit + to_f(f[c]) : 1.f, o != nullptr ? to_f(o[c]) : 0.f));
+    }
+  }
+}
+
+// One pass over x and dy: the block walks rows of its part of a group, with the next row's elements on their way.
+template <typename T, int kE>
+__global__ void __launch_bounds__(kWide, 1) ln_bwd_elements_kernel(const LnBwdArgs a) {
+  __shared__ float2 red[2][16];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t group = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+  const int64_t base = group * a.rows_per_group;
+  const T* f = a.factor != nullptr ? static_cast<const T*>(a.factor) + group * a.vec_stride : nullptr;
+  float factor[kE], df[kE], dof[kE];
+  T xn[kE], dn[kE];
+  float mean_n = 0.f, rstd_n = 0.f;
+  auto ask = [&](int64_t r) {
+    if (r >= a.rows_per_group) return;
+    const T* x = static_cast<const T*>(a.x) + (base + r) * a.x_ld + tid;
+    const T* dy = static_cast<const T*>(a.dy) + (base + r) * a.dy_ld + tid;
+    mean_n = __ldg(a.mean + base + r);
+    rstd_n = __ldg(a.rstd + base + r);
+#pragma unroll
+    for (int i = 0; i < kE; ++i)
+      if (tid + i * kWide < a.cols) {
+        xn[i] = x[i * kWide];
+        dn[i] = dy[i * kWide];
+      }
+  };
+#pragma unroll
+  for (int i = 0; i < kE; ++i) {
+    factor[i] = f == nullptr ? 1.f : (tid + i * kWide < a.cols ? a.unit + to_f(f[tid + i * kWide]) : 0.f);
+    df[i] = dof[i] = 0.f;
+    xn[i] = dn[i] = static_cast<T>(0.f);
+  }
+  ask(part);
+  const float inv_cols = 1.f / a.cols;
+  int buf = 0;
+  for (int64_t r = part; r < a.rows_per_group; r += a.parts) {
+    const float mean = mean_n, rstd = rstd_n;
+    float g[kE], h[kE], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < kE; ++i) {
+      const bool in = tid + i * kWide < a.cols;
+      const float d = in ? to_f(dn[i]) : 0.f;
+      h[i] = in ? (to_f(xn[i]) - mean) * rstd : 0.f;
+      g[i] = d * factor[i];
+      s1 += g[i];
+      s2 = fmaf(g[i], h[i], s2);
+      df[i] = fmaf(d, h[i], df[i]);
+      dof[i] += d;
+    }
+    ask(r + a.parts);
+    s1 = warp_sum(s1);
+    s2 = warp_sum(s2);
+    if (lane == 0) red[buf][warp] = make_float2(s1, s2);
+    __syncthreads();  // (the other buffer's readers are through before anyone writes it again)
+    s1 = s2 = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      s1 += red[buf][w].x;
+      s2 += red[buf][w].y;
+    }
+    buf ^= 1;
+    if (a.dx != nullptr) {
+      const float k1 = -s1 * inv_cols * rstd, k2 = -s2 * inv_cols * rstd;
+      T* dx = static_cast<T*>(a.dx) + (base + r) * a.dx_ld + tid;
+#pragma unroll
+      for (int i = 0; i < kE; ++i)
+        if (tid + i * kWide < a.cols) dx[i * kWide] = static_cast<T>(fmaf(h[i], k2, fmaf(g[i], rstd, k1)));
+    }
+  }
+  if (a.partial == nullptr) return;
+  float* out = a.partial + (int64_t)blockIdx.x * 2 * a.cols;
+#pragma unroll
+  for (int i = 0; i < kE; ++i)
+    if (tid + i * kWide < a.cols) {
+      out[tid + i * kWide] = df[i];
+      out[a.cols + tid + i * kWide] = dof[i];
+    }
 }
 
 // ---- aligned rows ------------------------------------------------------------------------------------------
@@ -554,7 +716,7 @@ ln_bwd_reduce_kernel(const float* __restrict__ partial, O* __restrict__ df, O* _
 
 // How the backward pass runs: which kernel, and how many blocks share the rows of one group (one partial row each).
 struct BwdPlan {
-  enum Kind { kAny, kWarp, kTeam } kind;
+  enum Kind { kAny, kElements, kWarp, kTeam } kind;
   int vecs;  // 16-byte pieces per thread
   int wpr, teams, slots, parts;
   size_t smem;
@@ -602,7 +764,15 @@ static BwdPlan bwd_plan(int64_t groups, int64_t rows_per_group, int64_t cols, in
       }
     }
   }
-  if (p.kind == BwdPlan::kAny) { blocks = 2 * sm_count(); rows_at_once = 8; }
+  if (p.kind == BwdPlan::kAny) {
+    blocks = 2 * sm_count();
+    rows_at_once = 8;
+    if (cols <= 16 * kWide) {
+      p.kind = BwdPlan::kElements;
+      blocks = (cols <= 4 * kWide ? 2 : 1) * sm_count();
+      rows_at_once = 1;
+    }
+  }
   const int64_t want = blocks / groups, most = (rows_per_group + rows_at_once - 1) / rows_at_once;
   p.parts = (int)(want < 1 ? 1 : (want < most ? want : most));
   return p;
@@ -635,6 +805,19 @@ static int ln_check(const char* what, int64_t rows, int64_t cols, int64_t rows_p
   if (rows > INT32_MAX || cols > (1 << 20)) return set_error(FLUXB_ERR_UNSUPPORTED, "%s: too many rows or columns", what);
   *groups = rows / rows_per_group;
   return FLUXB_OK;
+}
+
+template <typename T>
+static void launch_any(const LnArgs& a, cudaStream_t st) {
+  const int e = (a.cols + kWide - 1) / kWide;
+  const unsigned rows = (unsigned)a.rows, eights = (rows + 7) / 8;
+  if (a.cols <= 128) ln_fwd_narrow_kernel<T, 4><<<eights, 256, 0, st>>>(a);
+  else if (a.cols <= 512) ln_fwd_narrow_kernel<T, 16><<<eights, 256, 0, st>>>(a);
+  else if (a.cols <= 1024) ln_fwd_narrow_kernel<T, 32><<<eights, 256, 0, st>>>(a);
+  else if (e <= 4) ln_fwd_elements_kernel<T, 4><<<rows, kWide, 0, st>>>(a);
+  else if (e <= 8) ln_fwd_elements_kernel<T, 8><<<rows, kWide, 0, st>>>(a);
+  else if (e <= 16) ln_fwd_elements_kernel<T, 16><<<rows, kWide, 0, st>>>(a);
+  else ln_fwd_any_kernel<T><<<rows, 256, 0, st>>>(a);
 }
 
 extern "C" int fluxb_layer_norm(const void* x, const void* factor, const void* offset, void* y, float* mean, float* rstd,
@@ -670,8 +853,8 @@ extern "C" int fluxb_layer_norm(const void* x, const void* factor, const void* o
     rc = launch_layer_norm_affine(x, factor, offset, y, mean, rstd, rows, cols, x_ld, y_ld, eps, dtype, st);
     return rc != FLUXB_OK ? rc : ln_status("layer_norm");
   }
-  if (dtype == FLUXB_BF16) ln_fwd_any_kernel<__nv_bfloat16><<<(unsigned)rows, 256, 0, st>>>(a);
-  else ln_fwd_any_kernel<float><<<(unsigned)rows, 256, 0, st>>>(a);
+  if (dtype == FLUXB_BF16) launch_any<__nv_bfloat16>(a, st);
+  else launch_any<float>(a, st);
   return ln_status("layer_norm");
 }
 
@@ -697,6 +880,16 @@ static int launch_bwd(const LnBwdArgs& a, const BwdPlan& p, bool sums, cudaStrea
   if (p.kind == BwdPlan::kAny) {
     if (a.dx != nullptr) ln_bwd_rows_any_kernel<T><<<(unsigned)a.rows, 256, 0, st>>>(a);
     if (sums) ln_bwd_cols_any_kernel<T><<<grid * (unsigned)((a.cols + 31) / 32), 256, 0, st>>>(a);
+    return FLUXB_OK;
+  }
+  if (p.kind == BwdPlan::kElements) {
+    const int e = (a.cols + kWide - 1) / kWide;
+    auto kern = e <= 1   ? ln_bwd_elements_kernel<T, 1>
+                : e <= 2 ? ln_bwd_elements_kernel<T, 2>
+                : e <= 4 ? ln_bwd_elements_kernel<T, 4>
+                : e <= 8 ? ln_bwd_elements_kernel<T, 8>
+                         : ln_bwd_elements_kernel<T, 16>;
+    kern<<<grid, kWide, 0, st>>>(a);
     return FLUXB_OK;
   }
   void (*kern)(LnBwdArgs) = nullptr;
