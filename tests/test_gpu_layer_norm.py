@@ -83,7 +83,7 @@ def grad_tols(x, f, h, rstd, dy, dh, rows_dim):
     return dx, df, do
 
 
-WIDTHS = [1, 2, 7, 8, 40, 63, 128, 384, 1000, 1001, 1024, 2048, 3072, 4096, 8192, 8200, 20000]
+WIDTHS = [1, 2, 7, 8, 40, 63, 128, 384, 515, 768, 1000, 1001, 1024, 2046, 2048, 3003, 3072, 4096, 6001, 8192, 8200, 12288, 20000]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -237,6 +237,13 @@ def test_no_rows(tk):
     y = tk.layer_norm_modulation(x3, sc, sc.detach())
     dx, ds = torch.autograd.grad(y, (x3, sc), torch.empty_like(y))
     assert y.shape == dx.shape == (2, 0, 64) and ds.shape == (2, 1, 64) and bool((ds == 0).all())
+
+
+def test_empty_last_dim_is_refused(tk):
+    for call in (lambda: tk.layer_norm(torch.empty(3, 0, device="cuda")),
+                 lambda: tk.layer_norm_modulation(*(torch.empty(2, n, 0, device="cuda") for n in (4, 1, 1)))):
+        with pytest.raises(AssertionError):
+            call()
 
 
 def test_scale_of_another_type_gets_a_gradient_of_its_own(tk):

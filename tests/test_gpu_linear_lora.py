@@ -213,6 +213,36 @@ def test_two_calls_at_once(tk):
     assert all(torch.equal(x, y) for x, y in outs)
 
 
+def test_first_call_of_a_process_inside_a_capture(lib):
+    """Nothing that a first call sets up needs to run outside a capture."""
+    code = """
+import torch, triton_kernels_b200 as tk
+torch.manual_seed(0)
+r = lambda *s: torch.randn(*s, device="cuda").bfloat16()
+sets = [(r(B, L, 256), r(512, 256), r(512), r(2, 16, 256), r(2, 512, 16), torch.arange(B, device="cuda") % 2) for B, L in ((2, 1), (3, 100), (2, 3000))]
+x, w = r(64, 1024).requires_grad_(), r(1024).requires_grad_()
+dy = r(64, 1024)
+torch.cuda.synchronize()
+def work():
+    y = tk.layer_norm(x, w, w)
+    return [tk.linear_lora(*s) for s in sets] + [y.detach(), *torch.autograd.grad(y, (x, w), dy)]
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = work()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, work()))
+print("same")
+"""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    root = Path(__file__).resolve().parent.parent
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
 def test_module(tk):
     torch.manual_seed(0)
     m = tk.LinearLoRA(256, 512, num_adapters=3, rank=8).to(BF).cuda()
@@ -239,6 +269,11 @@ def test_refusals_on_the_device(tk):
         tk.linear_lora(x, p["w"], p["b"], p["lora_a"], p["lora_b"], p["adapter"][:1])
     with pytest.raises(RuntimeError):
         tk.linear_lora(x, p["w"], p["b"], p["lora_a"], p["lora_b"], p["adapter"].cpu())
+    with pytest.raises(AssertionError):
+        e = lambda *s: torch.empty(*s, device="cuda", dtype=BF)  # noqa: E731
+        tk.linear_lora(e(2, 0), e(8, 0), None, e(1, 8, 0), e(1, 8, 8), p["adapter"])
+    with pytest.raises(NotImplementedError, match="rank"):
+        call(tk, problem(23, 2, 4, 64, 64, 264, 1))
     odd = problem(21, 2, 4, 64, 60, 8, 2)
     with pytest.raises(ValueError, match="multiples of 8"):
         call(tk, odd)

@@ -802,7 +802,8 @@ static int ln_check(const char* what, int64_t rows, int64_t cols, int64_t rows_p
   if (rows == 0) return FLUXB_OK;
   if (rows_per_group == 0 || rows % rows_per_group)
     return set_error(FLUXB_ERR_BAD_ARG, "%s: rows must be a multiple of rows_per_group", what);
-  if (rows > INT32_MAX || cols > (1 << 20)) return set_error(FLUXB_ERR_UNSUPPORTED, "%s: too many rows or columns", what);
+  // row numbers and their next steps stay in 32 bits
+  if (rows > (1 << 30) || cols > (1 << 20)) return set_error(FLUXB_ERR_UNSUPPORTED, "%s: too many rows or columns", what);
   *groups = rows / rows_per_group;
   return FLUXB_OK;
 }

@@ -232,7 +232,7 @@ extern "C" int fluxb_rope_axes(const void* q, int64_t q_sb, int64_t q_sh, int64_
   if (!ids || (Hq > 0 && (!q || !oq)) || (Hk > 0 && (!k || !ok)))
     return set_error(FLUXB_ERR_BAD_ARG, "rope_axes: null pointer");
   const int64_t half = (D + 1) / 2;
-  if (D > (1 << 16) || Hq > (1 << 20) || Hk > (1 << 20) || B * L > INT32_MAX || (B * L * half + 255) / 256 > INT32_MAX)
+  if (D > (1 << 16) || Hq > (1 << 20) || Hk > (1 << 20) || B > (1 << 30) || L > (1 << 30) || B * L > (1 << 30) || (B * L * half + 255) / 256 > INT32_MAX)
     return set_error(FLUXB_ERR_UNSUPPORTED, "rope_axes: too many tokens or heads");
   RopeAxesArgs a;
   a.t[0] = RopeTensor{q, oq, q_sb, q_sh, q_sl, oq_sb, oq_sh, oq_sl, (int)Hq};

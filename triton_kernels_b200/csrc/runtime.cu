@@ -31,9 +31,18 @@ DeviceStatus* device_status_ptr() {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return nullptr;
   std::lock_guard<std::mutex> lk(g_mu);
   if (g_status[dev] == nullptr) {
+    // The first call may come from inside a stream capture: there an allocation is allowed in relaxed mode only, and
+    // the clearing goes through a stream of its own, which nothing captures.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
     DeviceStatus* p = nullptr;
-    if (cudaMalloc(&p, sizeof(DeviceStatus)) != cudaSuccess) return nullptr;
-    if (cudaMemset(p, 0, sizeof(DeviceStatus)) != cudaSuccess) return nullptr;
+    cudaStream_t st = nullptr;
+    bool ok = cudaMalloc(&p, sizeof(DeviceStatus)) == cudaSuccess;
+    ok = ok && cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking) == cudaSuccess;
+    ok = ok && cudaMemsetAsync(p, 0, sizeof(DeviceStatus), st) == cudaSuccess && cudaStreamSynchronize(st) == cudaSuccess;
+    if (st != nullptr) cudaStreamDestroy(st);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (!ok) return nullptr;
     g_status[dev] = p;
   }
   return g_status[dev];

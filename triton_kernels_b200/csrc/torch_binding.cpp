@@ -154,7 +154,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight_in, const std::optional<Tensor>& bias_in, double eps) {
   require_cuda(x);
   dtype_code(x);
-  require(x.dim() > 0, "layer_norm runs over the last dim");
+  require(x.dim() > 0 && x.size(-1) > 0, "layer_norm runs over the last dim, which must not be empty");
   const int64_t C = x.size(-1);
   for (const std::optional<Tensor>* p : {&weight_in, &bias_in}) {
     if (!p->has_value()) continue;
@@ -229,6 +229,7 @@ Tensor layer_norm_modulation(const Tensor& x, const Tensor& weight, const Tensor
   require(x.dim() > 0 && weight.dim() > 0 && bias.dim() > 0 && x.size(0) == weight.size(0) && x.size(0) == bias.size(0),
           "x, weight and bias differ in the batch dim");
   require(x.size(-1) == weight.size(-1) && x.size(-1) == bias.size(-1), "x, weight and bias differ in the last dim");
+  require(x.size(-1) > 0, "the last dim must not be empty");
   require_cuda(x);
   same_device(x, weight);
   same_device(x, bias);
@@ -307,7 +308,7 @@ std::pair<Tensor, Tensor> apply_rope_axes(const Tensor& q, const Tensor& k, cons
 // ---- adapters ----------------------------------------------------------------------------------------------------
 Tensor linear_lora(const Tensor& x, const Tensor& w_in, const std::optional<Tensor>& b_in, const Tensor& lora_a, const Tensor& lora_b_in,
                    const Tensor& adapter, const std::optional<Tensor>& scale_in, bool gelu) {
-  require(x.dim() >= 2 && w_in.dim() == 2 && x.size(-1) == w_in.size(1), "Incompatible dimensions");
+  require(x.dim() >= 2 && w_in.dim() == 2 && x.size(-1) == w_in.size(1) && w_in.size(1) > 0, "Incompatible dimensions");
   const int64_t N = w_in.size(0), K = w_in.size(1), n = lora_a.dim() == 3 ? lora_a.size(0) : 0, R = n > 0 ? lora_a.size(1) : 0;
   require(n > 0 && R > 0 && lora_a.size(2) == K && lora_b_in.dim() == 3 && lora_b_in.size(0) == n && lora_b_in.size(1) == N &&
               lora_b_in.size(2) == R,
