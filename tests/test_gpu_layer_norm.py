@@ -309,3 +309,18 @@ def test_gradients_are_not_differentiable_again(tk):
     dx = torch.autograd.grad(tk.layer_norm(x).square().sum(), x, create_graph=True)[0]
     with pytest.raises(RuntimeError, match="once_differentiable"):
         dx.sum().backward()
+
+
+def test_a_single_row_of_any_stride(tk):
+    """The row stride of a single row says nothing (a view may have any)."""
+    base = make(71, (96,), torch.float32)
+    x = base.as_strided((1, 96), (1, 1))
+    assert x.is_contiguous()
+    w = make(72, (96,), torch.float32)
+    want = tk.layer_norm(base[None].clone(), w, w)
+    assert torch.equal(tk.layer_norm(x, w, w), want)
+    leaf = x.detach().requires_grad_(True)
+    ref = base[None].clone().requires_grad_(True)
+    (got,) = torch.autograd.grad(tk.layer_norm(leaf, w, w).square().sum(), leaf)
+    (exp,) = torch.autograd.grad(tk.layer_norm(ref, w, w).square().sum(), ref)
+    assert torch.equal(got, exp)

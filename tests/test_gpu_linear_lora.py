@@ -310,3 +310,18 @@ def test_norm_adapter_rotation_attention_as_they_are_used_together(tk):
     od = ((rot(qd) @ rot(kd).transpose(2, 3) * D**-0.5).softmax(-1) @ vd).transpose(1, 2).reshape(B, L, C)
     yd = definition(dict(out, x=od))[0]
     assert float((y.double() - yd).norm() / yd.norm()) < 6 * 2.0**-8
+
+
+@pytest.mark.parametrize("L", [1, 20, 200])
+def test_an_infinite_input_stays_infinite(tk, L):
+    """Rank 5: the ranks that fill up the tensor cores' sixteen must not turn infinity into NaN."""
+    p = problem(41, 3, L, 64, 48, 5, 2)
+    for key in ("w", "lora_a", "lora_b"):
+        p[key] = p[key].abs() + 2.0**-10  # all positive: no infinity meets one of the other sign
+    p["adapter"] = torch.tensor([1, -1, 0]).cuda()
+    clean = call(tk, p)
+    p["x"][0, 0, 3] = float("inf")
+    y = call(tk, p)
+    assert bool((y[0, 0] == float("inf")).all())
+    y[0, 0] = clean[0, 0]
+    assert torch.equal(y, clean)

@@ -212,3 +212,18 @@ def test_refusals_on_the_device(tk):
         tk.apply_rope_axes(q, q, ids[:, :3], (32, 32))
     with pytest.raises(AssertionError):
         tk.apply_rope_axes(q, q[:, :, :3], ids, (32, 32))
+
+
+def test_a_theta_below_one_turns_faster(tk):
+    """theta 2^-10, positions up to 2^24: 7.3e9 radians.  The angle itself is a product of three fp64 roundings on either
+    side (frequency, turn, product), 6 x 2^-53 of it, next to the kernel's 16 u."""
+    axes, theta = (16,), 2.0**-10
+    ids = (2**24 - 1 - torch.randint(0, 2**20, (1, 70, 1), generator=torch.Generator().manual_seed(5))).cuda()
+    q = make(6, (1, 2, 70, 16), torch.float32)
+    got, _ = tk.apply_rope_axes(q, q, ids, axes, theta)
+    want = rotation(q, ids, axes, theta)
+    pair = q.double().unflatten(-1, (8, 2)).norm(dim=-1).repeat_interleave(2, -1)
+    angle = float(ids.max()) * theta ** (-14 / 16)
+    limit = (16 * U + 6 * 2.0**-53 * angle) * pair
+    limit = limit + U * (want.abs() + limit)
+    assert bool(((got.double() - want).abs() <= limit).all())

@@ -82,8 +82,6 @@ __global__ void __launch_bounds__(THREADS, 1) lora_shrink_kernel(const __grid_co
   pdl_release();  // behind the TMEM allocation: the projection's blocks take all of an SM's TMEM
 
   if (warp == 0) {
-    // (the whole warp walks the ring and an elected lane issues: with one lane on its own in the loop the copies' operands
-    // are not known to be uniform, and issuing a slot took 440 cycles)
     int stage = 0;
     uint32_t phase = 0;
     const uint32_t bytes = (uint32_t)(p.box_rows + p.rpad) * BK * 2;
@@ -180,6 +178,9 @@ __global__ void __launch_bounds__(THREADS, 1) lora_shrink_kernel(const __grid_co
         v[4] += hi4[s].x; v[5] += hi4[s].y; v[6] += hi4[s].z; v[7] += hi4[s].w;
       }
     }
+    // the ranks behind R, which the projection multiplies, too: zeros would be NaN here beside an infinite x
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c8 + e < p.low.R ? v[e] : 0.f;
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -369,8 +370,8 @@ static int launch_shrink_short(const void* x, int64_t ldx, const void* lora_a, c
 // its A fragments of two MMAs, with x's fragment taken from the same k positions: the order of k does not matter as
 // long as both sides agree.  x's fragments stay in registers for all tiles (kPieces pieces of W; 0: read each time).
 // The adapters are R more products per output, from t's two parts widened to fp32.
-// 18432 x 3072, eight rows: 23.9 us with the low-rank rows.  (With W loaded straight to registers, 98 KB in flight per SM: 27 us; with 2 KB
-// copies: 25 us.)
+// Bound by HBM: 18432 x 3072, eight rows, 24.1 us with the low-rank rows (113 MB of W; 4.7 TB/s).  (With W loaded
+// straight to registers, 98 KB in flight per SM: 27 us; with 2 KB copies: 25 us.)
 // ----------------------------------------------------------------------------------------
 namespace rows {
 constexpr int WARPS = 8;

@@ -24,8 +24,8 @@ struct RequestAdapters {
 
 // Layout of the low-rank rows t: ranks in groups of 16, 32 or 64 (the smallest that holds R, else 64), each group as
 // its high parts, then its low parts: a group of 16 is a 64-byte line, of 32 a 128-byte line, of 64 two of them.  TMA
-// moves a line of up to 128 bytes per request, so wide lines matter: with 16-rank pieces throughout (64- and 32-byte
-// lines) the adapters cost the joint q|k|v projection at rank 128 20 % of its time.
+// moves a line of up to 128 bytes per request, and a ring slot costs its warps some 500 cycles whatever it holds, so
+// few wide lines are asked for rather than many narrow ones; small ranks do not pay for a full group.
 struct LowRank {
   int R, units, group, groups;  // units: sixteens of ranks in use
   explicit LowRank(int64_t rank = 16)

