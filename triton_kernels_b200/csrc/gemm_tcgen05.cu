@@ -311,6 +311,8 @@ constexpr int THREADS = 320;  // TMA warp, MMA warp, two groups of four epilogue
 constexpr int TMEM_COLS = 512;
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 2 * OUT_BUF_BYTES + 1024 + 256;
 constexpr int MAX_PROBLEMS = 4;
+constexpr int LORA_STAGES = 6;  // of kMode 3
+constexpr int lora_smem(int cols) { return LORA_STAGES * (A_BYTES + cols / 2 * BK * 2) + 2 * OUT_BUF_BYTES + 1024 + 256; }
 
 // Up to four GEMMs that differ in operands, outputs and row counts run as ONE persistent
 // launch: their tiles are concatenated (problem 0's tiles first) and dealt round-robin to the
@@ -409,14 +411,17 @@ struct TileAdapters {
 // 32 accumulator columns of one row through bias and activation, packed to four 16-byte pieces.  The bias comes from
 // shared memory, staged once per tile while the tile is still being multiplied: asked for eight columns at a time in the
 // epilogue itself, each of those loads is waited for (8370 x 176 -> 5496, all epilogue: 75 us instead of 50).
-__device__ __forceinline__ void finish32(const uint32_t (&acc)[32], const float* bias, int epi, uint4 (&out)[4]) {
+__device__ __forceinline__ void finish32(const uint32_t (&acc)[32], const __nv_bfloat16* bias, int epi, uint4 (&out)[4]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float4 b0 = *reinterpret_cast<const float4*>(bias + j * 8), b1 = *reinterpret_cast<const float4*>(bias + j * 8 + 4);
-    float v[8] = {__uint_as_float(acc[j * 8]) + b0.x,     __uint_as_float(acc[j * 8 + 1]) + b0.y,
-                  __uint_as_float(acc[j * 8 + 2]) + b0.z, __uint_as_float(acc[j * 8 + 3]) + b0.w,
-                  __uint_as_float(acc[j * 8 + 4]) + b1.x, __uint_as_float(acc[j * 8 + 5]) + b1.y,
-                  __uint_as_float(acc[j * 8 + 6]) + b1.z, __uint_as_float(acc[j * 8 + 7]) + b1.w};
+    const uint4 b = *reinterpret_cast<const uint4*>(bias + j * 8);
+    const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[2 * e] = __uint_as_float(acc[j * 8 + 2 * e]) + bf16_lo(w[e]);
+      v[2 * e + 1] = __uint_as_float(acc[j * 8 + 2 * e + 1]) + bf16_hi(w[e]);
+    }
     if (epi == FLUXB_EPI_GELU) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = gelu_tanh(v[e]);
@@ -424,8 +429,8 @@ __device__ __forceinline__ void finish32(const uint32_t (&acc)[32], const float*
     out[j] = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
   }
 }
-__device__ __forceinline__ float bias_at(const Params& p, int col) {
-  return p.bias != nullptr && col < p.N ? __bfloat162float(p.bias[col]) : 0.f;
+__device__ __forceinline__ __nv_bfloat16 bias_at(const Params& p, int col) {
+  return p.bias != nullptr && col < p.N ? p.bias[col] : __float2bfloat16_rn(0.f);
 }
 // What the producer leaves beside a ring slot for the MMA warp: of an adapter's slot the mask of the rows that it leaves
 // alone, and of the last slot of a K loop and of every adapter's whether another adapter's slot follows.  The MMA warp
@@ -436,7 +441,7 @@ struct SlotNote {
   uint32_t more;
 };
 // A ring slot of the adapters: a line of t and a group of B; a group of 64 takes two (high parts, low parts).
-__device__ __forceinline__ int lora_slots(const LowRank& low) { return low.group == 64 ? 2 * low.groups : low.groups; }
+__host__ __device__ __forceinline__ int lora_slots(const LowRank& low) { return low.group == 64 ? 2 * low.groups : low.groups; }
 
 // Epilogue of one 128-row x 256-column tile (two heads of q, of k or of v) for EPI_QKV_HEADS:
 // bias, rounding to bf16 (the projection's output precision in the reference), per-head RMS norm
@@ -602,22 +607,27 @@ __device__ __forceinline__ void qkv_tile_epilogue(const Params& p, const CUtenso
 //      same TMEM tile through the same ring, with a lane mask that leaves the other requests' rows
 //      alone (so a request never meets another one's adapter, not even as a product with zero).
 //      Cost: R / 32 ring slots per adapter of a tile, next to K / 64 of the projection.
-template <int kMode, typename G = Grouped>
+// kCols: output columns per tile.  Modes 0 to 2 have one width, 256; mode 3 takes a narrower one where that fills the
+// machine better.
+template <int kMode, typename G = Grouped, int kCols = BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 gemm_pair_kernel(const __grid_constant__ G g) {
+  constexpr int kStages = kMode == 3 ? LORA_STAGES : STAGES;
+  constexpr int kSlot = kMode == 3 ? A_BYTES + kCols / 2 * BK * 2 : STAGE_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  uint8_t* out_stage = smem + STAGES * STAGE_BYTES;  // two 16 KB output staging tiles
+  uint8_t* out_stage = smem + kStages * kSlot;  // two 16 KB output staging tiles
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(out_stage + 2 * OUT_BUF_BYTES);
-  uint64_t* empty_bar = full_bar + STAGES;
-  uint64_t* acc_full = empty_bar + STAGES;
+  uint64_t* empty_bar = full_bar + kStages;
+  uint64_t* acc_full = empty_bar + kStages;
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  __shared__ SlotNote<8> notes[kMode == 3 ? STAGES : 1];  // (kMode 3 alone uses these two)
-  __shared__ __align__(16) float bias_s[2][kMode == 3 ? BN : 4];
+  __shared__ SlotNote<8> notes[kMode == 3 ? kStages : 1];  // (kMode 3 alone uses these two)
+  __shared__ __align__(16) __nv_bfloat16 bias_s[2][kMode == 3 ? kCols : 8];
+  static_assert(kMode == 3 ? kCols % 64 == 0 && kCols <= BN : kCols == BN, "one 64-column piece is staged at a time");
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -628,7 +638,7 @@ gemm_pair_kernel(const __grid_constant__ G g) {
   DeviceStatus* const status = g.prob[0].p.status;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
+    for (int s = 0; s < kStages; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
@@ -675,7 +685,7 @@ gemm_pair_kernel(const __grid_constant__ G g) {
         n_blk = next_n;
         rows = next_rows;
         const int row0 = m_blk * 2 * BM + (int)rank * BM;
-        const int col0 = n_blk * BN + (int)rank * BNH;
+        const int col0 = n_blk * kCols + (int)rank * (kCols / 2);
         uint32_t off[8], next_off[8];
         int cur = -1;
         for (int kb = 0; kb < num_kb; ++kb) {
@@ -686,10 +696,10 @@ gemm_pair_kernel(const __grid_constant__ G g) {
           ok = ok && __all_sync(0xffffffffu, mbar_wait_cluster(&empty_bar[stage], phase ^ 1, abort_flag, status, 41));
           if (ok) {
             const uint32_t full_addr = map_to_cta(smem_u32(&full_bar[stage]), 0);
-            uint8_t* a_dst = smem + stage * STAGE_BYTES;
+            uint8_t* a_dst = smem + stage * kSlot;
             if (elect_one()) {
               if (kb == num_kb - 1) notes[stage].more = cur >= 0;
-              if (leader) mbar_expect_tx(&full_bar[stage], 2 * STAGE_BYTES);
+              if (leader) mbar_expect_tx(&full_bar[stage], 2 * kSlot);
               tma_load_2d_pair(a_dst, &pr.tm_a, full_addr, kb * BK, row0);
               tma_load_2d_pair(a_dst + A_BYTES, &pr.tm_b, full_addr, kb * BK, col0);
             }
@@ -709,12 +719,12 @@ gemm_pair_kernel(const __grid_constant__ G g) {
             ok = __all_sync(0xffffffffu, mbar_wait_cluster(&empty_bar[stage], phase ^ 1, abort_flag, status, 46));
             if (!ok) break;
             const uint32_t full_addr = map_to_cta(smem_u32(&full_bar[stage]), 0);
-            uint8_t* a_dst = smem + stage * STAGE_BYTES;
+            uint8_t* a_dst = smem + stage * kSlot;
             if (elect_one()) {
 #pragma unroll
               for (int i = 0; i < 8; ++i) notes[stage].off[i] = off[i];
               notes[stage].more = q + 1 < slots || next >= 0;
-              if (leader) mbar_expect_tx(&full_bar[stage], 2 * (BM * line * 2 + BNH * g.low.group * 2));
+              if (leader) mbar_expect_tx(&full_bar[stage], 2 * (BM * line * 2 + kCols / 2 * g.low.group * 2));
               tma_load_2d_pair(a_dst, &g.tm_t, full_addr, q * line, row0);
               tma_load_3d_pair(a_dst + A_BYTES, &g.tm_b, full_addr, (g.low.group == 64 ? q >> 1 : q) * g.low.group, col0, cur);
             }
@@ -742,9 +752,9 @@ gemm_pair_kernel(const __grid_constant__ G g) {
         const int col0 = n_blk * BN + (int)rank * BNH;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait_cluster(&empty_bar[stage], phase ^ 1, abort_flag, status, 41)) { ok = false; break; }
-          if (leader) mbar_expect_tx(&full_bar[stage], 2 * STAGE_BYTES);
+          if (leader) mbar_expect_tx(&full_bar[stage], 2 * kSlot);
           const uint32_t full_addr = map_to_cta(smem_u32(&full_bar[stage]), 0);
-          uint8_t* a_dst = smem + stage * STAGE_BYTES;
+          uint8_t* a_dst = smem + stage * kSlot;
           tma_load_2d_pair(a_dst, &pr.tm_a, full_addr, kb * BK, row0);
           tma_load_2d_pair(a_dst + A_BYTES, &pr.tm_b, full_addr, kb * BK, col0);
           if (++stage == g.pair_stages) { stage = 0; phase ^= 1; }
@@ -756,7 +766,7 @@ gemm_pair_kernel(const __grid_constant__ G g) {
     // The whole warp of the leader CTA walks the loop and an elected lane issues, so that
     // addresses and descriptors stay warp-uniform.
     if (leader) {
-      constexpr uint32_t idesc = make_idesc_bf16(2 * BM, BN, 0, 0);
+      constexpr uint32_t idesc = make_idesc_bf16(2 * BM, kCols, 0, 0);
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -775,7 +785,7 @@ gemm_pair_kernel(const __grid_constant__ G g) {
           if constexpr (kMode == 3) {
             if (kb == num_kb - 1) more = notes[stage].more;  // before the slot is given back
           }
-          const uint32_t a_addr = smem_u32(smem + stage * STAGE_BYTES);
+          const uint32_t a_addr = smem_u32(smem + stage * kSlot);
           const uint64_t adesc = make_smem_desc(a_addr, 16, 1024);
           const uint64_t bdesc = make_smem_desc(a_addr + A_BYTES, 16, 1024);
           if (elect_one()) {
@@ -793,7 +803,7 @@ gemm_pair_kernel(const __grid_constant__ G g) {
             tc_fence_after_sync();
             const SlotNote<8> note = notes[stage];
             more = note.more;
-            const uint32_t a_addr = smem_u32(smem + stage * STAGE_BYTES);
+            const uint32_t a_addr = smem_u32(smem + stage * kSlot);
             const uint64_t adesc = g.low.desc(a_addr);
             const uint64_t bdesc = g.low.group == 64   ? make_smem_desc(a_addr + A_BYTES, 16, 1024)
                                    : g.low.group == 32 ? make_smem_desc(a_addr + A_BYTES, 16, 512, 4)
@@ -839,11 +849,11 @@ gemm_pair_kernel(const __grid_constant__ G g) {
       const int row0 = m_blk * 2 * BM + (int)rank * BM;
       const int r_local = quad * 32 + lane;
       const int row = row0 + r_local;
-      const int n0 = n_blk * BN;
+      const int n0 = n_blk * kCols;
       const bool second = n0 >= p.split;
       if constexpr (kMode == 3) {
         // (a tile's bias is overwritten two tiles later, behind the barrier of the tile between)
-        bias_s[acc][threadIdx.x - 64] = bias_at(p, n0 + (int)threadIdx.x - 64);
+        if ((int)threadIdx.x - 64 < kCols) bias_s[acc][threadIdx.x - 64] = bias_at(p, n0 + (int)threadIdx.x - 64);
         asm volatile("bar.sync 3, 256;" ::: "memory");
       }
       if (!mbar_wait_cluster(&acc_full[acc], acc_phase, abort_flag, status, 45)) { ok = false; break; }
@@ -871,7 +881,7 @@ gemm_pair_kernel(const __grid_constant__ G g) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int c = eg + 2 * i;
-        if (n0 + c * OUT_CHUNK_COLS < p.N) {  // uniform
+        if (c * OUT_CHUNK_COLS < kCols && n0 + c * OUT_CHUNK_COLS < p.N) {  // uniform
           uint32_t r0[32], r1[32];
           tmem_ld_x32(t_addr + c * OUT_CHUNK_COLS, r0);
           tmem_ld_x32(t_addr + c * OUT_CHUNK_COLS + 32, r1);
@@ -957,7 +967,7 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], acc_full[2], acc_empty[2], t_full, t_empty;
   __shared__ SlotNote<4> notes[MAX_STAGES];
-  __shared__ __align__(16) float bias_s[2][BN];
+  __shared__ __align__(16) __nv_bfloat16 bias_s[2][BN];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   uint8_t* t_smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -1220,6 +1230,22 @@ static bool use_pair_kernel() {
   return pair_env != 0;
 }
 
+// The tile order for row blocks of `row_blk` and `concurrent` tiles at a time; p has M, N, K and tiles_n.
+static void choose_raster(fluxb::gemm::Params& p, int row_blk, int concurrent) {
+  // Keep the smaller operand resident in L2 when it fits, sweep the larger one.
+  const int tm = (p.M + row_blk - 1) / row_blk, tn = p.tiles_n;
+  const double a_bytes = 2.0 * (double)p.M * (double)p.K, w_bytes = 2.0 * (double)p.N * (double)p.K;
+  const double keep_limit = 48e6;
+  if (a_bytes <= w_bytes) {
+    p.raster_band_n = 0;  // keep x row-blocks
+    p.raster_group = a_bytes <= keep_limit ? tm : (concurrent / tn > 1 ? concurrent / tn : 1);
+  } else {
+    p.raster_band_n = 1;  // keep w row-blocks
+    p.raster_group = w_bytes <= keep_limit ? tn : (concurrent / tm > 1 ? concurrent / tm : 1);
+  }
+  if (p.raster_group < 1) p.raster_group = 1;
+}
+
 // Validates one problem, encodes its tensor maps and fills its kernel parameters.
 static int prepare_problem(const fluxb_linear_problem& a, int64_t N, int64_t K, int epi, int64_t split, int epi2,
                            int round_before_act, bool use_pair, CUtensorMap* tm_a, CUtensorMap* tm_b,
@@ -1282,23 +1308,7 @@ static int prepare_problem(const fluxb_linear_problem& a, int64_t N, int64_t K, 
   p.scat_groups = 0; p.scat_hpg = 1; p.scat_sb = p.scat_sh = p.scat_sl = p.scat_koff = p.scat_voff = 0;
   for (int gi = 0; gi < 8; ++gi) p.scat_base[gi] = nullptr;
   p.pair_stages = fluxb::gemm2::STAGES;
-  {
-    // Keep the smaller operand resident in L2 when it fits, sweep the larger one.
-    const int row_blk = use_pair ? 256 : 128;
-    const int tm = (int)((M + row_blk - 1) / row_blk);
-    const int tn = p.tiles_n;
-    const int concurrent = use_pair ? sm_count() / 2 : sm_count();
-    const double a_bytes = 2.0 * (double)M * (double)K, w_bytes = 2.0 * (double)N * (double)K;
-    const double keep_limit = 48e6;
-    if (a_bytes <= w_bytes) {
-      p.raster_band_n = 0;  // keep x row-blocks
-      p.raster_group = a_bytes <= keep_limit ? tm : (concurrent / tn > 1 ? concurrent / tn : 1);
-    } else {
-      p.raster_band_n = 1;  // keep w row-blocks
-      p.raster_group = w_bytes <= keep_limit ? tn : (concurrent / tm > 1 ? concurrent / tm : 1);
-    }
-    if (p.raster_group < 1) p.raster_group = 1;
-  }
+  choose_raster(p, use_pair ? 256 : 128, use_pair ? sm_count() / 2 : sm_count());
   return FLUXB_OK;
 }
 
@@ -1503,46 +1513,14 @@ static int encode_low_rank(CUtensorMap* out, const void* t_rows, int64_t M, cons
                           low.group == 16 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// The projection of fluxb_linear_lora for more rows than the row-streaming kernel takes; t as lora.cu leaves it.
-int fluxb::launch_lora_gemm(const fluxb_linear_problem& a, int64_t N, int64_t K, int epi, const void* t_rows,
-                            const void* lora_b, const LowRank& low, int64_t ldb, const RequestAdapters& req, cudaStream_t st) {
-  // Which tiles, by an estimate in cycles fitted to both kernels over 20 problems (9 to 31131 rows, K 96 to 4696, N 72 to
-  // 5496; it is within a fifth of each time and picks the faster kernel or one within 5 %).  A 256 x 256 tile of a CTA
-  // pair takes 700 per 64-wide K step, and at least the 7500 of its epilogue; a 128 x BN tile of one CTA takes two per
-  // operand row and step, and at least its own epilogue.  For example 1024 x 2048 -> 2048: pairs 19.2 us, BN 128 15.5,
-  // 64 21.6, 32 34.4; 128 x 1024 -> 4096: 13.8, 10.4, 9.7, 9.2; 4096 x 4096 -> 4096: 97.5, 129, 209, 385.
-  const int64_t kb = (K + 63) / 64, sms = sm_count();
-  const int64_t a_rows = a.M < 128 ? (a.M + 7) / 8 * 8 : 128;
-  const int64_t pair_tiles = ((a.M + 255) / 256) * ((N + 255) / 256);
-  int64_t best = (pair_tiles + sms / 2 - 1) / (sms / 2) * (700 * kb > 7500 ? 700 * kb : 7500) + 13000;
-  int bn = 256;
-  for (int c = 128; c >= 32; c /= 2) {
-    const int64_t tiles = ((a.M + 127) / 128) * ((N + c - 1) / c);
-    const int64_t steps = ((a_rows + c) * 2 + 100) * kb, epilogue = 1100 + 30 * c;
-    const int64_t t = (tiles + sms - 1) / sms * ((steps > epilogue ? steps : epilogue) + 1000) + 7000;
-    if (t < best) { best = t; bn = c; }
-  }
-  if (bn < 256) {
-    fluxb::gemm3::Tiles t;
-    int rc = prepare_problem(a, N, K, epi, N, FLUXB_EPI_NONE, 0, false, &t.tm_a, &t.tm_b, &t.p);
-    if (rc != FLUXB_OK) return rc;
-    t.req = req;
-    t.low = low;
-    t.a_rows = (int)a_rows;
-    {
-      const uint64_t dims[2] = {(uint64_t)K, (uint64_t)a.M}, strides[1] = {(uint64_t)a.ldx * 2};
-      const uint32_t box[2] = {64, (uint32_t)a_rows};
-      if ((rc = encode_tmap_bf16(&t.tm_a, a.x, 2, dims, strides, box)) != FLUXB_OK) return rc;
-    }
-    if ((rc = encode_low_rank(&t.tm_t, t_rows, a.M, low)) != FLUXB_OK) return rc;
-    if (bn == 128) return fluxb::gemm3::launch_tiles<128>(t, a, N, K, lora_b, ldb, st);
-    if (bn == 64) return fluxb::gemm3::launch_tiles<64>(t, a, N, K, lora_b, ldb, st);
-    return fluxb::gemm3::launch_tiles<32>(t, a, N, K, lora_b, ldb, st);
-  }
+// The adapter projection on CTA pairs: tiles of 256 rows and kCols columns.
+template <int kCols>
+static int launch_lora_pairs(const fluxb_linear_problem& a, int64_t N, int64_t K, int epi, const void* t_rows, const void* lora_b,
+                             const LowRank& low, int64_t ldb, const RequestAdapters& req, cudaStream_t st) {
   using namespace fluxb::gemm2;
   LoraGrouped g;
   g.count = 1;
-  g.pair_stages = STAGES;
+  g.pair_stages = LORA_STAGES;
   Problem& pr = g.prob[0];
   int rc = prepare_problem(a, N, K, epi, N, FLUXB_EPI_NONE, 0, true, &pr.tm_a, &pr.tm_b, &pr.p);
   if (rc != FLUXB_OK) return rc;
@@ -1552,12 +1530,19 @@ int fluxb::launch_lora_gemm(const fluxb_linear_problem& a, int64_t N, int64_t K,
     if ((rc = encode_tmap_bf16(&pr.tm_y, a.y, 2, dims, strides, box)) != FLUXB_OK) return rc;
     pr.tm_y2 = pr.tm_y;
   }
+  if (kCols < BN) {
+    const uint64_t dims[2] = {(uint64_t)K, (uint64_t)N}, strides[1] = {(uint64_t)a.ldw * 2};
+    const uint32_t box[2] = {BK, kCols / 2};
+    if ((rc = encode_tmap_bf16(&pr.tm_b, a.w, 2, dims, strides, box)) != FLUXB_OK) return rc;
+    pr.p.tiles_n = (int)((N + kCols - 1) / kCols);
+    choose_raster(pr.p, 2 * BM, sm_count() / 2);
+  }
   g.low = low;
   if ((rc = encode_low_rank(&g.tm_t, t_rows, a.M, low)) != FLUXB_OK) return rc;
   {
     const uint64_t dims[3] = {(uint64_t)low.R, (uint64_t)N, (uint64_t)req.n_adapters};
     const uint64_t strides[2] = {(uint64_t)ldb * 2, (uint64_t)(N * ldb) * 2};
-    const uint32_t box[3] = {(uint32_t)low.group, BNH, 1};
+    const uint32_t box[3] = {(uint32_t)low.group, kCols / 2, 1};
     const CUtensorMapSwizzle swz = low.group == 64   ? CU_TENSOR_MAP_SWIZZLE_128B
                                    : low.group == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
                                                      : CU_TENSOR_MAP_SWIZZLE_32B;
@@ -1567,13 +1552,78 @@ int fluxb::launch_lora_gemm(const fluxb_linear_problem& a, int64_t N, int64_t K,
   pr.tiles_m = (int)((a.M + 255) / 256);
   pr.tile_start = 0;
   g.total_tiles = pr.tiles_m * pr.p.tiles_n;
-  auto kern = gemm_pair_kernel<3, LoraGrouped>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+  auto kern = gemm_pair_kernel<3, LoraGrouped, kCols>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, lora_smem(kCols));
   if (e != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "linear_lora: cannot set shared memory size: %s", cudaGetErrorString(e));
   const int pairs = g.total_tiles < sm_count() / 2 ? g.total_tiles : sm_count() / 2;
-  e = launch_after(kern, 2 * pairs, THREADS, SMEM_BYTES, st, g);
+  e = launch_after(kern, 2 * pairs, THREADS, lora_smem(kCols), st, g);
   if (e != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "linear_lora: launch failed: %s", cudaGetErrorString(e));
   return FLUXB_OK;
+}
+
+// Which tiles, and over how many blocks the kernel of the low-rank rows splits K, by an estimate in cycles.  The tiles'
+// part is fitted to the kernels over 20 problems (9 to 31131 rows, K 96 to 4696, N 72 to 5496) and within a fifth of each
+// time: a tile of a CTA pair takes 400 and 75 per 64 columns for a 64-wide K step, and at least 7500 for its epilogue; a
+// 128 x BN tile of one CTA takes two per operand row and step, and at least its own epilogue.  For example
+// 2048 x 3072 -> 3072: pairs 256 wide 39.1 us (two rounds of 96 tiles on 74 pairs), 192 wide 36.4; 4096 x 4096 -> 4096:
+// 95.4 and 105; 1024 x 2048 -> 2048: pairs 18.7, BN 128 15.5, 64 21.6, 32 34.4; 128 x 1024 -> 4096: 13.8, 10.4, 9.7, 9.2.
+// A ring slot of adapters takes 550, for as many adapters as a tile's rows may use.
+// The low-rank rows run beside the projection's first tiles, on SMs of their own: SMs whose projection blocks have a tile
+// less to do than the others cost nothing as long as t is there when the first tile needs it (4 x 512 rows, 192 wide,
+// 20 spare pairs: 43.3 us with 64 blocks of low-rank rows, 37.7 with 16); others wait for some 0.6 of their time (700
+// rows of three requests, K 2048, 72 tiles on 74 pairs: 20.3 us without, 25.1 with 72 blocks, 26.7 with 18).
+LoraPlan fluxb::plan_lora(int64_t M, int64_t N, int64_t K, const RequestAdapters& req, const LowRank& low) {
+  const int64_t L = req.length, rpad = low.units * 16;
+  const int64_t shrink_rows = L < 128 ? L : 128, shrink_tiles = L <= kLoraShort ? 0 : M / L * ((L + 127) / 128);
+  const int64_t kb = (K + 63) / 64, sms = sm_count();
+  const int64_t a_rows = M < 128 ? (M + 7) / 8 * 8 : 128;
+  LoraPlan plan{};
+  int64_t best = INT64_MAX;
+  for (int c : {256, 192, 128, 64, 32}) {
+    const bool pair = c > 128;
+    const int64_t tiles = (M + (pair ? 255 : 127)) / (pair ? 256 : 128) * ((N + c - 1) / c);
+    const int64_t steps = (pair ? 400 + 75 * c / 64 : (a_rows + c) * 2 + 100) * kb, epilogue = pair ? 7500 : 1100 + 30 * c;
+    const int64_t rows = pair ? 256 : 128, requests = L % rows == 0 ? 1 : (rows + L - 2) / L + 1;
+    const int64_t slots = (pair ? fluxb::gemm2::lora_slots(low) : (low.units + 3) / 4) * (requests < req.n_adapters ? requests : req.n_adapters);
+    const int64_t tile = (steps > epilogue ? steps : epilogue) + slots * 550 + (pair ? 0 : 1000);
+    const int64_t units = pair ? sms / 2 : sms, rounds = (tiles + units - 1) / units;
+    const int64_t spare = (rounds * units - tiles) * (pair ? 2 : 1);
+    int64_t shrink = shrink_tiles > 0 ? INT64_MAX : 0;
+    int ksplit = 1;
+    // (clusters of eight do not all find a place at once from 16 on: 2048 rows, K 3072 alone: 16.7 us with eight, 9.9
+    // with four, 12.0 with two)
+    for (int ks = 1; shrink_tiles > 0 && ks <= (shrink_tiles < 12 ? 8 : 4); ks *= 2) {
+      if (ks > 1 && (shrink_tiles * ks > sms || kb < ks * 4)) break;
+      int64_t t = (9000 + (kb + ks - 1) / ks * ((shrink_rows + rpad) * 2 + 100)) * ((shrink_tiles * ks + sms - 1) / sms);
+      t = shrink_tiles * ks <= spare ? (t > tile ? t - tile : 0) : t * 3 / 5;
+      if (t < shrink) { shrink = t; ksplit = ks; }
+    }
+    const int64_t all = rounds * tile + (pair ? 13000 : 7000) + shrink;
+    if (all < best) { best = all; plan = LoraPlan{c, ksplit}; }
+  }
+  return plan;
+}
+
+// The projection of fluxb_linear_lora for more rows than the row-streaming kernel takes; t as lora.cu leaves it.
+int fluxb::launch_lora_gemm(const LoraPlan& plan, const fluxb_linear_problem& a, int64_t N, int64_t K, int epi, const void* t_rows,
+                            const void* lora_b, const LowRank& low, int64_t ldb, const RequestAdapters& req, cudaStream_t st) {
+  if (plan.cols == 256) return launch_lora_pairs<256>(a, N, K, epi, t_rows, lora_b, low, ldb, req, st);
+  if (plan.cols == 192) return launch_lora_pairs<192>(a, N, K, epi, t_rows, lora_b, low, ldb, req, st);
+  fluxb::gemm3::Tiles t;
+  int rc = prepare_problem(a, N, K, epi, N, FLUXB_EPI_NONE, 0, false, &t.tm_a, &t.tm_b, &t.p);
+  if (rc != FLUXB_OK) return rc;
+  t.req = req;
+  t.low = low;
+  t.a_rows = (int)(a.M < 128 ? (a.M + 7) / 8 * 8 : 128);
+  {
+    const uint64_t dims[2] = {(uint64_t)K, (uint64_t)a.M}, strides[1] = {(uint64_t)a.ldx * 2};
+    const uint32_t box[2] = {64, (uint32_t)t.a_rows};
+    if ((rc = encode_tmap_bf16(&t.tm_a, a.x, 2, dims, strides, box)) != FLUXB_OK) return rc;
+  }
+  if ((rc = encode_low_rank(&t.tm_t, t_rows, a.M, low)) != FLUXB_OK) return rc;
+  if (plan.cols == 128) return fluxb::gemm3::launch_tiles<128>(t, a, N, K, lora_b, ldb, st);
+  if (plan.cols == 64) return fluxb::gemm3::launch_tiles<64>(t, a, N, K, lora_b, ldb, st);
+  return fluxb::gemm3::launch_tiles<32>(t, a, N, K, lora_b, ldb, st);
 }
 
 extern "C" int fluxb_linear(const void* x, const void* w, const void* bias, void* y, int64_t M,

@@ -23,7 +23,7 @@ struct Params {
   const float* scale;  // nullptr: ones
   __nv_bfloat16* t;    // [M, low.ld()]
   LowRank low;
-  int L, tiles_per_request, box_rows;
+  int L, tiles, tiles_per_request, box_rows;
   int num_kb, ksplit, rpad, stages, subs, tmem_cols;  // subs: 64-wide K steps per ring slot
   DeviceStatus* status;
 };
@@ -34,9 +34,10 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
   return v;
 }
 
-// One cluster of `ksplit` CTAs per 128 rows of one request: each CTA multiplies its share of K (x and A tiles by TMA,
-// fp32 accumulator in TMEM, N = the rank in sixteens), leaves its partial sums in shared memory, and after a cluster
-// barrier each takes a share of the outputs, adds the partial sums in a fixed order, scales, splits and stores.
+// One cluster of `ksplit` CTAs per 128 rows of one request (ksplit 1: clusters of two CTAs that do not meet): each CTA
+// multiplies its share of K (x and A tiles by TMA, fp32 accumulator in TMEM, N = the rank in sixteens), leaves its
+// partial sums in shared memory, and after a cluster barrier each takes a share of the outputs, adds the partial sums
+// in a fixed order, scales, splits and stores.
 __global__ void __launch_bounds__(THREADS, 1) lora_shrink_kernel(const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], acc_full;
@@ -45,8 +46,9 @@ __global__ void __launch_bounds__(THREADS, 1) lora_shrink_kernel(const __grid_co
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = (int)cluster_ctarank();
+  const int in_cluster = (int)cluster_ctarank(), rank = p.ksplit > 1 ? in_cluster : 0;
   const int tile = blockIdx.x / p.ksplit;
+  if (tile >= p.tiles) return;
   const int request = tile / p.tiles_per_request;
   const int l0 = (tile - request * p.tiles_per_request) * BM;
   const int row0 = request * p.L + l0;
@@ -155,7 +157,7 @@ __global__ void __launch_bounds__(THREADS, 1) lora_shrink_kernel(const __grid_co
     tc_fence_after_sync();
     tmem_dealloc(tmem_base, p.tmem_cols);
   }
-  cluster_sync_all();
+  if (p.ksplit > 1) cluster_sync_all();
   const float scale = p.scale != nullptr ? p.scale[adapter] : 1.f;
   const int t_ld = p.low.ld();
   const int eights = p.rpad / 8;
@@ -165,7 +167,7 @@ __global__ void __launch_bounds__(THREADS, 1) lora_shrink_kernel(const __grid_co
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
       if (s < p.ksplit) {
-        const uint32_t src = map_to_cta(smem_u32(part + row * pitch + c8), (uint32_t)s);
+        const uint32_t src = map_to_cta(smem_u32(part + row * pitch + c8), (uint32_t)(in_cluster - rank + s));
         lo4[s] = ld_cluster_f32x4(src);
         hi4[s] = ld_cluster_f32x4(src + 16);
       }
@@ -194,13 +196,13 @@ __global__ void __launch_bounds__(THREADS, 1) lora_shrink_kernel(const __grid_co
     *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     *reinterpret_cast<uint4*>(dst + p.low.group) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
-  cluster_sync_all();  // no CTA leaves while another reads its partial sums
+  if (p.ksplit > 1) cluster_sync_all();  // no CTA leaves while another reads its partial sums
 }
 
 }  // namespace shrink
 
 static int launch_shrink(const void* x, int64_t ldx, const void* lora_a, const float* scale, void* t, const RequestAdapters& req,
-                         int64_t B, int64_t L, int64_t K, const LowRank& low, cudaStream_t st) {
+                         int64_t B, int64_t L, int64_t K, const LowRank& low, int ksplit, cudaStream_t st) {
   using namespace shrink;
   Params p;
   p.req = req;
@@ -214,10 +216,8 @@ static int launch_shrink(const void* x, int64_t ldx, const void* lora_a, const f
   p.num_kb = (int)((K + BK - 1) / BK);
   p.status = device_status_ptr();
   const int64_t tiles = B * p.tiles_per_request;
-  // K is split until the clusters fill the machine, as long as a CTA keeps four 64-wide steps.  Clusters of eight do
-  // not all find a place at once from 16 on (2048 rows, K 3072: 16.7 us with eight, 9.9 with four, 12.0 with two).
-  p.ksplit = 1;
-  while (p.ksplit < (tiles < 12 ? 8 : 4) && tiles * p.ksplit * 2 <= sm_count() && p.num_kb >= p.ksplit * 2 * 4) p.ksplit *= 2;
+  p.tiles = (int)tiles;
+  p.ksplit = ksplit;
   const int step_bytes = BM * BK * 2 + p.rpad * BK * 2;
   // two K steps per slot where three slots fit: a slot costs its warps some 500 cycles each
   p.subs = MAX_SMEM / step_bytes >= 6 ? 2 : 1;
@@ -247,13 +247,16 @@ static int launch_shrink(const void* x, int64_t ldx, const void* lora_a, const f
   cudaError_t e = cudaFuncSetAttribute(lora_shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM + 1024);
   if (e != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "linear_lora: cannot set shared memory size: %s", cudaGetErrorString(e));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * p.ksplit));
+  // Where K is not split, a cluster is two neighbouring tiles: the projection's CTA pairs start beside this kernel and
+  // need both SMs of a pair free.
+  const unsigned cluster = ksplit > 1 ? (unsigned)ksplit : 2;
+  cfg.gridDim = dim3((unsigned)((tiles * ksplit + cluster - 1) / cluster * cluster));
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)p.ksplit;
+  attr[0].val.clusterDim.x = cluster;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
@@ -269,7 +272,7 @@ static int launch_shrink(const void* x, int64_t ldx, const void* lora_a, const f
 // beside it.
 // ----------------------------------------------------------------------------------------
 namespace shrink {
-constexpr int SHORT = 8;
+constexpr int SHORT = kLoraShort;
 struct ShortParams {
   const __nv_bfloat16 *x, *a;
   const float* scale;
@@ -646,14 +649,17 @@ extern "C" int fluxb_linear_lora(const void* x, const void* w, const void* bias,
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const RequestAdapters req{adapter, adapter_is64, (int)L, (int)n_adapters};
   const LowRank low(R);
-  int rc = L <= shrink::SHORT ? launch_shrink_short(x, ldx, lora_a, lora_scale, scratch, req, B, K, low, st)
-                              : launch_shrink(x, ldx, lora_a, lora_scale, scratch, req, B, L, K, low, st);
+  const bool brief = L <= kLoraShort;
+  const int64_t M = B * L;
+  const LoraPlan plan = M <= 8 ? LoraPlan{} : plan_lora(M, N, K, req, low);
+  int rc = brief ? launch_shrink_short(x, ldx, lora_a, lora_scale, scratch, req, B, K, low, st)
+                 : launch_shrink(x, ldx, lora_a, lora_scale, scratch, req, B, L, K, low, plan.ksplit, st);
   if (rc != FLUXB_OK) return rc;
   fluxb_linear_problem a = {};
-  a.x = x; a.w = w; a.bias = bias; a.y = y; a.M = B * L; a.ldx = ldx; a.ldw = ldw; a.ldy = ldy;
+  a.x = x; a.w = w; a.bias = bias; a.y = y; a.M = M; a.ldx = ldx; a.ldw = ldw; a.ldy = ldy;
   a.rows_per_batch = 1;
   rc = a.M <= 8 ? launch_rows(a, N, K, epi, scratch, lora_b, low, ldb, req, st)
-                : launch_lora_gemm(a, N, K, epi, scratch, lora_b, low, ldb, req, st);
+                : launch_lora_gemm(plan, a, N, K, epi, scratch, lora_b, low, ldb, req, st);
   if (rc != FLUXB_OK) return rc;
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "linear_lora: launch failed: %s", cudaGetErrorString(e));

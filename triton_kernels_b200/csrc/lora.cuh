@@ -43,7 +43,14 @@ struct LowRank {
   __device__ __forceinline__ int low(int i) const { return 2 * i + (group == 64 ? 1024 : group / 8); }
 };
 
-int launch_lora_gemm(const fluxb_linear_problem& a, int64_t N, int64_t K, int epi, const void* t, const void* lora_b,
+// How a problem of more than eight rows runs: columns per tile of the projection (256 and 192: CTA pairs, 256 rows; less:
+// single CTAs, 128 rows), and the blocks among which the low-rank rows of 128 rows of a request split K.
+struct LoraPlan {
+  int cols, ksplit;
+};
+LoraPlan plan_lora(int64_t M, int64_t N, int64_t K, const RequestAdapters& req, const LowRank& low);
+constexpr int kLoraShort = 8;  // requests of up to so many rows take another kernel for their low-rank rows
+int launch_lora_gemm(const LoraPlan& plan, const fluxb_linear_problem& a, int64_t N, int64_t K, int epi, const void* t, const void* lora_b,
                      const LowRank& low, int64_t ldb, const RequestAdapters& req, cudaStream_t st);
 
 }  // namespace fluxb
