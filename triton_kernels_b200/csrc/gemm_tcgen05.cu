@@ -435,9 +435,8 @@ __device__ __forceinline__ __nv_bfloat16 bias_at(const Params& p, int col) {
 // What the producer leaves beside a ring slot for the MMA warp: of an adapter's slot the mask of the rows that it leaves
 // alone, and of the last slot of a K loop and of every adapter's whether another adapter's slot follows.  The MMA warp
 // reads it behind its wait for the slot (the producer's arrival there releases it) and so has nothing to find out.
-template <int W>
 struct SlotNote {
-  uint32_t off[W];
+  uint32_t off[8];
   uint32_t more;
 };
 // A ring slot of the adapters: a line of t and a group of B; a group of 64 takes two (high parts, low parts).
@@ -625,7 +624,7 @@ gemm_pair_kernel(const __grid_constant__ G g) {
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  __shared__ SlotNote<8> notes[kMode == 3 ? kStages : 1];  // (kMode 3 alone uses these two)
+  __shared__ SlotNote notes[kMode == 3 ? kStages : 1];  // (kMode 3 alone uses these two)
   __shared__ __align__(16) __nv_bfloat16 bias_s[2][kMode == 3 ? kCols : 8];
   static_assert(kMode == 3 ? kCols % 64 == 0 && kCols <= BN : kCols == BN, "one 64-column piece is staged at a time");
   const int warp = threadIdx.x >> 5;
@@ -801,7 +800,7 @@ gemm_pair_kernel(const __grid_constant__ G g) {
             ok = __all_sync(0xffffffffu, mbar_wait_cluster(&full_bar[stage], phase, abort_flag, status, 47));
             if (!ok) break;
             tc_fence_after_sync();
-            const SlotNote<8> note = notes[stage];
+            const SlotNote note = notes[stage];
             more = note.more;
             const uint32_t a_addr = smem_u32(smem + stage * kSlot);
             const uint64_t adesc = g.low.desc(a_addr);
@@ -941,13 +940,13 @@ namespace gemm3 {
 using gemm::BK;
 using gemm::BM;
 using gemm::Params;
-using gemm2::SlotNote;
 using gemm2::TileAdapters;
 using gemm2::bias_at;
 using gemm2::finish32;
-constexpr int THREADS = 192;
+constexpr int THREADS = 224;  // TMA warp, MMA warp, four epilogue warps, a warp that lists the adapters
 constexpr int MAX_STAGES = 16;
-constexpr int MAX_SMEM = 224 * 1024;
+constexpr int MAX_SMEM = 220 * 1024;
+constexpr int CHUNKS = 4;  // tiles of B per ring slot, at most
 
 struct Tiles {
   CUtensorMap tm_a, tm_b, tm_t, tm_lb;
@@ -960,13 +959,22 @@ struct Tiles {
                // shared memory as the other rows, whose results are never stored
 };
 
+// The adapters of a tile's rows, each with the mask of the rows that do not use it.  A warp of its own writes the list
+// while the tile's K loop runs: with the search in the producer and a ring slot for each adapter, an adapter cost its warp
+// and the MMA warp 850 cycles each (the search 345, waits, barrier updates and the copy's issue the rest).
+struct AdapterList {
+  uint4 off[BM];
+  int id[BM];
+  int count;
+};
+
 template <int BN>
 __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_constant__ Tiles g) {
   constexpr int B_BYTES = BN * BK * 2;
   const int A_BYTES = g.a_rows * BK * 2, SLOT_A = g.subs * A_BYTES, STAGE_BYTES = SLOT_A + g.subs * B_BYTES;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], acc_full[2], acc_empty[2], t_full, t_empty;
-  __shared__ SlotNote<4> notes[MAX_STAGES];
+  __shared__ uint64_t full_bar[MAX_STAGES], empty_bar[MAX_STAGES], acc_full[2], acc_empty[2], list_full[2], list_empty[2], t_full, t_empty;
+  __shared__ AdapterList lists[2];
   __shared__ __align__(16) __nv_bfloat16 bias_s[2][BN];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
@@ -977,7 +985,8 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
   const Params& p = g.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int num_kb = (p.K + BK - 1) / BK;
-  const int slots = (g.low.units + 3) / 4;  // of 64 ranks of B
+  const int parts = (g.low.units + 3) / 4;  // of 64 ranks of B
+  const int chunks = min(CHUNKS, STAGE_BYTES / B_BYTES);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < g.stages; ++s) {
@@ -987,6 +996,8 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
       mbar_init(&acc_empty[a], 128);
+      mbar_init(&list_full[a], 1);
+      mbar_init(&list_empty[a], 2);
     }
     mbar_init(&t_full, 1);
     mbar_init(&t_empty, 1);
@@ -1010,64 +1021,53 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
     int stage = 0;
     uint32_t phase = 0, t_phase = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; ok && tile < p.num_tiles; tile += gridDim.x) {
+    int local = 0;
+    for (int tile = blockIdx.x; ok && tile < p.num_tiles; tile += gridDim.x, ++local) {
       const int row0 = tile % p.tiles_m * BM, col0 = tile / p.tiles_m * BN;
-      TileAdapters<4> rows;
-      rows.fetch(g.req, row0, p.M, lane);
-      uint32_t off[4], next_off[4];
-      int cur = -1;
       for (int kb = 0; kb < num_kb; kb += g.subs) {
         const int subs = min(g.subs, num_kb - kb);
-        const bool last = kb + g.subs >= num_kb;
-        if (last) {
-          rows.begin();
-          cur = rows.next(off);
-        }
-        ok = ok && __all_sync(0xffffffffu, mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, 91));
-        if (ok) {
-          uint8_t* dst = smem + stage * STAGE_BYTES;
-          if (elect_one()) {
-            if (last) notes[stage].more = cur >= 0;
-            mbar_expect_tx(&full_bar[stage], subs * (A_BYTES + B_BYTES));
-            for (int i = 0; i < subs; ++i) {
-              tma_load_2d(dst + i * A_BYTES, &g.tm_a, &full_bar[stage], (kb + i) * BK, row0);
-              tma_load_2d(dst + SLOT_A + i * B_BYTES, &g.tm_b, &full_bar[stage], (kb + i) * BK, col0);
-            }
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, 91));
+        if (!ok) break;
+        uint8_t* dst = smem + stage * STAGE_BYTES;
+        if (elect_one()) {
+          mbar_expect_tx(&full_bar[stage], subs * (A_BYTES + B_BYTES));
+          for (int i = 0; i < subs; ++i) {
+            tma_load_2d(dst + i * A_BYTES, &g.tm_a, &full_bar[stage], (kb + i) * BK, row0);
+            tma_load_2d(dst + SLOT_A + i * B_BYTES, &g.tm_b, &full_bar[stage], (kb + i) * BK, col0);
           }
-          if (++stage == g.stages) { stage = 0; phase ^= 1; }
         }
+        if (++stage == g.stages) { stage = 0; phase ^= 1; }
       }
-      __syncwarp();
-      if (tile == (int)blockIdx.x) pdl_wait();  // t is complete
-      bool first = true;
-      while (cur >= 0) {
-        const int next = rows.next(next_off);
-        if (first) {
-          ok = ok && __all_sync(0xffffffffu, mbar_wait(&t_empty, t_phase ^ 1, abort_flag, p.status, 92));
+      const int buf = local & 1;
+      const AdapterList& list = lists[buf];
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(&list_full[buf], (local >> 1) & 1, abort_flag, p.status, 92));
+      const int total = ok ? list.count * parts : 0;
+      for (int c = 0; ok && c < total; c += chunks) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, 93));
+        if (!ok) break;
+        const int n = min(chunks, total - c);
+        if (elect_one()) {
+          mbar_expect_tx(&full_bar[stage], n * B_BYTES);
+          for (int i = 0; i < n; ++i) {
+            const int item = (c + i) / parts, part = c + i - item * parts;
+            tma_load_3d(smem + stage * STAGE_BYTES + i * B_BYTES, &g.tm_lb, &full_bar[stage], part * 64, col0, list.id[item]);
+          }
+        }
+        if (++stage == g.stages) { stage = 0; phase ^= 1; }
+        if (c == 0) {  // t, as soon as it is complete
+          if (tile == (int)blockIdx.x) pdl_wait();
+          ok = __all_sync(0xffffffffu, mbar_wait(&t_empty, t_phase ^ 1, abort_flag, p.status, 99));
+          t_phase ^= 1;
           if (ok && elect_one()) {
             const int line = g.low.group == 16 ? 32 : 64;
             mbar_expect_tx(&t_full, T_BYTES);
-            for (int c = 0; c < g.low.ld(); c += line) tma_load_2d(t_smem + c * BM * 2, &g.tm_t, &t_full, c, row0);
+            for (int k = 0; k < g.low.ld(); k += line) tma_load_2d(t_smem + k * BM * 2, &g.tm_t, &t_full, k, row0);
           }
         }
-        for (int q = 0; ok && q < slots; ++q) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, 93));
-          if (!ok) break;
-          if (elect_one()) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) notes[stage].off[i] = off[i];
-            notes[stage].more = q + 1 < slots || next >= 0;
-            mbar_expect_tx(&full_bar[stage], B_BYTES);
-            tma_load_3d(smem + stage * STAGE_BYTES + SLOT_A, &g.tm_lb, &full_bar[stage], q * 64, col0, cur);
-          }
-          if (++stage == g.stages) { stage = 0; phase ^= 1; }
-        }
-        if (first) t_phase ^= 1;
-        first = false;
-        cur = next;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) off[i] = next_off[i];
       }
+      if (tile == (int)blockIdx.x && total == 0) pdl_wait();  // every CTA waits for the first kernel, with adapters or without
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&list_empty[buf]);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -1079,16 +1079,14 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
     for (int tile = blockIdx.x; ok && tile < p.num_tiles; tile += gridDim.x, ++local) {
       const int acc = local & 1;
       const uint32_t acc_phase = (local >> 1) & 1;
-      ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[acc], acc_phase ^ 1, abort_flag, p.status, 94));
+      ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[acc], acc_phase ^ 1, abort_flag, p.status, 100));
       if (!ok) break;
       tc_fence_after_sync();
       const uint32_t d_tmem = tmem_base + acc * BN;
-      uint32_t more = 0;
       for (int kb = 0; kb < num_kb; kb += g.subs) {
         ok = __all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, abort_flag, p.status, 95));
         if (!ok) break;
         tc_fence_after_sync();
-        if (kb + g.subs >= num_kb) more = notes[stage].more;  // before the slot is given back
         const int subs = min(g.subs, num_kb - kb);
         const uint32_t a_addr = smem_u32(smem + stage * STAGE_BYTES);
         const uint64_t adesc = make_smem_desc(a_addr, 16, 1024), bdesc = make_smem_desc(a_addr + SLOT_A, 16, 1024);
@@ -1102,35 +1100,68 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
         }
         if (++stage == g.stages) { stage = 0; phase ^= 1; }
       }
-      const bool any = more != 0;
-      if (ok && any) {
+      const int buf = local & 1;
+      const AdapterList& list = lists[buf];
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(&list_full[buf], (local >> 1) & 1, abort_flag, p.status, 94));
+      const int total = ok ? list.count * parts : 0;
+      const bool any = total > 0;
+      if (any) {
         ok = __all_sync(0xffffffffu, mbar_wait(&t_full, t_phase, abort_flag, p.status, 96));
         t_phase ^= 1;
       }
-      for (int q = 0; ok && more != 0;) {
+      for (int c = 0; ok && c < total; c += chunks) {
         ok = __all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, abort_flag, p.status, 97));
         if (!ok) break;
         tc_fence_after_sync();
-        const SlotNote<4> note = notes[stage];
-        more = note.more;
-        // (more than 64 ranks: groups of 64, one per slot; up to 64 there is one group and one slot)
-        const uint64_t adesc = g.low.desc(smem_u32(t_smem + q * g.low.tile_bytes()));
-        const uint64_t bdesc = make_smem_desc(smem_u32(smem + stage * STAGE_BYTES) + SLOT_A, 16, 1024);
-        const int n_units = min(4, g.low.units - q * 4);
+        const int n = min(chunks, total - c);
+        const uint64_t bdesc = make_smem_desc(smem_u32(smem + stage * STAGE_BYTES), 16, 1024);
         if (elect_one()) {
-          for (int i = 0; i < n_units; ++i) {
-            umma_ss_masked(d_tmem, adesc + g.low.high(i), bdesc + 2 * i, idesc, note.off);
-            umma_ss_masked(d_tmem, adesc + g.low.low(i), bdesc + 2 * i, idesc, note.off);
+          for (int i = 0; i < n; ++i) {
+            // (more than 64 ranks: groups of 64, one per part; up to 64 there is one group and one part)
+            const int item = (c + i) / parts, part = c + i - item * parts;
+            const uint64_t ad = g.low.desc(smem_u32(t_smem + part * g.low.tile_bytes())), bd = bdesc + i * (B_BYTES >> 4);
+            const uint4 o = list.off[item];
+            const uint32_t off[4] = {o.x, o.y, o.z, o.w};
+            const int n_units = min(4, g.low.units - part * 4);
+            for (int u = 0; u < n_units; ++u) {
+              umma_ss_masked(d_tmem, ad + g.low.high(u), bd + 2 * u, idesc, off);
+              umma_ss_masked(d_tmem, ad + g.low.low(u), bd + 2 * u, idesc, off);
+            }
           }
           umma_commit(&empty_bar[stage]);
         }
-        if (++q == slots) q = 0;
         if (++stage == g.stages) { stage = 0; phase ^= 1; }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&list_empty[buf]);
       if (ok && elect_one()) {
         if (any) umma_commit(&t_empty);
         umma_commit(&acc_full[acc]);
       }
+    }
+    __syncwarp();
+  } else if (warp == 6) {
+    int local = 0;
+    for (int tile = blockIdx.x; tile < p.num_tiles; tile += gridDim.x, ++local) {
+      TileAdapters<4> rows;
+      rows.fetch(g.req, tile % p.tiles_m * BM, p.M, lane);
+      const int buf = local & 1;
+      if (!__all_sync(0xffffffffu, mbar_wait(&list_empty[buf], ((local >> 1) & 1) ^ 1, abort_flag, p.status, 101))) break;
+      AdapterList& list = lists[buf];
+      rows.begin();
+      uint32_t off[4];
+      int n = 0;
+      for (int cur = rows.next(off); cur >= 0; cur = rows.next(off), ++n) {
+        if (lane == 0) {
+          list.off[n] = make_uint4(off[0], off[1], off[2], off[3]);
+          list.id[n] = cur;
+        }
+      }
+      if (lane == 0) {
+        list.count = n;
+        mbar_arrive(&list_full[buf]);
+      }
+      __syncwarp();
     }
     __syncwarp();
   } else {

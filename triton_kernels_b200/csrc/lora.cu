@@ -6,6 +6,7 @@
 // between the two products.  An adapter index outside [-1, n) leaves its request without an adapter and is recorded
 // in the device status word (site 81).
 #include "lora.cuh"
+#include "vec.cuh"
 
 namespace fluxb {
 
@@ -284,46 +285,55 @@ struct ShortParams {
   DeviceStatus* status;
 };
 
-// Four warps share K; a block takes kRanks ranks of one request.
-template <int kRanks>
-__global__ void __launch_bounds__(128) lora_shrink_short_kernel(const ShortParams p) {
-  __shared__ float red[4][kRanks][SHORT];
+__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                            uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// One value of t, scaled and split; a rank behind R (zeros, which would be NaN beside an infinite x) is zero.
+__device__ __forceinline__ void store_low_rank(const ShortParams& p, int adapter, int64_t row, int j, float v) {
+  v = j < p.low.R ? v * (p.scale != nullptr ? p.scale[adapter] : 1.f) : 0.f;
+  const __nv_bfloat16 hi = __float2bfloat16_rn(v);
+  const float h = __bfloat162float(hi);
+  __nv_bfloat16* dst = p.t + row * p.low.ld() + p.low.column(j);
+  dst[0] = hi;
+  dst[p.low.group] = __float2bfloat16_rn(isinf(h) ? 0.f : v - h);
+}
+
+// Few requests: a block per rank, four warps sharing K, so that the reading of A is spread over the machine.
+__global__ void __launch_bounds__(128) lora_shrink_one_kernel(const ShortParams p) {
+  __shared__ float red[4][SHORT];
   const int ranks = p.low.units * 16;  // the ranks behind R are zeros: the tensor cores multiply them, too
-  const int request = blockIdx.x / (ranks / kRanks), j0 = (blockIdx.x - request * (ranks / kRanks)) * kRanks;
+  const int request = blockIdx.x / ranks, j = blockIdx.x - request * ranks;
   const int L = p.req.length, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_release();  // (its stream of W does not get in front: the loads here are all on their way within the launch)
   const int adapter = p.req.of_request(request);
   if (adapter < 0) {
-    if (j0 == 0 && threadIdx.x == 0 && p.req.raw(request) != -1) report_error(p.status, FLUXB_ERR_BAD_ARG, 81);
+    if (j == 0 && threadIdx.x == 0 && p.req.raw(request) != -1) report_error(p.status, FLUXB_ERR_BAD_ARG, 81);
     return;
   }
-  const __nv_bfloat16* a = p.a + ((int64_t)adapter * p.low.R + j0) * p.K;
+  const __nv_bfloat16* a = p.a + ((int64_t)adapter * p.low.R + j) * p.K;
   const __nv_bfloat16* x = p.x + (int64_t)request * L * p.ldx;
-  float acc[kRanks][SHORT] = {};
-  constexpr int kAhead = kRanks == 1 ? 4 : 1;  // steps whose loads are in flight together
+  float acc[SHORT] = {};
+  constexpr int kAhead = 4;  // steps whose loads are in flight together
   for (int k0 = threadIdx.x * 8; k0 < p.K; k0 += 1024 * kAhead) {
-    uint4 av[kAhead][kRanks];
+    uint4 av[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
-#pragma unroll
-      for (int r = 0; r < kRanks; ++r)
-        av[i][r] = k0 + i * 1024 < p.K && j0 + r < p.low.R ? __ldg(reinterpret_cast<const uint4*>(a + (int64_t)r * p.K + k0 + i * 1024))
-                                                          : make_uint4(0, 0, 0, 0);
+      av[i] = k0 + i * 1024 < p.K && j < p.low.R ? __ldg(reinterpret_cast<const uint4*>(a + k0 + i * 1024)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       if (k0 + i * 1024 >= p.K) break;
+      const uint32_t aw[4] = {av[i].x, av[i].y, av[i].z, av[i].w};
 #pragma unroll
       for (int l = 0; l < SHORT; ++l) {
         if (l < L) {
           const uint4 xv = __ldg(reinterpret_cast<const uint4*>(x + l * p.ldx + k0 + i * 1024));
           const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
 #pragma unroll
-          for (int r = 0; r < kRanks; ++r) {
-            const uint32_t aw[4] = {av[i][r].x, av[i][r].y, av[i][r].z, av[i][r].w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              acc[r][l] = fmaf(bf16_hi(aw[e]), bf16_hi(xw[e]), fmaf(bf16_lo(aw[e]), bf16_lo(xw[e]), acc[r][l]));
-          }
+          for (int e = 0; e < 4; ++e) acc[l] = fmaf(bf16_hi(aw[e]), bf16_hi(xw[e]), fmaf(bf16_lo(aw[e]), bf16_lo(xw[e]), acc[l]));
         }
       }
     }
@@ -331,25 +341,64 @@ __global__ void __launch_bounds__(128) lora_shrink_short_kernel(const ShortParam
 #pragma unroll
   for (int l = 0; l < SHORT; ++l) {
     if (l < L) {
-#pragma unroll
-      for (int r = 0; r < kRanks; ++r) {
-        const float s = warp_sum(acc[r][l]);
-        if (lane == 0) red[warp][r][l] = s;
-      }
+      const float s = warp_sum(acc[l]);
+      if (lane == 0) red[warp][l] = s;
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < kRanks * L; i += 128) {
-    const int r = i % kRanks, l = i / kRanks;
-    float v = 0.f;
-    if (j0 + r < p.low.R)  // (a rank of zeros would be NaN beside an infinite x)
-      v = (red[0][r][l] + red[1][r][l] + red[2][r][l] + red[3][r][l]) * (p.scale != nullptr ? p.scale[adapter] : 1.f);
-    const __nv_bfloat16 hi = __float2bfloat16_rn(v);
-    const float h = __bfloat162float(hi);
-    __nv_bfloat16* dst = p.t + ((int64_t)request * L + l) * p.low.ld() + p.low.column(j0 + r);
-    dst[0] = hi;
-    dst[p.low.group] = __float2bfloat16_rn(isinf(h) ? 0.f : v - h);
+  if ((int)threadIdx.x < L) {
+    const int l = threadIdx.x;
+    store_low_rank(p, adapter, request * (int64_t)L + l, j, red[0][l] + red[1][l] + red[2][l] + red[3][l]);
   }
+}
+
+// Many requests: a block per request and sixteen ranks, which reads x a sixteenth as often.  Eight warps share K; the
+// products run as mma.m16n8k16 with A's rows on the M side and the rows of x on the N side, the fragments straight from
+// global memory: a lane reads 16 consecutive bytes of two rows of A and one of x and uses them for two MMAs (the order of
+// k does not matter as long as both sides agree).  Bound by latency.
+__global__ void __launch_bounds__(256) lora_shrink_mma_kernel(const ShortParams p) {
+  __shared__ float red[8][16][SHORT + 1];
+  const int request = blockIdx.x / p.low.units, j0 = (blockIdx.x - request * p.low.units) * 16;
+  const int L = p.req.length, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_release();
+  const int adapter = p.req.of_request(request);
+  if (adapter < 0) {
+    if (j0 == 0 && threadIdx.x == 0 && p.req.raw(request) != -1) report_error(p.status, FLUXB_ERR_BAD_ARG, 81);
+    return;
+  }
+  const int g = lane >> 2, t4 = lane & 3;
+  const __nv_bfloat16* a = p.a + ((int64_t)adapter * p.low.R + j0 + g) * p.K;
+  const __nv_bfloat16* x = p.x + ((int64_t)request * L + g) * p.ldx;
+  const bool r0 = j0 + g < p.low.R, r1 = j0 + g + 8 < p.low.R, rx = g < L;
+  const uint4 none = make_uint4(0, 0, 0, 0);
+  float c[4] = {};
+  constexpr int kAhead = 4;
+  for (int k0 = warp * 32 + t4 * 8; k0 < p.K + t4 * 8; k0 += 256 * kAhead) {
+    uint4 a0[kAhead], a1[kAhead], b[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int k = k0 + i * 256;
+      a0[i] = r0 && k < p.K ? ld_nc_u4(a + k) : none;
+      a1[i] = r1 && k < p.K ? ld_nc_u4(a + (int64_t)8 * p.K + k) : none;
+      b[i] = rx && k < p.K ? ld_nc_u4(x + k) : none;
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      mma_16x8x16(c, a0[i].x, a1[i].x, a0[i].y, a1[i].y, b[i].x, b[i].y);
+      mma_16x8x16(c, a0[i].z, a1[i].z, a0[i].w, a1[i].w, b[i].z, b[i].w);
+    }
+  }
+  red[warp][g][2 * t4] = c[0];
+  red[warp][g][2 * t4 + 1] = c[1];
+  red[warp][g + 8][2 * t4] = c[2];
+  red[warp][g + 8][2 * t4 + 1] = c[3];
+  __syncthreads();
+  const int j = threadIdx.x & 15, l = threadIdx.x >> 4;
+  if (l >= L) return;
+  float v = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) v += red[w][j][l];
+  store_low_rank(p, adapter, request * (int64_t)L + l, j0 + j, v);
 }
 }  // namespace shrink
 
@@ -359,9 +408,8 @@ static int launch_shrink_short(const void* x, int64_t ldx, const void* lora_a, c
   shrink::ShortParams p{static_cast<const __nv_bfloat16*>(x), static_cast<const __nv_bfloat16*>(lora_a), scale,
                         static_cast<__nv_bfloat16*>(t), req, low, ldx, (int)K, device_status_ptr()};
   const int64_t ranks = B * low.units * 16;
-  // four ranks a block read x a quarter as often; one a block spreads few requests over the machine
-  if (ranks >= 4 * sm_count()) shrink::lora_shrink_short_kernel<4><<<(unsigned)(ranks / 4), 128, 0, st>>>(p);
-  else shrink::lora_shrink_short_kernel<1><<<(unsigned)ranks, 128, 0, st>>>(p);
+  if (ranks >= 4 * sm_count()) shrink::lora_shrink_mma_kernel<<<(unsigned)(B * low.units), 256, 0, st>>>(p);
+  else shrink::lora_shrink_one_kernel<<<(unsigned)ranks, 128, 0, st>>>(p);
   return FLUXB_OK;
 }
 
@@ -395,13 +443,6 @@ struct Params {
   DeviceStatus* status;
 };
 
-__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                            uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ float dot8(const uint4& b, const float* t, float acc) {
   const uint32_t w[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
@@ -553,8 +594,8 @@ __global__ void __launch_bounds__(THREADS, 1) lora_rows_kernel(const Params p) {
           uint4 a0 = *reinterpret_cast<const uint4*>(base + s * 64);
           uint4 a1 = *reinterpret_cast<const uint4*>(base + 8 * pitch + s * 64);
           if (!whole && piece * p.piece + col + s * 32 >= p.K) a0 = a1 = make_uint4(0, 0, 0, 0);  // behind the copy
-          mma_16x8x16(c, a0.x, a1.x, a0.y, a1.y, b[s].x, b[s].y);
-          mma_16x8x16(c, a0.z, a1.z, a0.w, a1.w, b[s].z, b[s].w);
+          shrink::mma_16x8x16(c, a0.x, a1.x, a0.y, a1.y, b[s].x, b[s].y);
+          shrink::mma_16x8x16(c, a0.z, a1.z, a0.w, a1.w, b[s].z, b[s].w);
         }
       }
       __syncwarp();
