@@ -325,3 +325,19 @@ def test_an_infinite_input_stays_infinite(tk, L):
     assert bool((y[0, 0] == float("inf")).all())
     y[0, 0] = clean[0, 0]
     assert torch.equal(y, clean)
+
+
+MANY = [  # B, L, K, N, R, adapters: tiles whose rows use many adapters, several parts of ranks, several tiles a block
+    (130, 1, 64, 136, 72, 130), (128, 1, 128, 64, 256, 128), (61, 2, 264, 328, 130, 61), (600, 2, 64, 4096, 16, 600),
+    (300, 9, 64, 2048, 8, 7), (40, 60, 192, 1544, 64, 40), (3, 700, 512, 2048, 40, 3), (1, 2100, 256, 3096, 16, 1),
+    (150, 130, 128, 24, 16, 5), (11, 129, 320, 1160, 200, 11), (3, 333, 1536, 3064, 64, 3), (9, 128, 4096, 2048, 8, 4),
+]
+
+
+@pytest.mark.parametrize("B,L,K,N,R,n", MANY)
+def test_many_adapters_and_many_tiles(tk, B, L, K, N, R, n):
+    p = problem(51 + B, B, L, K, N, R, n)
+    p["adapter"] = (torch.arange(B) % (n + 1) - 1).cuda()
+    check(call(tk, p), p)
+    p["adapter"] = torch.arange(B).clamp(max=n - 1).cuda()
+    check(call(tk, p), p)

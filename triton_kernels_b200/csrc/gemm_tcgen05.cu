@@ -1048,9 +1048,12 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
         const int n = min(chunks, total - c);
         if (elect_one()) {
           mbar_expect_tx(&full_bar[stage], n * B_BYTES);
-          for (int i = 0; i < n; ++i) {
-            const int item = (c + i) / parts, part = c + i - item * parts;
-            tma_load_3d(smem + stage * STAGE_BYTES + i * B_BYTES, &g.tm_lb, &full_bar[stage], part * 64, col0, list.id[item]);
+#pragma unroll
+          for (int i = 0; i < CHUNKS; ++i) {
+            if (i >= n) break;
+            const int item = parts == 1 ? c + i : (c + i) / parts;
+            tma_load_3d(smem + stage * STAGE_BYTES + i * B_BYTES, &g.tm_lb, &full_bar[stage], (c + i - item * parts) * 64, col0,
+                        list.id[item]);
           }
         }
         if (++stage == g.stages) { stage = 0; phase ^= 1; }
@@ -1072,6 +1075,9 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
     __syncwarp();
   } else if (warp == 1) {
     constexpr uint32_t idesc = make_idesc_bf16(BM, BN, 0, 0);
+    // of t: the first 16 ranks' high parts, how far behind a group's high parts its low parts lie, and the next group
+    const uint64_t t_desc = g.low.desc(smem_u32(t_smem));
+    const int to_low = g.low.low(0) - g.low.high(0), part_step = g.low.tile_bytes() >> 4;
     int stage = 0;
     uint32_t phase = 0, t_phase = 0;
     bool ok = true;
@@ -1116,16 +1122,27 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
         const int n = min(chunks, total - c);
         const uint64_t bdesc = make_smem_desc(smem_u32(smem + stage * STAGE_BYTES), 16, 1024);
         if (elect_one()) {
-          for (int i = 0; i < n; ++i) {
-            // (more than 64 ranks: groups of 64, one per part; up to 64 there is one group and one part)
-            const int item = (c + i) / parts, part = c + i - item * parts;
-            const uint64_t ad = g.low.desc(smem_u32(t_smem + part * g.low.tile_bytes())), bd = bdesc + i * (B_BYTES >> 4);
-            const uint4 o = list.off[item];
-            const uint32_t off[4] = {o.x, o.y, o.z, o.w};
-            const int n_units = min(4, g.low.units - part * 4);
-            for (int u = 0; u < n_units; ++u) {
-              umma_ss_masked(d_tmem, ad + g.low.high(u), bd + 2 * u, idesc, off);
-              umma_ss_masked(d_tmem, ad + g.low.low(u), bd + 2 * u, idesc, off);
+          // (more than 64 ranks: groups of 64, one per part; up to 64 there is one group and one part)
+          int part[CHUNKS];
+          uint4 o[CHUNKS];  // all asked for before the first is needed
+#pragma unroll
+          for (int i = 0; i < CHUNKS; ++i) {
+            if (i >= n) break;
+            const int item = parts == 1 ? c + i : (c + i) / parts;
+            part[i] = c + i - item * parts;
+            o[i] = list.off[item];
+          }
+#pragma unroll
+          for (int i = 0; i < CHUNKS; ++i) {
+            if (i >= n) break;
+            const uint64_t ad = t_desc + part[i] * part_step, bd = bdesc + i * (B_BYTES >> 4);
+            const uint32_t off[4] = {o[i].x, o[i].y, o[i].z, o[i].w};
+            const int n_units = g.low.units - part[i] * 4;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              if (u >= n_units) break;
+              umma_ss_masked(d_tmem, ad + 2 * u, bd + 2 * u, idesc, off);
+              umma_ss_masked(d_tmem, ad + to_low + 2 * u, bd + 2 * u, idesc, off);
             }
           }
           umma_commit(&empty_bar[stage]);
@@ -1598,9 +1615,9 @@ static int launch_lora_pairs(const fluxb_linear_problem& a, int64_t N, int64_t K
 // 128 x BN tile of one CTA takes two per operand row and step, and at least its own epilogue.  For example
 // 2048 x 3072 -> 3072: pairs 256 wide 39.1 us (two rounds of 96 tiles on 74 pairs), 192 wide 36.4; 4096 x 4096 -> 4096:
 // 95.4 and 105; 1024 x 2048 -> 2048: pairs 18.7, BN 128 15.5, 64 21.6, 32 34.4; 128 x 1024 -> 4096: 13.8, 10.4, 9.7, 9.2.
-// A ring slot of adapters takes 550, for as many adapters as a tile's rows may use.
+// The adapters that a tile's rows may use take 850 a ring slot, or, on one CTA, 80 each and 120 per sixteen ranks.
 // The low-rank rows run beside the projection's first tiles, on SMs of their own: SMs whose projection blocks have a tile
-// less to do than the others cost nothing as long as t is there when the first tile needs it (4 x 512 rows, 192 wide,
+// less to do than the others cost nothing as long as t is there at the end of the first K loop (4 x 512 rows, 192 wide,
 // 20 spare pairs: 43.3 us with 64 blocks of low-rank rows, 37.7 with 16); others wait for some 0.6 of their time (700
 // rows of three requests, K 2048, 72 tiles on 74 pairs: 20.3 us without, 25.1 with 72 blocks, 26.7 with 18).
 LoraPlan fluxb::plan_lora(int64_t M, int64_t N, int64_t K, const RequestAdapters& req, const LowRank& low) {
@@ -1615,8 +1632,9 @@ LoraPlan fluxb::plan_lora(int64_t M, int64_t N, int64_t K, const RequestAdapters
     const int64_t tiles = (M + (pair ? 255 : 127)) / (pair ? 256 : 128) * ((N + c - 1) / c);
     const int64_t steps = (pair ? 400 + 75 * c / 64 : (a_rows + c) * 2 + 100) * kb, epilogue = pair ? 7500 : 1100 + 30 * c;
     const int64_t rows = pair ? 256 : 128, requests = L % rows == 0 ? 1 : (rows + L - 2) / L + 1;
-    const int64_t slots = (pair ? fluxb::gemm2::lora_slots(low) : (low.units + 3) / 4) * (requests < req.n_adapters ? requests : req.n_adapters);
-    const int64_t tile = (steps > epilogue ? steps : epilogue) + slots * 550 + (pair ? 0 : 1000);
+    const int64_t adapters = requests < req.n_adapters ? requests : req.n_adapters;
+    const int64_t each = pair ? fluxb::gemm2::lora_slots(low) * 850 : 80 + 120 * low.units;
+    const int64_t tile = (steps > epilogue ? steps : epilogue) + adapters * each + (pair ? 0 : 1000);
     const int64_t units = pair ? sms / 2 : sms, rounds = (tiles + units - 1) / units;
     const int64_t spare = (rounds * units - tiles) * (pair ? 2 : 1);
     int64_t shrink = shrink_tiles > 0 ? INT64_MAX : 0;
@@ -1626,7 +1644,7 @@ LoraPlan fluxb::plan_lora(int64_t M, int64_t N, int64_t K, const RequestAdapters
     for (int ks = 1; shrink_tiles > 0 && ks <= (shrink_tiles < 12 ? 8 : 4); ks *= 2) {
       if (ks > 1 && (shrink_tiles * ks > sms || kb < ks * 4)) break;
       int64_t t = (9000 + (kb + ks - 1) / ks * ((shrink_rows + rpad) * 2 + 100)) * ((shrink_tiles * ks + sms - 1) / sms);
-      t = shrink_tiles * ks <= spare ? (t > tile ? t - tile : 0) : t * 3 / 5;
+      t = shrink_tiles * ks <= spare ? (t > steps ? t - steps : 0) : t * 3 / 5;
       if (t < shrink) { shrink = t; ksplit = ks; }
     }
     const int64_t all = rounds * tile + (pair ? 13000 : 7000) + shrink;
