@@ -42,9 +42,9 @@ __device__ __forceinline__ float2 split(double f) {
   return make_float2(high, static_cast<float>(f - high));
 }
 
+// Cosine and signed sine of position `id` for pair j, whose frequency is `turns`.
 template <typename Id>
-__device__ __forceinline__ float2 turn_of(const RopeAxesArgs& a, int64_t b, int64_t l, int j, float2 turns, int axis) {
-  const Id id = __ldg(static_cast<const Id*>(a.ids) + b * a.id_sb + l * a.id_sl + axis * a.id_sa);
+__device__ __forceinline__ float2 turn_of(const RopeAxesArgs& a, Id id, int j, float2 turns) {
   float r;
   const float pos = static_cast<float>(id), high = pos * turns.x;
   if (id > static_cast<Id>(-(1 << 24)) && id < static_cast<Id>(1 << 24) && fabsf(high) < 4194304.f) {
@@ -62,17 +62,20 @@ __device__ __forceinline__ float2 turn_of(const RopeAxesArgs& a, int64_t b, int6
   return make_float2(c, a.sign * s);
 }
 
-// Rows of whole 16-byte pieces.  A block takes a few tokens: its threads first take one angle each, sines and cosines go
-// through shared memory, and then every thread owns one piece of one token's rows, keeps its four pairs' sines and
-// cosines in registers and walks every `slots`-th head of q and k.  A pair's angle is so taken once, no table is read or
-// written, and the next kAhead pieces of a thread are on their way while it works on the current ones.  Bound by HBM:
-// every element is read once and written once; 24 + 24 heads of 4608 tokens, 128 columns bf16: 21.6 us, 5.2 TB/s.  (With
-// the angles per thread instead, taken again for every group of heads: 37 us.)
-template <typename T, typename Id>
+// Rows of whole 16-byte pieces.  A block takes a few tokens; a thread owns one piece of one token's rows, keeps its four
+// pairs' sines and cosines in registers and walks every `slots`-th head of q and k.  A pair's angle is so taken once, no
+// table is read or written, and the next kAhead pieces of a thread are on their way while it works on the current ones.
+// Bound by HBM: every element is read once and written once; 24 + 24 heads of 4608 tokens, 128 columns bf16: 21.6 us, 5.2
+// TB/s.  (With the angles taken again for every group of heads: 37 us.)
+// kShare: where several threads walk the same piece's heads (slots > 1), the block's threads first take one angle each and
+// pass them on through shared memory; where a piece has one thread it takes its own.  With 512 tokens of 8 + 8 heads sharing
+// takes 5.1 us and not sharing 6.2; with one thread a piece the barriers cost: 16 x 4096 tokens of 1 + 1 heads, 64 columns,
+// 23.2 us sharing, 16.9 not; 16 + 4 heads of 16896 tokens fp32 31.4 and 30.4.
+template <typename T, typename Id, bool kShare>
 __global__ void __launch_bounds__(256, 4) rope_axes_vec_kernel(const __grid_constant__ RopeAxesArgs a) {
   constexpr int VN = Vec<T>::N;
   constexpr int kAhead = 3;
-  extern __shared__ float2 table[];  // [tokens][D / 2]
+  extern __shared__ float2 table[];  // [tokens][D / 2] (kShare)
   __shared__ float2 turns[kMaxPairs];
   __shared__ uint8_t axis[kMaxPairs];
   // (the kernel's parameters can be read at one address per warp and cycle only: with lanes that
@@ -106,20 +109,32 @@ __global__ void __launch_bounds__(256, 4) rope_axes_vec_kernel(const __grid_cons
   };
   if (nq > 0) load(sq, qs, nq);
   else load(sk, ks, nk);
-#pragma unroll 4
-  for (int i = threadIdx.x; i < a.tokens * half; i += 256) {
-    const int ti = i / half, j = i - ti * half;
-    if (tok0 + ti < tokens && j < a.pairs) {
-      const int bi = (tok0 + ti) / (int)a.L;
-      table[i] = turn_of<Id>(a, bi, tok0 + ti - bi * (int)a.L, j, turns[j], axis[j]);
-    }
-  }
-  __syncthreads();
   const int rotated = min(VN / 2, a.pairs - piece * (VN / 2));  // pairs of this piece: all, some, or none (0 or less)
+  const Id* const ids = static_cast<const Id*>(a.ids);
   float2 cs[VN / 2];
+  if constexpr (kShare) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < a.tokens * half; i += 256) {
+      const int ti = i / half, j = i - ti * half;
+      if (tok0 + ti < tokens && j < a.pairs) {
+        const int bi = (tok0 + ti) / (int)a.L;
+        const Id id = __ldg(ids + bi * a.id_sb + (tok0 + ti - bi * (int)a.L) * a.id_sl + axis[j] * a.id_sa);
+        table[i] = turn_of<Id>(a, id, j, turns[j]);
+      }
+    }
+    __syncthreads();
 #pragma unroll
-  for (int p = 0; p < VN / 2; ++p)
-    if (active && p < rotated) cs[p] = table[t * half + piece * (VN / 2) + p];
+    for (int p = 0; p < VN / 2; ++p)
+      if (active && p < rotated) cs[p] = table[t * half + piece * (VN / 2) + p];
+  } else {
+    Id id[VN / 2];
+#pragma unroll
+    for (int p = 0; p < VN / 2; ++p)
+      if (active && p < rotated) id[p] = __ldg(ids + b * a.id_sb + l * a.id_sl + axis[piece * (VN / 2) + p] * a.id_sa);
+#pragma unroll
+    for (int p = 0; p < VN / 2; ++p)
+      if (active && p < rotated) cs[p] = turn_of<Id>(a, id[p], piece * (VN / 2) + p, turns[piece * (VN / 2) + p]);
+  }
   auto finish = [&](T* p, int64_t step, const uint4 (&now)[kAhead], int n) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u, p += step) {
@@ -171,7 +186,7 @@ __global__ void __launch_bounds__(256, 4) rope_axes_vec_kernel(const __grid_cons
     dk += kAhead * ko;
     nk -= kAhead;
   }
-  __syncthreads();  // the table is free
+  if constexpr (kShare) __syncthreads();  // the table is free
   }
 }
 
@@ -184,7 +199,7 @@ __global__ void __launch_bounds__(256) rope_axes_any_kernel(const __grid_constan
   const int j = (int)(i % half);
   const int64_t tok = i / half, b = tok / a.L, l = tok % a.L;
   const bool rot = j < a.pairs;
-  const float2 cs = rot ? turn_of<Id>(a, b, l, j, split(a.turns[j]), a.axis[j]) : make_float2(1.f, 0.f);
+  const float2 cs = rot ? turn_of<Id>(a, __ldg(static_cast<const Id*>(a.ids) + b * a.id_sb + l * a.id_sl + a.axis[j] * a.id_sa), j, split(a.turns[j])) : make_float2(1.f, 0.f);
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
     const RopeTensor& t = a.t[w];
@@ -273,15 +288,22 @@ extern "C" int fluxb_rope_axes(const void* q, int64_t q_sb, int64_t q_sh, int64_
     a.tokens = (int)(256 / (pieces * slots));
     const int64_t most = 4 * sm_count(), blocks = (B * L + a.tokens - 1) / a.tokens;
     const unsigned vgrid = (unsigned)(blocks < most ? blocks : most);
-    const size_t smem = (size_t)a.tokens * (D / 2) * sizeof(float2);
-#define FLUXB_ROPE_AXES(T)                                                                    \
-  do {                                                                                        \
-    if (id_type == FLUXB_ID_F32) rope_axes_vec_kernel<T, float><<<vgrid, 256, smem, st>>>(a);    \
-    else if (id_type == FLUXB_ID_I32) rope_axes_vec_kernel<T, int><<<vgrid, 256, smem, st>>>(a); \
-    else rope_axes_vec_kernel<T, long long><<<vgrid, 256, smem, st>>>(a);                        \
+    const bool share = slots > 1;
+    const size_t smem = share ? (size_t)a.tokens * (D / 2) * sizeof(float2) : 0;
+#define FLUXB_ROPE_AXES(T, Id)                                                             \
+  do {                                                                                     \
+    if (share) rope_axes_vec_kernel<T, Id, true><<<vgrid, 256, smem, st>>>(a);             \
+    else rope_axes_vec_kernel<T, Id, false><<<vgrid, 256, 0, st>>>(a);                     \
   } while (0)
-    if (dtype == FLUXB_BF16) FLUXB_ROPE_AXES(__nv_bfloat16);
-    else FLUXB_ROPE_AXES(float);
+    if (dtype == FLUXB_BF16) {
+      if (id_type == FLUXB_ID_F32) FLUXB_ROPE_AXES(__nv_bfloat16, float);
+      else if (id_type == FLUXB_ID_I32) FLUXB_ROPE_AXES(__nv_bfloat16, int);
+      else FLUXB_ROPE_AXES(__nv_bfloat16, long long);
+    } else {
+      if (id_type == FLUXB_ID_F32) FLUXB_ROPE_AXES(float, float);
+      else if (id_type == FLUXB_ID_I32) FLUXB_ROPE_AXES(float, int);
+      else FLUXB_ROPE_AXES(float, long long);
+    }
 #undef FLUXB_ROPE_AXES
     cudaError_t ve = cudaGetLastError();
     if (ve != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "rope_axes: %s", cudaGetErrorString(ve));
