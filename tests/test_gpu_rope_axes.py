@@ -227,3 +227,27 @@ def test_a_theta_below_one_turns_faster(tk):
     limit = (16 * U + 6 * 2.0**-53 * angle) * pair
     limit = limit + U * (want.abs() + limit)
     assert bool(((got.double() - want).abs() <= limit).all())
+
+
+LONG = [  # B, H, G, L, D, axes: so many tokens that each piece of a row has one thread for all heads
+    (3, 1, 2, 2000, 128, (16, 56, 56)), (2, 5, 1, 2501, 128, (10, 14, 22)), (6000, 1, 1, 1, 128, (64, 64)),
+    (1, 4, 0, 5003, 256, (128, 126)), (7, 2, 3, 1400, 64, (64,)),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,H,G,L,D,axes", LONG)
+def test_many_tokens(tk, B, H, G, L, D, axes, dtype):
+    q, k = make(81, (B, H, L, D), dtype), make(82, (B, G, L, D), dtype)
+    for ids in (positions(83, B, L, len(axes)), positions(84, 1, L, len(axes), 2**24).int(),
+                positions(85, B, L, len(axes)).float() + 0.25, positions(86, B, L, len(axes)) + 2**33):
+        oq, ok = tk.apply_rope_axes(q, k, ids, axes)
+        slack = 2**33 * 6 * 2.0**-53 if ids.dtype == torch.int64 and int(ids.max()) > 2**32 else 0.0
+        for got, x in ((oq, q), (ok, k)):
+            if slack == 0.0:
+                check(got, x, ids, axes, 10000.0)
+            elif x.numel():  # fp64 angles of 2^33: three roundings on either side, next to the 16 u
+                want = rotation(x, ids, axes, 10000.0)
+                limit = (16 * U + slack) * x.double().abs().amax() * 2**0.5
+                limit = limit + torch.finfo(dtype).eps / 2 * (want.abs() + limit)
+                assert bool(((got.double() - want).abs() <= limit).all())
