@@ -212,6 +212,8 @@ def test_refusals_on_the_device(tk):
         tk.apply_rope_axes(q, q, ids[:, :3], (32, 32))
     with pytest.raises(AssertionError):
         tk.apply_rope_axes(q, q[:, :, :3], ids, (32, 32))
+    with pytest.raises(NotImplementedError, match="no gradient"):
+        tk.apply_rope_axes(q, q, ids.float().requires_grad_(True), (32, 32))
 
 
 def test_a_theta_below_one_turns_faster(tk):

@@ -298,6 +298,7 @@ std::pair<Tensor, Tensor> apply_rope_axes(const Tensor& q, const Tensor& k, cons
           "ids must be [B or 1, L, number of axes]");
   id_code(ids);
   dtype_code(q);
+  if (wants_grad({&ids})) fail(PyExc_NotImplementedError, "position ids get no gradient: detach them");
   if (wants_grad({&q, &k})) {
     variable_list out = RopeAxes::apply(q, k, ids, std::move(axes), theta);
     return {out[0], out[1]};

@@ -40,5 +40,5 @@ def apply_rope_axes(xq: torch.Tensor, xk: torch.Tensor, ids: torch.Tensor, axes_
     [1, L, n_axes], float32 (fractions allowed), int32 or int64.  axes_dim: the even number of
     columns of each axis, in order; their sum may be less than D, and the columns behind them are
     copied.  Pair j of an axis of d columns turns by ids * theta^(-2j/d), taken in fp64.
-    Differentiable once in xq and xk."""
+    Differentiable once in xq and xk; ids that require a gradient are refused."""
     return _lib.binding().apply_rope_axes(xq, xk, ids, axes_dim, theta)
