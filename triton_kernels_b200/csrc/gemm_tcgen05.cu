@@ -663,6 +663,7 @@ gemm_pair_kernel(const __grid_constant__ G g) {
   cluster_sync_all();  // partner's barriers exist before anything signals them
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
+  if constexpr (kMode == 3) pdl_release();
 
   if (kMode == 3 && warp == 0) {
     if constexpr (kMode == 3) {
@@ -1019,6 +1020,7 @@ __global__ void __launch_bounds__(THREADS, 1) lora_tile_kernel(const __grid_cons
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = tmem_slot;
+  pdl_release();
 
   if (warp == 0) {
     int stage = 0;

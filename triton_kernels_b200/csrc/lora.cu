@@ -3,7 +3,10 @@
 // x holds L rows per request.  Two launches: the low-rank rows t = s_a (x A_a^T) here, then the projection with
 // the adapters' second half fused in (gemm_tcgen05.cu).  t is carried as two bf16 parts, high and low
 // (t = high + low to 2^-17 of |t|), so that the tensor cores take it without the rounding a single bf16 would put
-// between the two products.  An adapter index outside [-1, n) leaves its request without an adapter and is recorded
+// between the two products.  Both kernels may start while the one in front of them ends: the first waits for everything
+// before it (in every block, before anything is read), only then does it let the second start, and that one waits for
+// t.  In a stream of such calls that took 16.4 us to 13.2 (48 x 5 rows, 1024 -> 4096, 16 adapters) and 26.0 to 24.2 (8 x 1
+// row, 3072 -> 18432).  An adapter index outside [-1, n) leaves its request without an adapter and is recorded
 // in the device status word (site 81).
 #include "lora.cuh"
 #include "vec.cuh"
@@ -49,11 +52,15 @@ __global__ void __launch_bounds__(THREADS, 1) lora_shrink_kernel(const __grid_co
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int in_cluster = (int)cluster_ctarank(), rank = p.ksplit > 1 ? in_cluster : 0;
   const int tile = blockIdx.x / p.ksplit;
-  if (tile >= p.tiles) return;
+  if (tile >= p.tiles) {
+    pdl_wait();  // (a block that leaves lets the projection start, too)
+    return;
+  }
   const int request = tile / p.tiles_per_request;
   const int l0 = (tile - request * p.tiles_per_request) * BM;
   const int row0 = request * p.L + l0;
   const int rows = min(BM, p.L - l0);
+  pdl_wait();
   const int adapter = p.req.of_request(request);
   if (adapter < 0) {  // the whole cluster leaves; nobody reads these rows of t
     if (threadIdx.x == 0 && rank == 0 && l0 == 0 && p.req.raw(request) != -1) report_error(p.status, FLUXB_ERR_BAD_ARG, 81);
@@ -255,12 +262,14 @@ static int launch_shrink(const void* x, int64_t ldx, const void* lora_a, const f
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = cluster;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   e = cudaLaunchKernelEx(&cfg, lora_shrink_kernel, p);
   if (e != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "linear_lora: launch failed: %s", cudaGetErrorString(e));
   return FLUXB_OK;
@@ -308,6 +317,7 @@ __global__ void __launch_bounds__(128) lora_shrink_one_kernel(const ShortParams 
   const int ranks = p.low.units * 16;  // the ranks behind R are zeros: the tensor cores multiply them, too
   const int request = blockIdx.x / ranks, j = blockIdx.x - request * ranks;
   const int L = p.req.length, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_wait();
   pdl_release();  // (its stream of W does not get in front: the loads here are all on their way within the launch)
   const int adapter = p.req.of_request(request);
   if (adapter < 0) {
@@ -360,6 +370,7 @@ __global__ void __launch_bounds__(256) lora_shrink_mma_kernel(const ShortParams 
   __shared__ float red[8][16][SHORT + 1];
   const int request = blockIdx.x / p.low.units, j0 = (blockIdx.x - request * p.low.units) * 16;
   const int L = p.req.length, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_wait();
   pdl_release();
   const int adapter = p.req.of_request(request);
   if (adapter < 0) {
@@ -408,8 +419,9 @@ static int launch_shrink_short(const void* x, int64_t ldx, const void* lora_a, c
   shrink::ShortParams p{static_cast<const __nv_bfloat16*>(x), static_cast<const __nv_bfloat16*>(lora_a), scale,
                         static_cast<__nv_bfloat16*>(t), req, low, ldx, (int)K, device_status_ptr()};
   const int64_t ranks = B * low.units * 16;
-  if (ranks >= 4 * sm_count()) shrink::lora_shrink_mma_kernel<<<(unsigned)(B * low.units), 256, 0, st>>>(p);
-  else shrink::lora_shrink_one_kernel<<<(unsigned)ranks, 128, 0, st>>>(p);
+  const cudaError_t e = ranks >= 4 * sm_count() ? launch_after(shrink::lora_shrink_mma_kernel, (unsigned)(B * low.units), 256, 0, st, p)
+                                                : launch_after(shrink::lora_shrink_one_kernel, (unsigned)ranks, 128, 0, st, p);
+  if (e != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "linear_lora: launch failed: %s", cudaGetErrorString(e));
   return FLUXB_OK;
 }
 
@@ -476,6 +488,7 @@ __global__ void __launch_bounds__(THREADS, 1) lora_rows_kernel(const Params p) {
     fence_proxy_async_smem();
   }
   __syncthreads();
+  pdl_release();
   int slot = 0;
   uint32_t phase = 0;
   if (warp == WARPS) {

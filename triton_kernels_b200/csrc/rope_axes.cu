@@ -85,6 +85,8 @@ __global__ void __launch_bounds__(256, 4) rope_axes_vec_kernel(const __grid_cons
     axis[threadIdx.x] = a.axis[threadIdx.x];
   }
   __syncthreads();
+  pdl_wait();  // the block may have started while the kernel in front was ending
+  pdl_release();
   const int pieces = a.D / VN, half = a.D / 2;
   const int tokens = (int)(a.B * a.L);
   const int piece = threadIdx.x % pieces, rest = threadIdx.x / pieces;
@@ -289,11 +291,12 @@ extern "C" int fluxb_rope_axes(const void* q, int64_t q_sb, int64_t q_sh, int64_
     const int64_t most = 4 * sm_count(), blocks = (B * L + a.tokens - 1) / a.tokens;
     const unsigned vgrid = (unsigned)(blocks < most ? blocks : most);
     const bool share = slots > 1;
+    cudaError_t ve;
     const size_t smem = share ? (size_t)a.tokens * (D / 2) * sizeof(float2) : 0;
 #define FLUXB_ROPE_AXES(T, Id)                                                             \
   do {                                                                                     \
-    if (share) rope_axes_vec_kernel<T, Id, true><<<vgrid, 256, smem, st>>>(a);             \
-    else rope_axes_vec_kernel<T, Id, false><<<vgrid, 256, 0, st>>>(a);                     \
+    ve = share ? launch_after(rope_axes_vec_kernel<T, Id, true>, vgrid, 256, smem, st, a)  \
+               : launch_after(rope_axes_vec_kernel<T, Id, false>, vgrid, 256, 0, st, a);   \
   } while (0)
     if (dtype == FLUXB_BF16) {
       if (id_type == FLUXB_ID_F32) FLUXB_ROPE_AXES(__nv_bfloat16, float);
@@ -305,7 +308,6 @@ extern "C" int fluxb_rope_axes(const void* q, int64_t q_sb, int64_t q_sh, int64_
       else FLUXB_ROPE_AXES(float, long long);
     }
 #undef FLUXB_ROPE_AXES
-    cudaError_t ve = cudaGetLastError();
     if (ve != cudaSuccess) return set_error(FLUXB_ERR_CUDA, "rope_axes: %s", cudaGetErrorString(ve));
     return FLUXB_OK;
   }
