@@ -313,13 +313,15 @@ __global__ void __launch_bounds__(256) ln_fwd_block_kernel(const LnArgs a) {
   const T* fp = static_cast<const T*>(a.factor) + vec;
   const T* op = static_cast<const T*>(a.offset) + vec;
   uint4 raw[kV], fr[kV], orw[kV];
+  pdl_wait();  // (the block may have started while the kernel in front was ending)
+  pdl_release();
 #pragma unroll
   for (int i = 0; i < kV; ++i) {
     const int c = (i * 256 + threadIdx.x) * VN;
     if (c < a.cols) {
-      raw[i] = ld_nc_u4(x + c);
-      fr[i] = ld_nc_u4(fp + c);
-      orw[i] = ld_nc_u4(op + c);
+      raw[i] = ld_u4(x + c);
+      fr[i] = ld_u4(fp + c);
+      orw[i] = ld_u4(op + c);
     }
   }
   float s = 0.f;
@@ -842,11 +844,11 @@ extern "C" int fluxb_layer_norm(const void* x, const void* factor, const void* o
                      vec_stride % vn == 0 && all16(x, y, factor, offset);
   if (whole && rows <= 2 * sm_count() && cols <= 1024 * vn) {
     const int v = (int)((cols / vn + 255) / 256);
-#define FLUXB_LN_BLOCK(T)                                                                    \
-  do {                                                                                       \
-    if (v == 1) ln_fwd_block_kernel<T, 1><<<(unsigned)rows, 256, 0, st>>>(a);                \
-    else if (v == 2) ln_fwd_block_kernel<T, 2><<<(unsigned)rows, 256, 0, st>>>(a);           \
-    else ln_fwd_block_kernel<T, 4><<<(unsigned)rows, 256, 0, st>>>(a);                       \
+#define FLUXB_LN_BLOCK(T)                                                                        \
+  do {                                                                                           \
+    if (v == 1) launch_after(ln_fwd_block_kernel<T, 1>, (unsigned)rows, 256, 0, st, a);          \
+    else if (v == 2) launch_after(ln_fwd_block_kernel<T, 2>, (unsigned)rows, 256, 0, st, a);     \
+    else launch_after(ln_fwd_block_kernel<T, 4>, (unsigned)rows, 256, 0, st, a);                 \
   } while (0)
     if (dtype == FLUXB_BF16) FLUXB_LN_BLOCK(__nv_bfloat16);
     else FLUXB_LN_BLOCK(float);

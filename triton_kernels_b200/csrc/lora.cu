@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(128) lora_shrink_one_kernel(const ShortParams 
     uint4 av[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
-      av[i] = k0 + i * 1024 < p.K && j < p.low.R ? __ldg(reinterpret_cast<const uint4*>(a + k0 + i * 1024)) : make_uint4(0, 0, 0, 0);
+      av[i] = k0 + i * 1024 < p.K && j < p.low.R ? ld_u4(a + k0 + i * 1024) : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       if (k0 + i * 1024 >= p.K) break;
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(128) lora_shrink_one_kernel(const ShortParams 
 #pragma unroll
       for (int l = 0; l < SHORT; ++l) {
         if (l < L) {
-          const uint4 xv = __ldg(reinterpret_cast<const uint4*>(x + l * p.ldx + k0 + i * 1024));
+          const uint4 xv = ld_u4(x + l * p.ldx + k0 + i * 1024);
           const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[l] = fmaf(bf16_hi(aw[e]), bf16_hi(xw[e]), fmaf(bf16_lo(aw[e]), bf16_lo(xw[e]), acc[l]));
@@ -389,9 +389,9 @@ __global__ void __launch_bounds__(256) lora_shrink_mma_kernel(const ShortParams 
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int k = k0 + i * 256;
-      a0[i] = r0 && k < p.K ? ld_nc_u4(a + k) : none;
-      a1[i] = r1 && k < p.K ? ld_nc_u4(a + (int64_t)8 * p.K + k) : none;
-      b[i] = rx && k < p.K ? ld_nc_u4(x + k) : none;
+      a0[i] = r0 && k < p.K ? ld_u4(a + k) : none;
+      a1[i] = r1 && k < p.K ? ld_u4(a + (int64_t)8 * p.K + k) : none;
+      b[i] = rx && k < p.K ? ld_u4(x + k) : none;
     }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {

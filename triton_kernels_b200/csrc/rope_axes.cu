@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(256, 4) rope_axes_vec_kernel(const __grid_cons
   auto load = [&](const T* p, int64_t step, int n) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u, p += step)
-      if (u < n) next[u] = ld_nc_u4(p);
+      if (u < n) next[u] = ld_u4(p);
   };
   if (nq > 0) load(sq, qs, nq);
   else load(sk, ks, nk);
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(256, 4) rope_axes_vec_kernel(const __grid_cons
       const int ti = i / half, j = i - ti * half;
       if (tok0 + ti < tokens && j < a.pairs) {
         const int bi = (tok0 + ti) / (int)a.L;
-        const Id id = __ldg(ids + bi * a.id_sb + (tok0 + ti - bi * (int)a.L) * a.id_sl + axis[j] * a.id_sa);
+        const Id id = ids[bi * a.id_sb + (tok0 + ti - bi * (int)a.L) * a.id_sl + axis[j] * a.id_sa];
         table[i] = turn_of<Id>(a, id, j, turns[j]);
       }
     }
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(256, 4) rope_axes_vec_kernel(const __grid_cons
     Id id[VN / 2];
 #pragma unroll
     for (int p = 0; p < VN / 2; ++p)
-      if (active && p < rotated) id[p] = __ldg(ids + b * a.id_sb + l * a.id_sl + axis[piece * (VN / 2) + p] * a.id_sa);
+      if (active && p < rotated) id[p] = ids[b * a.id_sb + l * a.id_sl + axis[piece * (VN / 2) + p] * a.id_sa];
 #pragma unroll
     for (int p = 0; p < VN / 2; ++p)
       if (active && p < rotated) cs[p] = turn_of<Id>(a, id[p], piece * (VN / 2) + p, turns[piece * (VN / 2) + p]);
