@@ -57,8 +57,13 @@ __device__ __forceinline__ void forget(uint4& t) {
 
 __device__ __forceinline__ uint4 ld_nc_u4(const void* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 // The same for kernels that may start before the one in front has ended: what they read is not constant for their whole
-// life, and a load by the read-only path might be moved in front of the wait.
-__device__ __forceinline__ uint4 ld_u4(const void* p) { return *reinterpret_cast<const uint4*>(p); }
+// life, and a load by the read-only path might be moved in front of the wait.  (As a volatile instruction it stays behind
+// the wait, but may pass the stores of other elements, which a plain load may not.)
+__device__ __forceinline__ uint4 ld_u4(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
 
 // One row from global into shared memory by an asynchronous bulk copy (16-byte multiples and alignment).
 __device__ __forceinline__ void bulk_load_row(void* smem_dst, const void* gsrc, uint32_t bytes, uint64_t* bar) {
