@@ -937,8 +937,8 @@ gemm_pair_kernel(const __grid_constant__ G g) {
 // over the machine instead of filling a handful of CTA pairs.  Same roles and ring as the kernels above, and a warp that
 // lists the adapters of a tile's rows; the tile's low-rank rows t stay in shared memory while the adapters pass through the
 // ring, up to four pieces of 64 ranks of B a slot.  With K small and many adapters it is bound by their MMAs, which read t
-// from shared memory for every adapter (some 55 cycles each at 64 columns): 48 requests of 5 rows, 1024 -> 4096, 16
-// adapters of rank 64 take 15.9 us with the low-rank rows, one adapter of them 10.3.
+// from shared memory for every adapter (some 55 cycles each at 64 columns): 48 requests of 5 rows, 1024 -> 4096,
+// rank 64: 14.2 us with the low-rank rows, 4.5 of them for 15 of the 16 adapters.
 // ----------------------------------------------------------------------------------------
 namespace gemm3 {
 using gemm::BK;

@@ -433,7 +433,7 @@ static int launch_shrink_short(const void* x, int64_t ldx, const void* lora_a, c
 // its A fragments of two MMAs, with x's fragment taken from the same k positions: the order of k does not matter as
 // long as both sides agree.  x's fragments stay in registers for all tiles (kPieces pieces of W; 0: read each time).
 // The adapters are R more products per output, from t's two parts widened to fp32.
-// Bound by HBM: 18432 x 3072, eight rows, 24.1 us with the low-rank rows (113 MB of W; 4.7 TB/s).  (With W loaded
+// Bound by HBM: 18432 x 3072, eight rows, 23.4 us with the low-rank rows (113 MB of W; 4.8 TB/s).  (With W loaded
 // straight to registers, 98 KB in flight per SM: 27 us; with 2 KB copies: 25 us.)
 // ----------------------------------------------------------------------------------------
 namespace rows {

@@ -65,7 +65,7 @@ __device__ __forceinline__ float2 turn_of(const RopeAxesArgs& a, Id id, int j, f
 // Rows of whole 16-byte pieces.  A block takes a few tokens; a thread owns one piece of one token's rows, keeps its four
 // pairs' sines and cosines in registers and walks every `slots`-th head of q and k.  A pair's angle is so taken once, no
 // table is read or written, and the next kAhead pieces of a thread are on their way while it works on the current ones.
-// Bound by HBM: every element is read once and written once; 24 + 24 heads of 4608 tokens, 128 columns bf16: 21.6 us, 5.2
+// Bound by HBM: every element is read once and written once; 24 + 24 heads of 4608 tokens, 128 columns bf16: 21.0 us, 5.4
 // TB/s.  (With the angles taken again for every group of heads: 37 us.)
 // kShare: where several threads walk the same piece's heads (slots > 1), the block's threads first take one angle each and
 // pass them on through shared memory; where a piece has one thread it takes its own.  With 512 tokens of 8 + 8 heads sharing
