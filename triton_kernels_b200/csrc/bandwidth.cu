@@ -5,7 +5,7 @@
 //
 // Common shape of every kernel: 16-byte vector loads/stores, a row (or row segment) held in
 // registers or, for rows of 2-24 KB, staged in shared memory by a bulk copy; fp32 statistics
-// (one pass over staged rows, mean then centred variance over register-held rows), reductions
+// (one pass over staged rows where nothing cancels, mean then centred variance otherwise), reductions
 // by warp shuffles only.  Algorithmic traffic is "every input once, every output once"; nothing
 // is staged through global scratch.  The 57-113 MB problems of the block are short enough
 // (10-20 us) that issue slots, shared-memory traffic and the order in which requests are made
@@ -55,6 +55,8 @@ enum Norm {
 };
 template <int kNorm>
 __device__ __forceinline__ float scale_of(float a) { return kNorm == kAffine ? a : 1.0f + a; }
+template <int kNorm>
+__device__ __forceinline__ float2 scale_of(float2 a) { return kNorm == kAffine ? a : __fadd2_rn(a, make_float2(1.f, 1.f)); }
 
 // ----------------------------------------------------------------------------------------
 // LayerNorm (no affine) + modulation.  G lanes own one row; each lane holds VPL vectors.
@@ -177,15 +179,19 @@ ln_mod_generic_kernel(const T* __restrict__ x, const T* __restrict__ scale,
 //
 // Once a row has landed the warp's cost is shared-memory traffic (32 rows per SM land within a
 // few microseconds of each other and share one 128 B/clock pipe), so the kernel touches the row
-// as few times as it can: ONE pass for the statistics, one pass that reads the row again, applies
+// as few times as it can: ONE pass for the statistics of most rows, one pass that reads the row again, applies
 // the modulation and writes the result over it, and a bulk copy out.  With kStagedMod the
 // per-column vectors (scale and shift, or the RMSNorm weight) are fetched once per block into
 // shared memory instead of once per row through L1 (12 KB per 6 KB row otherwise).
 //
-// The LayerNorm statistics are the shifted one-pass form: with p = the row's first element,
-// mean = p + E[x - p] and var = E[(x - p)^2] - E[x - p]^2, accumulated in fp32.  Shifting by an
-// element of the row keeps the subtraction benign when |mean| >> std (the plain
-// E[x^2] - mean^2 form is not).
+// The LayerNorm statistics: one pass takes E[x] and E[x^2] in fp32, and var = E[x^2] - E[x]^2 is kept where the
+// subtraction costs two bits at most (E[x]^2 <= 3 (var + eps)), as for rows whose mean is within 1.7 deviations of zero,
+// whatever single columns hold.  Any other row - far from zero, or of almost one value, where the difference is rounding
+// noise - is read again from shared memory, centred: with d = x - mean, mean += E[d] and var = E[d^2] - E[d]^2.  (A
+// shift by one element of the row instead of the second pass depends on that element: a first column of 100 deviations
+// put fp32 rows of 3072 off by 3e-4.  4096 x 3072 bf16: 11.5 us where no row
+// takes the second pass, 13.7 where all do; centring every row from the start 13.2, a shift by the mean of the row's first
+// 32 pieces 12.2.)  Sums and the modulation work on pairs of columns, one instruction for two.
 // ----------------------------------------------------------------------------------------
 // Waits (bounded) for a staged copy.  If the copy never lands the row stays unwritten, so the
 // give-up is recorded in the device status word like every other bounded wait (site 71).
@@ -246,31 +252,39 @@ norm_rows_bulk_kernel(const T* __restrict__ x, const T* __restrict__ scale, cons
   const int nvec = kVPL > 0 ? kVPL * 32 : cols / VN;
   float mean = 0.f, rstd;
   if (kLayerNorm) {
-    // The modulated form does not shift 16-bit rows: their own quantisation (2^-9 of |x|) is 64 times
-    // the fp32 cancellation error of the unshifted form at any mean/std ratio of rows that vary from
-    // element to element.  The affine form shifts every type.
-    constexpr bool kShift = sizeof(T) > 2 || kNorm == kAffine;
-    float pivot = 0.f;
-    if (kShift) {
-      Vec<T> first;
-      first.load(srow);
-      pivot = first.v[0];
-    }
-    float s = 0.f, q = 0.f;
+    float2 s2 = make_float2(0.f, 0.f), q2 = s2;
 #pragma unroll(kVPL > 0 ? kVPL : 1)
     for (int i = lane; i < nvec; i += 32) {
       Vec<T> t;
       t.load(srow + i * VN);
 #pragma unroll
-      for (int j = 0; j < VN; ++j) {
-        const float d = kShift ? t.v[j] - pivot : t.v[j];
-        s += d;
-        q = fmaf(d, d, q);
+      for (int j = 0; j < VN; j += 2) {
+        const float2 d = make_float2(t.v[j], t.v[j + 1]);
+        s2 = __fadd2_rn(s2, d);
+        q2 = __ffma2_rn(d, d, q2);
       }
     }
-    const float ds = warp_sum(s) / cols;
-    mean = pivot + ds;
-    rstd = rsqrtf(fmaxf(warp_sum(q) / cols - ds * ds, 0.f) + eps);
+    float ds = warp_sum(s2.x + s2.y) / cols;
+    mean = ds;
+    float var = warp_sum(q2.x + q2.y) / cols - ds * ds;
+    if (!(ds * ds <= 3.f * (var + eps))) {  // (NaN comes here, too, and stays NaN)
+      float s = 0.f, q = 0.f;
+#pragma unroll 1
+      for (int i = lane; i < nvec; i += 32) {
+        Vec<T> t;
+        t.load(srow + i * VN);
+#pragma unroll
+        for (int j = 0; j < VN; ++j) {
+          const float d = t.v[j] - mean;
+          s += d;
+          q = fmaf(d, d, q);
+        }
+      }
+      ds = warp_sum(s) / cols;
+      mean += ds;
+      var = warp_sum(q) / cols - ds * ds;
+    }
+    rstd = rsqrtf((var < 0.f ? 0.f : var) + eps);
     if (mean_out != nullptr && lane == 0) { mean_out[row] = mean; rstd_out[row] = rstd; }
   } else {
     float q = 0.f;
@@ -308,7 +322,12 @@ norm_rows_bulk_kernel(const T* __restrict__ x, const T* __restrict__ scale, cons
         d.load_nc(sh + i * VN);
       }
 #pragma unroll
-      for (int j = 0; j < VN; ++j) t.v[j] = fmaf(fmaf(t.v[j], rstd, neg_mean_rstd), scale_of<kNorm>(a.v[j]), d.v[j]);
+      for (int j = 0; j < VN; j += 2) {
+        const float2 h = __ffma2_rn(make_float2(t.v[j], t.v[j + 1]), make_float2(rstd, rstd), make_float2(neg_mean_rstd, neg_mean_rstd));
+        const float2 o = __ffma2_rn(h, scale_of<kNorm>(make_float2(a.v[j], a.v[j + 1])), make_float2(d.v[j], d.v[j + 1]));
+        t.v[j] = o.x;
+        t.v[j + 1] = o.y;
+      }
       t.store(srow + i * VN);
     }
   } else {

@@ -28,9 +28,9 @@ def layer_norm_modulation_into(x2d, scale2d, shift2d, y2d, rows_per_batch: int, 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
                eps: float = 1e-5) -> torch.Tensor:
     """LayerNorm over the last dim with a learned scale and offset ([C] each, or None), for fp32 or
-    bf16 tensors of any width; weight and bias have x's dtype.  Statistics are fp32 (rows of 2-24 KB:
-    sum and sum of squares in one pass, shifted by the row's first element; others: mean, then
-    centred variance).  Differentiable once in x, weight and bias; the scale's and the offset's
+    bf16 tensors of any width; weight and bias have x's dtype.  Statistics are fp32 (more than
+    two rows per SM, of 2-24 KB: sum and sum of squares in one pass, and a centred second one for rows
+    where their difference would cancel; others: mean, then centred variance).  Differentiable once in x, weight and bias; the scale's and the offset's
     gradients are summed in fp32 in a fixed order.  (No counterpart in the reference, whose only
     LayerNorm is the modulated one.)"""
     return _lib.binding().layer_norm(x, weight, bias, eps)
@@ -40,7 +40,8 @@ def layer_norm_modulation(x: torch.Tensor, weight: torch.Tensor, bias: torch.Ten
     """LayerNorm(x) without affine, then `* (1 + weight) + bias` with weight/bias of shape
     [B, 1, C] broadcast over the sequence (reference :47-77; its default eps 1e-5 is kept).
     Statistics are fp32 whatever the storage dtype (rows of 2-24 KB: sum and sum of squares in
-    one pass, fp32 rows shifted by their first element; other widths: mean, then centred variance).
+    one pass, and a centred second one for rows where their difference would cancel; other widths:
+    mean, then centred variance).
     Differentiable once in x, weight and bias (the reference's is forward only)."""
     return _lib.binding().layer_norm_modulation(x, weight, bias, eps)
 
