@@ -1,0 +1,67 @@
+"""`LinearLoRA` as a part of a model, on the host: blocks that would leave its adapters out refuse it."""
+import pytest
+import torch
+
+import triton_kernels_b200 as tk
+from triton_kernels_b200.flux.model import FluxDiT, FluxParams, LastLayer, MLPEmbedder
+from triton_kernels_b200.modules import Modulation, SelfAttention
+
+
+def lora(n_in, n_out):
+    return tk.LinearLoRA(n_in, n_out, num_adapters=2, rank=4)
+
+
+C, H = 256, 2
+PLACES = ["img_attn.qkv", "img_attn.proj", "txt_attn.qkv", "txt_attn.proj", "img_mlp.0", "img_mlp.2", "txt_mlp.0", "txt_mlp.2", "img_mod.lin", "txt_mod.lin"]
+
+
+def put(block, place):
+    old = block.get_submodule(place)
+    owner, _, name = place.rpartition(".")
+    setattr(block.get_submodule(owner), name, lora(old.in_features, old.out_features))
+    return block.to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("place", PLACES)
+def test_double_block_refuses_an_adapter_that_it_would_leave_out(place):
+    block = put(tk.DoubleStreamBlock(C, H, 4.0, qkv_bias=True), place)
+    x = torch.zeros(1, 8, C, dtype=torch.bfloat16)
+    for modulation in (None, (x[:, 0].repeat(1, 6), x[:, 0].repeat(1, 6))):
+        if modulation is not None and "mod" in place:
+            continue  # not called then
+        with pytest.raises(NotImplementedError, match="LinearLoRA"):
+            block(x, x, x[:, 0], torch.zeros(1, 1, 16, C // H // 2, 2, 2), modulation=modulation)
+
+
+@pytest.mark.parametrize("place", ["linear1", "linear2", "modulation.lin"])
+def test_single_block_refuses_an_adapter_that_it_would_leave_out(place):
+    block = put(tk.SingleStreamBlock(C, H), place)
+    x = torch.zeros(1, 8, C, dtype=torch.bfloat16)
+    with pytest.raises(NotImplementedError, match="LinearLoRA"):
+        block(x, x[:, 0], torch.zeros(1, 1, 8, C // H // 2, 2, 2))
+
+
+def test_parts_refuse_it():
+    x = torch.zeros(1, 8, C, dtype=torch.bfloat16)
+    for double in (False, True):
+        with pytest.raises(NotImplementedError, match="LinearLoRA"):
+            put(Modulation(C, double), "lin")(x[:, 0])
+    with pytest.raises(NotImplementedError, match="LinearLoRA"):
+        put(Modulation(C, True), "lin").packed_rows(x[:, 0], torch.empty(1, 6 * C, dtype=torch.bfloat16), True)
+    for place in ("qkv", "proj"):
+        with pytest.raises(NotImplementedError, match="LinearLoRA"):
+            put(SelfAttention(C, H), place)(x, torch.zeros(1, 1, 8, C // H // 2, 2, 2))
+
+
+def test_model_parts_refuse_it():
+    p = FluxParams(in_channels=16, context_in_dim=32, hidden_size=C, num_heads=H, depth=1, depth_single_blocks=1, axes_dim=[16, 56, 56])
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
+    for place in ("img_in", "txt_in"):
+        with pytest.raises(NotImplementedError, match="LinearLoRA"):
+            put(FluxDiT(p), place)(z(1, 8, 16), z(1, 4, 32), z(1), z(1), z(1, 1, 12, 64, 2, 2))
+    for place in ("in_layer", "out_layer"):
+        with pytest.raises(NotImplementedError, match="LinearLoRA"):
+            put(MLPEmbedder(256, C), place)(z(1, 256))
+    for place in ("linear", "adaLN_modulation.1"):
+        with pytest.raises(NotImplementedError, match="LinearLoRA"):
+            put(LastLayer(C, 1, 16), place)(z(1, 8, C), z(1, C))

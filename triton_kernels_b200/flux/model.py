@@ -23,7 +23,7 @@ from triton_kernels_b200 import _lib
 from triton_kernels_b200.kernels.linear import linear, linear_into
 from triton_kernels_b200.kernels.normalization import layer_norm_modulation_into
 from triton_kernels_b200.kernels.positional_embedding import apply_rope_axes
-from triton_kernels_b200.modules.blocks import DoubleStreamBlock, SingleStreamBlock
+from triton_kernels_b200.modules.blocks import DoubleStreamBlock, SingleStreamBlock, shared_only
 from triton_kernels_b200.ops.fused import modulation_silu_linear
 
 
@@ -86,6 +86,7 @@ class MLPEmbedder(nn.Module):
         self.out_layer = nn.Linear(hidden_dim, hidden_dim, bias=True)
 
     def forward(self, x: Tensor) -> Tensor:
+        shared_only(self.in_layer, self.out_layer)
         h = linear(x, self.in_layer.weight, self.in_layer.bias)
         return modulation_silu_linear(h, self.out_layer.weight, self.out_layer.bias)
 
@@ -103,6 +104,7 @@ class LastLayer(nn.Module):
     def forward(self, x: Tensor, vec: Tensor) -> Tensor:
         B, L, C = x.shape
         lin = self.adaLN_modulation[1]
+        shared_only(lin, self.linear)
         mod = modulation_silu_linear(vec, lin.weight, lin.bias)  # [B, 2C] = shift | scale
         x = x.contiguous()
         h = torch.empty_like(x)
@@ -155,6 +157,7 @@ class FluxDiT(nn.Module):
         """`pe` is the RoPE table of the joint (text first, then image) sequence, e.g.
         `self.pe_embedder(torch.cat((txt_ids, img_ids), 1))`; it does not change between
         denoising steps, so callers compute it once."""
+        shared_only(self.img_in, self.txt_in)
         _lib.require_cuda(img, txt, timesteps, pe)
         dt = self.img_in.weight.dtype
         img = linear(img.to(dt), self.img_in.weight, self.img_in.bias)

@@ -78,7 +78,8 @@ class LinearGELU(nn.Linear):
 class LinearLoRA(Linear):
     """Linear with `num_adapters` low-rank adapters of one rank; each request of a batch names its
     own.  The adapters are buffers (`lora_a` [n, R, in], `lora_b` [n, out, R], fp32 `lora_scale` [n]):
-    they are served, not trained, here.  B starts at zero, as a fresh adapter does."""
+    they are served, not trained, here.  B starts at zero, as a fresh adapter does.  It is called by
+    itself: the blocks read their linears' weight and bias and refuse one among them."""
 
     def __init__(self, in_features: int, out_features: int, num_adapters: int, rank: int, bias: bool = True):
         super().__init__(in_features, out_features, bias=bias)
@@ -91,6 +92,15 @@ class LinearLoRA(Linear):
         if adapter is None:
             return super().forward(input)
         return linear_lora(input, self.weight, self.bias, self.lora_a, self.lora_b, adapter, self.lora_scale)
+
+
+def shared_only(*linears: nn.Module) -> None:
+    """Refuses adapters where a fused path reads a linear's weight and bias and would leave them out."""
+    for lin in linears:
+        if isinstance(lin, LinearLoRA):
+            raise NotImplementedError(
+                "the blocks' fused projections have no low-rank adapters: a LinearLoRA in their place would run without its "
+                "own (call it by itself, or merge the adapter into the weight)")
 
 
 def MLP(hidden_size: int, mlp_hidden_dim: int, bias: bool = True) -> nn.Sequential:
@@ -111,6 +121,7 @@ class SelfAttention(nn.Module):
         self.proj = Linear(dim, dim)
 
     def forward(self, x: Tensor, pe: Tensor) -> Tensor:
+        shared_only(self.qkv, self.proj)
         B, L, C = x.shape
         qkv = self.qkv(x)
         attn = torch.empty((B, L, C), device=x.device, dtype=x.dtype)
@@ -134,17 +145,21 @@ class Modulation(nn.Module):
 
     def packed(self, vec: Tensor) -> Tensor:
         """[B, multiplier*dim]: shift | scale | gate (| shift2 | scale2 | gate2)."""
-        return modulation_silu_linear(vec, self.lin.weight, self.lin.bias)
+        lin = self.lin
+        shared_only(lin)
+        return modulation_silu_linear(vec, lin.weight, lin.bias)
 
     def packed_rows(self, vec: Tensor, out: Tensor, first_half: bool, light: bool = False) -> None:
         """Fills one half of the packed [B, 6*dim] tensor of a double modulation: shift | scale |
         gate (needed before attention) or shift2 | scale2 | gate2 (needed after it)."""
-        n = self.lin.weight.shape[0] // 2
+        lin = self.lin
+        shared_only(lin)
+        n = lin.weight.shape[0] // 2
         r0, r1 = (0, n) if first_half else (n, 2 * n)
-        bias = self.lin.bias
+        bias = lin.bias
         if bias is not None and bias.dtype != torch.bfloat16:
             bias = bias.to(torch.bfloat16)
-        modulation_silu_linear_rows(vec.contiguous(), self.lin.weight, bias, out, r0, r1, light)
+        modulation_silu_linear_rows(vec.contiguous(), lin.weight, bias, out, r0, r1, light)
 
     def forward(self, vec: Tensor) -> tuple[ModulationOut, ModulationOut | None]:
         out = self.packed(vec)[:, None, :].chunk(self.multiplier, dim=-1)
@@ -284,6 +299,10 @@ class SingleStreamBlock(nn.Module):
     def forward(self, x: Tensor, vec: Tensor, pe: Tensor, modulation: Tensor | None = None) -> Tensor:
         """`modulation` may carry the packed [B, 3C] output of `self.modulation.packed(vec)`
         computed ahead of time (it depends on `vec` only); by default it is computed here."""
+        linear1, linear2 = self.linear1, self.linear2
+        shared_only(linear1, linear2)
+        if modulation is None:
+            shared_only(self.modulation.lin)
         _check_inputs(x, vec)
         x = x.contiguous()
         B, L, C = x.shape
@@ -301,13 +320,13 @@ class SingleStreamBlock(nn.Module):
             # through GELU into the concat buffer
             qkv_heads = torch.empty((3, B, H, L, D), device=x.device, dtype=x.dtype)
             linear_qkv_grouped_into(
-                [dict(x=x_mod, w=self.linear1.weight, b=self.linear1.bias, q_scale=self.norm.query_norm.scale,
+                [dict(x=x_mod, w=linear1.weight, b=linear1.bias, q_scale=self.norm.query_norm.scale,
                       k_scale=self.norm.key_norm.scale, y2=cat.view(B * L, C + M)[:, C:])],
                 pe, qkv_heads, eps=1e-6, epi2=_lib.EPI_GELU)
             attention_into(qkv_heads[0], qkv_heads[1], qkv_heads[2],
                            cat[:, :, :C].unflatten(2, (H, D)).permute(0, 2, 1, 3), self.scale)
             out = torch.empty_like(x)
-            _gated_linear(cat.view(B * L, C + M), self.linear2, x.view(B * L, C), mod[:, 2 * C : 3 * C], L, out.view(B * L, C))
+            _gated_linear(cat.view(B * L, C + M), linear2, x.view(B * L, C), mod[:, 2 * C : 3 * C], L, out.view(B * L, C))
             return out
         if (sp is not None and sp.world > 1 and sp.scatter_from_projection and self.fuse_qkv_epilogue
                 and qkv_projection_scatter_supported((L,), D, H, B) and (3 * C) % 256 == 0 and M % 8 == 0):
@@ -315,28 +334,28 @@ class SingleStreamBlock(nn.Module):
             # group straight into the arena of the rank that attends over it
             pb = sp.peer_buffers(B, L, H, D, x.dtype)
             linear_qkv_grouped_into(
-                [dict(x=x_mod, w=self.linear1.weight, b=self.linear1.bias, q_scale=self.norm.query_norm.scale,
+                [dict(x=x_mod, w=linear1.weight, b=linear1.bias, q_scale=self.norm.query_norm.scale,
                       k_scale=self.norm.key_norm.scale, y2=cat.view(B * L, C + M)[:, C:])],
                 pe, None, eps=1e-6, epi2=_lib.EPI_GELU, scatter=_scatter_target(pb, H, D))
             _peer_attention(pb, L, self.scale, cat[:, :, :C])
             out = torch.empty_like(x)
-            _gated_linear(cat.view(B * L, C + M), self.linear2, x.view(B * L, C), mod[:, 2 * C : 3 * C], L, out.view(B * L, C))
+            _gated_linear(cat.view(B * L, C + M), linear2, x.view(B * L, C), mod[:, 2 * C : 3 * C], L, out.view(B * L, C))
             return out
         qkv = torch.empty((B, L, 3 * C), device=x.device, dtype=x.dtype)
         if (3 * C) % 256 == 0:
             linear_into(
-                x_mod.view(B * L, C), self.linear1.weight, self.linear1.bias, qkv.view(B * L, 3 * C),
+                x_mod.view(B * L, C), linear1.weight, linear1.bias, qkv.view(B * L, 3 * C),
                 y2=cat.view(B * L, C + M)[:, C:], split=3 * C, epi2=_lib.EPI_GELU,
             )
         else:  # narrow models whose qkv width is not a whole number of column tiles
-            w, b = self.linear1.weight, self.linear1.bias
+            w, b = linear1.weight, linear1.bias
             linear_into(x_mod.view(B * L, C), w[: 3 * C], b[: 3 * C], qkv.view(B * L, 3 * C))
             linear_into(x_mod.view(B * L, C), w[3 * C :], b[3 * C :], cat.view(B * L, C + M)[:, C:], epi=_lib.EPI_GELU)
 
         _joint_attention([(qkv, self.norm)], pe, H, self.scale, cat[:, :, :C], self.sequence_parallel)
 
         out = torch.empty_like(x)
-        _gated_linear(cat.view(B * L, C + M), self.linear2, x.view(B * L, C), mod[:, 2 * C : 3 * C], L, out.view(B * L, C))
+        _gated_linear(cat.view(B * L, C + M), linear2, x.view(B * L, C), mod[:, 2 * C : 3 * C], L, out.view(B * L, C))
         return out
 
 
@@ -365,6 +384,13 @@ class DoubleStreamBlock(nn.Module):
                 modulation: tuple[Tensor, Tensor] | None = None) -> tuple[Tensor, Tensor]:
         """`modulation` may carry (txt, img) packed [B, 6C] modulation tensors computed ahead of
         time from `vec`; by default they are computed here."""
+        # stream order everywhere below: (txt, img), the order of the joint sequence
+        attns = (self.txt_attn, self.img_attn)
+        qkv_lins, proj_lins = [a.qkv for a in attns], [a.proj for a in attns]
+        ups_downs = [(mlp[0], mlp[2]) for mlp in (self.txt_mlp, self.img_mlp)]
+        shared_only(*qkv_lins, *proj_lins, *ups_downs[0], *ups_downs[1])
+        if modulation is None:
+            shared_only(self.txt_mod.lin, self.img_mod.lin)
         _check_inputs(img, txt, vec)
         img, txt = img.contiguous(), txt.contiguous()
         B, Li, C = img.shape
@@ -372,11 +398,8 @@ class DoubleStreamBlock(nn.Module):
         H = self.num_heads
         D = C // H
         dev, dt = img.device, img.dtype
-        # stream order everywhere below: (txt, img), the order of the joint sequence
         xs = (txt, img)
         Ls = (Lt, Li)
-        attns = (self.txt_attn, self.img_attn)
-        mlps = (self.txt_mlp, self.img_mlp)
         # The block opens with bandwidth-bound work only (two weight-streaming modulation
         # projections, two LayerNorms); the text stream's half runs on a side stream next to the
         # image stream's so that the two together keep HBM busy.
@@ -429,8 +452,8 @@ class DoubleStreamBlock(nn.Module):
             # rotation and the head-major text|image layout attention reads
             qkv_heads = torch.empty((3, B, H, Lt + Li, D), device=dev, dtype=dt)
             linear_qkv_grouped_into([
-                dict(x=h, w=a.qkv.weight, b=a.qkv.bias, q_scale=a.norm.query_norm.scale, k_scale=a.norm.key_norm.scale)
-                for h, a in zip(h1, attns)], pe, qkv_heads, eps=1e-6)
+                dict(x=h, w=lin.weight, b=lin.bias, q_scale=a.norm.query_norm.scale, k_scale=a.norm.key_norm.scale)
+                for h, a, lin in zip(h1, attns, qkv_lins)], pe, qkv_heads, eps=1e-6)
             attn = torch.empty((B, Lt + Li, C), device=dev, dtype=dt)
             attention_into(qkv_heads[0], qkv_heads[1], qkv_heads[2], attn.unflatten(2, (H, D)).permute(0, 2, 1, 3), D**-0.5)
         elif (sp is not None and sp.world > 1 and sp.scatter_from_projection and self.fuse_qkv_epilogue
@@ -439,8 +462,8 @@ class DoubleStreamBlock(nn.Module):
             # of the rank that attends over it
             pb = sp.peer_buffers(B, Lt + Li, H, D, dt)
             linear_qkv_grouped_into([
-                dict(x=h, w=a.qkv.weight, b=a.qkv.bias, q_scale=a.norm.query_norm.scale, k_scale=a.norm.key_norm.scale)
-                for h, a in zip(h1, attns)], pe, None, eps=1e-6, scatter=_scatter_target(pb, H, D))
+                dict(x=h, w=lin.weight, b=lin.bias, q_scale=a.norm.query_norm.scale, k_scale=a.norm.key_norm.scale)
+                for h, a, lin in zip(h1, attns, qkv_lins)], pe, None, eps=1e-6, scatter=_scatter_target(pb, H, D))
             attn = _peer_attention(pb, Lt + Li, D**-0.5, None)
         elif (sp is not None and sp.world > 1 and sp.exchange == "peer" and sp.pipeline_exchange and B == 1
               and Li >= 512):
@@ -454,15 +477,15 @@ class DoubleStreamBlock(nn.Module):
             pieces = exchange_pieces(Li, 2)
             qkvs = [torch.empty((B, L, 3 * C), device=dev, dtype=dt) for L in Ls]
             x_img, y_img = h1[1].view(Li, C), qkvs[1].view(Li, 3 * C)
-            a_t, a_i = attns
+            lin_t, lin_i = qkv_lins
             norms = [(a.norm.query_norm.scale.to(dt), a.norm.key_norm.scale.to(dt)) for a in attns]
             pe_rows = pe.reshape(-1, D // 2, 2, 2)
             scat = (pb.P, pb.k_off, pb.v_off, H, D, pb.qkv_strides)
             for i, (r0, r1) in enumerate(pieces):
                 last = r1 == Li
-                probs = [dict(x2d=x_img[r0:r1], w=a_i.qkv.weight, b=a_i.qkv.bias, y=y_img[r0:r1])]
+                probs = [dict(x2d=x_img[r0:r1], w=lin_i.weight, b=lin_i.bias, y=y_img[r0:r1])]
                 if i == 0:
-                    probs.insert(0, dict(x2d=h1[0].view(Lt, C), w=a_t.qkv.weight, b=a_t.qkv.bias, y=qkvs[0].view(Lt, 3 * C)))
+                    probs.insert(0, dict(x2d=h1[0].view(Lt, C), w=lin_t.weight, b=lin_t.bias, y=qkvs[0].view(Lt, 3 * C)))
                 linear_grouped_into(probs)
                 srcs = [(qkvs[1][:, r0:r1], *norms[1])]
                 if i == 0:
@@ -481,8 +504,8 @@ class DoubleStreamBlock(nn.Module):
             # both streams' qkv projections in one launch, then the assembly kernel
             qkvs = [torch.empty((B, L, 3 * C), device=dev, dtype=dt) for L in Ls]
             linear_grouped_into([
-                dict(x2d=h.view(B * L, C), w=a.qkv.weight, b=a.qkv.bias, y=o.view(B * L, 3 * C))
-                for h, a, o, L in zip(h1, attns, qkvs, Ls)])
+                dict(x2d=h.view(B * L, C), w=lin.weight, b=lin.bias, y=o.view(B * L, 3 * C))
+                for h, lin, o, L in zip(h1, qkv_lins, qkvs, Ls)])
             attn = _joint_attention([(qkvs[0], self.txt_attn.norm), (qkvs[1], self.img_attn.norm)], pe, H, D**-0.5,
                                     None, sp)
 
@@ -493,7 +516,7 @@ class DoubleStreamBlock(nn.Module):
         for s_ in range(2):
             for b in range(B):
                 g, gs = gate_of(mods[s_], 2, b)
-                probs.append(dict(x2d=attn[b, row0[s_] : row0[s_] + Ls[s_]], w=attns[s_].proj.weight, b=attns[s_].proj.bias,
+                probs.append(dict(x2d=attn[b, row0[s_] : row0[s_] + Ls[s_]], w=proj_lins[s_].weight, b=proj_lins[s_].bias,
                                   y=x1[s_][b], resid=xs[s_][b], gate=g, gate_stride=gs, rows_per_batch=Ls[s_]))
         linear_grouped_into(probs, epi=_lib.EPI_GATE_RESID)
 
@@ -508,15 +531,15 @@ class DoubleStreamBlock(nn.Module):
         h2 = [h2_txt, _ln_mod(x1[1], mods[1], 3)]
         main.wait_stream(side)
         h2_txt.record_stream(main)
-        ups = [torch.empty((B * L, mlp[0].out_features), device=dev, dtype=dt) for L, mlp in zip(Ls, mlps)]
+        ups = [torch.empty((B * L, up.out_features), device=dev, dtype=dt) for L, (up, _) in zip(Ls, ups_downs)]
         linear_grouped_into([
-            dict(x2d=h.view(B * L, C), w=mlp[0].weight, b=mlp[0].bias, y=u) for h, mlp, u, L in zip(h2, mlps, ups, Ls)],
+            dict(x2d=h.view(B * L, C), w=up.weight, b=up.bias, y=u) for h, (up, _), u, L in zip(h2, ups_downs, ups, Ls)],
             epi=_lib.EPI_GELU)
         outs = [torch.empty_like(x) for x in xs]
         probs = []
         for s_ in range(2):
             g, gs = gate_of(mods[s_], 5)
-            probs.append(dict(x2d=ups[s_], w=mlps[s_][2].weight, b=mlps[s_][2].bias, y=outs[s_].view(B * Ls[s_], C),
+            probs.append(dict(x2d=ups[s_], w=ups_downs[s_][1].weight, b=ups_downs[s_][1].bias, y=outs[s_].view(B * Ls[s_], C),
                               resid=x1[s_].view(B * Ls[s_], C), gate=g, gate_stride=gs, rows_per_batch=Ls[s_]))
         linear_grouped_into(probs, epi=_lib.EPI_GATE_RESID)
         return outs[1], outs[0]
