@@ -1,4 +1,5 @@
-"""`LinearLoRA` as a part of a model, on the host: blocks that would leave its adapters out refuse it."""
+"""`LinearLoRA` as a part of a model, on the host: its scales keep their type, and blocks that would
+leave its adapters out refuse it."""
 import pytest
 import torch
 
@@ -9,6 +10,27 @@ from triton_kernels_b200.modules import Modulation, SelfAttention
 
 def lora(n_in, n_out):
     return tk.LinearLoRA(n_in, n_out, num_adapters=2, rank=4)
+
+
+def test_scale_stays_fp32():
+    m = lora(16, 8)
+    m.lora_scale.copy_(torch.tensor([1 / 3, 0.7]))
+    want = m.lora_scale.clone()
+    for cast in (lambda t: t.to(torch.bfloat16), lambda t: t.half(), lambda t: t.double(), lambda t: t.float(), lambda t: torch.nn.Sequential(t).bfloat16()[0]):
+        m = cast(m)
+        assert m.lora_scale.dtype == torch.float32 and torch.equal(m.lora_scale, want)
+    assert m.lora_a.dtype == m.lora_b.dtype == m.weight.dtype == m.bias.dtype == torch.bfloat16
+    assert m.to("meta").lora_scale.is_meta and m.lora_scale.dtype == torch.float32
+    assert "lora_scale" in m.state_dict()
+
+
+def test_scale_is_fp32_whatever_the_default_type():
+    default = torch.get_default_dtype()
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        assert lora(16, 8).lora_scale.dtype == torch.float32
+    finally:
+        torch.set_default_dtype(default)
 
 
 C, H = 256, 2

@@ -85,7 +85,15 @@ class LinearLoRA(Linear):
         super().__init__(in_features, out_features, bias=bias)
         self.register_buffer("lora_a", torch.randn(num_adapters, rank, in_features) * in_features**-0.5)
         self.register_buffer("lora_b", torch.zeros(num_adapters, out_features, rank))
-        self.register_buffer("lora_scale", torch.ones(num_adapters))
+        self.register_buffer("lora_scale", torch.ones(num_adapters, dtype=torch.float32))
+
+    def _apply(self, fn, recurse=True):
+        """The scales stay fp32 when the module's type changes (`.to(torch.bfloat16)`), and follow it to a device."""
+        scale = self.lora_scale
+        super()._apply(fn, recurse)
+        if scale.dtype == torch.float32 and self.lora_scale.dtype != torch.float32:
+            self.lora_scale = scale.to(self.lora_scale.device)
+        return self
 
     def forward(self, input: Tensor, adapter: Tensor | None = None) -> Tensor:
         """`adapter` [B] int32 or int64, -1 for none; without it the shared projection alone."""
