@@ -3,6 +3,7 @@
 // results, and calls the C ABI (fluxb200.h) on the current stream of the tensors' device.  The autograd nodes live here
 // because a backward pass runs on a thread of its own, where Python code waits for the interpreter: a training call of
 // the norm took the host 121 us with Python wrappers and takes 67 here.  Nothing here computes anything.
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -81,6 +82,17 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
+// Forward-mode tangents would be lost without a word: refused.
+void no_tangents(std::initializer_list<const Tensor*> ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->_fw_grad(/*level=*/0).defined())
+      fail(PyExc_NotImplementedError, "fluxb200 kernels have no forward-mode derivative: detach the dual tensor");
+}
+const Tensor* given(const std::optional<Tensor>& t) {
+  static const Tensor none;
+  return t.has_value() ? &*t : &none;
+}
 // Results of a backward pass that somebody wants to differentiate: an error to be raised when they do, not a silent
 // zero (what torch.autograd.function.once_differentiable does for Python functions).
 variable_list once(variable_list grads) {
@@ -152,6 +164,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 };
 
 Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight_in, const std::optional<Tensor>& bias_in, double eps) {
+  no_tangents({&x, given(weight_in), given(bias_in)});
   require_cuda(x);
   dtype_code(x);
   require(x.dim() > 0 && x.size(-1) > 0, "layer_norm runs over the last dim, which must not be empty");
@@ -226,6 +239,7 @@ struct LayerNormModulation : torch::autograd::Function<LayerNormModulation> {
 };
 
 Tensor layer_norm_modulation(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps) {
+  no_tangents({&x, &weight, &bias});
   require(x.dim() > 0 && weight.dim() > 0 && bias.dim() > 0 && x.size(0) == weight.size(0) && x.size(0) == bias.size(0),
           "x, weight and bias differ in the batch dim");
   require(x.size(-1) == weight.size(-1) && x.size(-1) == bias.size(-1), "x, weight and bias differ in the last dim");
@@ -288,6 +302,7 @@ struct RopeAxes : torch::autograd::Function<RopeAxes> {
 };
 
 std::pair<Tensor, Tensor> apply_rope_axes(const Tensor& q, const Tensor& k, const Tensor& ids, std::vector<int64_t> axes, double theta) {
+  no_tangents({&q, &k, &ids});
   require_cuda(q);
   same_device(q, k);
   same_device(q, ids);
@@ -309,6 +324,7 @@ std::pair<Tensor, Tensor> apply_rope_axes(const Tensor& q, const Tensor& k, cons
 // ---- adapters ----------------------------------------------------------------------------------------------------
 Tensor linear_lora(const Tensor& x, const Tensor& w_in, const std::optional<Tensor>& b_in, const Tensor& lora_a, const Tensor& lora_b_in,
                    const Tensor& adapter, const std::optional<Tensor>& scale_in, bool gelu) {
+  no_tangents({&x, &w_in, given(b_in), &lora_a, &lora_b_in, given(scale_in)});
   require(x.dim() >= 2 && w_in.dim() == 2 && x.size(-1) == w_in.size(1) && w_in.size(1) > 0, "Incompatible dimensions");
   const int64_t N = w_in.size(0), K = w_in.size(1), n = lora_a.dim() == 3 ? lora_a.size(0) : 0, R = n > 0 ? lora_a.size(1) : 0;
   require(n > 0 && R > 0 && lora_a.size(2) == K && lora_b_in.dim() == 3 && lora_b_in.size(0) == n && lora_b_in.size(1) == N &&
