@@ -1,5 +1,5 @@
-"""`LinearLoRA` as a part of a model, on the host: its scales keep their type, and blocks that would
-leave its adapters out refuse it."""
+"""`LinearLoRA` as a part of a model, on the host: its scales keep their type, nothing of it is
+trained, and blocks that would leave its adapters out refuse it."""
 import pytest
 import torch
 
@@ -31,6 +31,28 @@ def test_scale_is_fp32_whatever_the_default_type():
         assert lora(16, 8).lora_scale.dtype == torch.float32
     finally:
         torch.set_default_dtype(default)
+
+
+def test_a_gradient_that_would_be_lost_is_refused():
+    """The operator is forward only; before it looks at anything else it refuses every argument that wants a gradient."""
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
+    args = [z(2, 3, 16), z(8, 16), z(8), z(1, 4, 16), z(1, 8, 4), torch.zeros(2, dtype=torch.int64), torch.ones(1)]
+    for i in (0, 1, 2, 3, 4, 6):
+        call = [a.clone().requires_grad_() if j == i else a for j, a in enumerate(args)]
+        with pytest.raises(NotImplementedError, match="forward only"):
+            tk.linear_lora(*call)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA tensors only"):
+            tk.linear_lora(*call)
+
+
+def test_weight_and_bias_of_the_module_are_not_trained():
+    m = lora(16, 8).to(torch.bfloat16)
+    assert not any(p.requires_grad for p in m.parameters()) and list(m.state_dict()) == ["weight", "bias", "lora_a", "lora_b", "lora_scale"]
+    x, idx = torch.zeros(2, 3, 16, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        m(x, idx)
+    with pytest.raises(NotImplementedError, match="forward only"):
+        m.requires_grad_()(x, idx)
 
 
 C, H = 256, 2

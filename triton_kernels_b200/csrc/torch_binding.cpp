@@ -324,7 +324,10 @@ std::pair<Tensor, Tensor> apply_rope_axes(const Tensor& q, const Tensor& k, cons
 // ---- adapters ----------------------------------------------------------------------------------------------------
 Tensor linear_lora(const Tensor& x, const Tensor& w_in, const std::optional<Tensor>& b_in, const Tensor& lora_a, const Tensor& lora_b_in,
                    const Tensor& adapter, const std::optional<Tensor>& scale_in, bool gelu) {
-  no_tangents({&x, &w_in, given(b_in), &lora_a, &lora_b_in, given(scale_in)});
+  const std::initializer_list<const Tensor*> numbers = {&x, &w_in, given(b_in), &lora_a, &lora_b_in, given(scale_in)};
+  no_tangents(numbers);
+  if (wants_grad(numbers))
+    fail(PyExc_NotImplementedError, "linear_lora is forward only: call it under torch.no_grad() or detach its inputs");
   require(x.dim() >= 2 && w_in.dim() == 2 && x.size(-1) == w_in.size(1) && w_in.size(1) > 0, "Incompatible dimensions");
   const int64_t N = w_in.size(0), K = w_in.size(1), n = lora_a.dim() == 3 ? lora_a.size(0) : 0, R = n > 0 ? lora_a.size(1) : 0;
   require(n > 0 && R > 0 && lora_a.size(2) == K && lora_b_in.dim() == 3 && lora_b_in.size(0) == n && lora_b_in.size(1) == N &&
@@ -345,9 +348,7 @@ Tensor linear_lora(const Tensor& x, const Tensor& w_in, const std::optional<Tens
   }
   if (adapter.scalar_type() != at::kInt && adapter.scalar_type() != at::kLong)
     fail(PyExc_TypeError, std::string("adapter indices are int32 or int64, got ") + c10::toString(adapter.scalar_type()));
-  if (wants_grad({&x, &lora_a, &lora_b_in}) || (scale_in.has_value() && wants_grad({&*scale_in})))
-    fail(PyExc_NotImplementedError, "linear_lora is forward only: call it under torch.no_grad() or detach its inputs");
-  at::NoGradGuard no_grad;  // (a weight that requires a gradient is used as it is, as by `linear`)
+  at::NoGradGuard no_grad;
   c10::cuda::CUDAGuard guard(x.device());
   std::vector<int64_t> shape = x.sizes().vec();
   shape.back() = N;

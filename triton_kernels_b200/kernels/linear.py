@@ -213,7 +213,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None, activation:
 def linear_lora(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None, lora_a: torch.Tensor, lora_b: torch.Tensor,
                 adapter: torch.Tensor, lora_scale: torch.Tensor | None = None, activation: str = "") -> torch.Tensor:
     """act(x @ w.T + b + scale_a * (x @ A_a.T) @ B_a.T): a projection shared by all requests plus one
-    low-rank adapter per request, a = adapter[request].  bf16 in/out, fp32 accumulation; forward only.
+    low-rank adapter per request, a = adapter[request].  bf16 in/out, fp32 accumulation; forward only:
+    where gradients are enabled, an argument that requires one (a weight or bias, too) is refused.
 
     x [B, ..., K]: the first dim counts the requests (x [B, K] is one row per request).  w [N, K], b
     [N] or None as in `linear`; lora_a [n, R, K], lora_b [n, N, R] bf16; lora_scale [n] fp32 or None

@@ -78,11 +78,13 @@ class LinearGELU(nn.Linear):
 class LinearLoRA(Linear):
     """Linear with `num_adapters` low-rank adapters of one rank; each request of a batch names its
     own.  The adapters are buffers (`lora_a` [n, R, in], `lora_b` [n, out, R], fp32 `lora_scale` [n]):
-    they are served, not trained, here.  B starts at zero, as a fresh adapter does.  It is called by
+    they are served, not trained, here, and so are weight and bias (`requires_grad` off; a call that would
+    have to give a gradient is refused).  B starts at zero, as a fresh adapter does.  It is called by
     itself: the blocks read their linears' weight and bias and refuse one among them."""
 
     def __init__(self, in_features: int, out_features: int, num_adapters: int, rank: int, bias: bool = True):
         super().__init__(in_features, out_features, bias=bias)
+        self.requires_grad_(False)
         self.register_buffer("lora_a", torch.randn(num_adapters, rank, in_features) * in_features**-0.5)
         self.register_buffer("lora_b", torch.zeros(num_adapters, out_features, rank))
         self.register_buffer("lora_scale", torch.ones(num_adapters, dtype=torch.float32))
