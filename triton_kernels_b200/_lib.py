@@ -86,7 +86,7 @@ SIGNATURES = {
 }
 
 _lib = None
-kernel_calls = 0  # C-ABI compute calls that returned success (each launches at least one kernel)
+_checked_calls = 0  # calls that `check` saw; `kernel_calls` adds those of the binding
 
 
 class FluxbError(RuntimeError):
@@ -114,10 +114,10 @@ def load() -> ctypes.CDLL:
 def check(rc: int, launches: bool = True) -> None:
     """Turns a status code into the Python exception the reference API would raise.  Setup calls
     that launch nothing pass launches=False so that `kernel_calls` counts kernels only."""
-    global kernel_calls
+    global _checked_calls
     if rc == 0:
         if launches:
-            kernel_calls += 1
+            _checked_calls += 1
         return
     msg = load().fluxb_last_error().decode()
     if rc == ERR_BAD_ARG:
@@ -150,7 +150,7 @@ def ptr(t) -> int | None:
 def binding():
     """The module of the operators that bind through torch's C++ API (csrc/torch_binding.cpp): calls
     so short that a Python wrapper would cost more than their kernels.  They do not pass through
-    `check`, so `kernel_calls` does not count them."""
+    `check`; the module counts its own calls for `kernel_calls`."""
     global _binding
     if _binding is None:
         path = LIB_PATH.parent / "_binding.so"
@@ -165,6 +165,13 @@ def binding():
 
 
 _binding = None
+
+
+def __getattr__(name: str):
+    """`kernel_calls`: C-ABI compute calls that returned success (each launches at least one kernel)."""
+    if name == "kernel_calls":
+        return _checked_calls + (_binding.calls() if _binding is not None else 0)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 def stream_handle() -> int:

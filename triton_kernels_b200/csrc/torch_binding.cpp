@@ -9,6 +9,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <atomic>
 #include <string>
 #include <vector>
 
@@ -30,8 +31,12 @@ namespace {
 void require(bool ok, const char* text) {
   if (!ok) fail(PyExc_AssertionError, text);
 }
+std::atomic<int64_t> calls{0};  // that returned success
 void check(int rc) {
-  if (rc == FLUXB_OK) return;
+  if (rc == FLUXB_OK) {
+    ++calls;
+    return;
+  }
   const std::string text = fluxb_last_error();
   if (rc == FLUXB_ERR_BAD_ARG) fail(PyExc_ValueError, text);
   if (rc == FLUXB_ERR_UNSUPPORTED) fail(PyExc_NotImplementedError, text);
@@ -387,4 +392,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layer_norm_modulation", &layer_norm_modulation);
   m.def("apply_rope_axes", &apply_rope_axes);
   m.def("linear_lora", &linear_lora);
+  m.def("calls", [] { return calls.load(); });
 }
