@@ -334,7 +334,10 @@ int fluxb_layer_norm_bwd(const void* dy, const void* x, const void* factor, cons
  * Rotary positions with several axes, from position ids instead of a table: the pairs (2j, 2j+1)
  * of a head are dealt to the axes in order, axes_dim[i] columns to axis i, and pair j' of an axis
  * of d columns turns by ids[b, l, axis] * theta^(-2 j'/d).  Columns behind the axes are copied.
- * The angle is taken in fp64.  backward != 0 turns the other way: the gradient.
+ * The turn left over after whole turns is right to 2^-24 of a turn for up to 2^27 turns (positions of
+ * 8e8 at the fastest pair of a theta above one), beyond that to 2^-52 of the number of turns: the
+ * frequency is fp64, the product two fp32 parts for positions below 2^24 and fp64 beyond; integers
+ * above 2^53 are rounded to fp64 first.  backward != 0 turns the other way: the gradient.
  *   q, k, oq, ok: [B, heads, L, D], each with strides (batch, head, row) in elements, unit stride
  *   on D; Hq and Hk may differ and either may be 0.  ids: [B, L, n_axes] of id_type
  *   (FLUXB_ID_*) with its three strides (0 to share).  At most 8 axes and 128 rotated pairs.

@@ -4,9 +4,11 @@
 // same rotation by the negative angle.
 //
 // Angles: the position times the pair's turns per unit position (theta^(-2j'/d) / 2 pi, from the host in fp64) is
-// taken exactly enough that the turn left over after whole turns, in [-1/2, 1/2], is right to 2^-25: in two fp32 parts
-// for positions below 2^24, in fp64 beyond (fp64 throughout: 17.5 us instead of 15.9 for 16 heads of 8192 tokens); sine
-// and cosine of the reduced turn are fp32.
+// taken exactly enough that the turn left over after whole turns is right to 2^-24 for up to 2^27 turns: in two fp32
+// parts for positions below 2^24 and less than 2^22 turns (the low part's rounding 2^-26, that of adding what it gives
+// 2^-26, the sum's 2^-25), in fp64 beyond (frequency and product each 2^-53 of the turns, 2^-25 at 2^27 of them, and 2^-26
+// for the result in fp32; past that the error grows with the turns, and integers above 2^53 are rounded first).  (fp64
+// throughout: 17.5 us instead of 15.9 for 16 heads of 8192 tokens.)  Sine and cosine of the reduced turn are fp32.
 #include <math.h>
 
 #include "vec.cuh"
@@ -50,7 +52,7 @@ __device__ __forceinline__ float2 turn_of(const RopeAxesArgs& a, Id id, int j, f
   if (id > static_cast<Id>(-(1 << 24)) && id < static_cast<Id>(1 << 24) && fabsf(high) < 4194304.f) {
     // pos is exact in fp32 and the turn count below 2^22 (a theta below one may turn faster): the product as high part
     // and error, both exact, the whole turns taken off the high part (exact, too), then what the frequency's low part
-    // adds (2^-49 of the turns off)
+    // adds (2^-48 of the turns off)
     const float whole = (high + 12582912.f) - 12582912.f;  // 1.5 * 2^23: to the nearest integer
     r = (high - whole) + fmaf(pos, turns.y, fmaf(pos, turns.x, -high));
   } else {
@@ -66,7 +68,8 @@ __device__ __forceinline__ float2 turn_of(const RopeAxesArgs& a, Id id, int j, f
 // pairs' sines and cosines in registers and walks every `slots`-th head of q and k.  A pair's angle is so taken once, no
 // table is read or written, and the next kAhead pieces of a thread are on their way while it works on the current ones.
 // Bound by HBM: every element is read once and written once; 24 + 24 heads of 4608 tokens, 128 columns bf16: 21.0 us, 5.4
-// TB/s.  (With the angles taken again for every group of heads: 37 us.)
+// TB/s.  (With the angles taken again for every group of heads: 37 us.)  At four blocks per SM the bf16 form without
+// sharing spills 28 to 44 bytes a thread.
 // kShare: where several threads walk the same piece's heads (slots > 1), the block's threads first take one angle each and
 // pass them on through shared memory; where a piece has one thread it takes its own.  With 512 tokens of 8 + 8 heads sharing
 // takes 5.1 us and not sharing 6.2; with one thread a piece the barriers cost: 16 x 4096 tokens of 1 + 1 heads, 64 columns,

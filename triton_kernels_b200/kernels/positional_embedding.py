@@ -39,6 +39,8 @@ def apply_rope_axes(xq: torch.Tensor, xk: torch.Tensor, ids: torch.Tensor, axes_
     layouts are copied); the results have the inputs' layout.  ids: [B, L, n_axes] or
     [1, L, n_axes], float32 (fractions allowed), int32 or int64.  axes_dim: the even number of
     columns of each axis, in order; their sum may be less than D, and the columns behind them are
-    copied.  Pair j of an axis of d columns turns by ids * theta^(-2j/d), taken in fp64.
+    copied.  Pair j of an axis of d columns turns by ids * theta^(-2j/d): right to 2^-24 of a turn
+    after whole turns for up to 2^27 turns (positions of 8e8), to 2^-52 of the number of turns beyond
+    (the product is two fp32 parts for positions below 2^24, fp64 for others).
     Differentiable once in xq and xk; ids that require a gradient are refused."""
     return _lib.binding().apply_rope_axes(xq, xk, ids, axes_dim, theta)
