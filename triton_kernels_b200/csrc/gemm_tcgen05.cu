@@ -605,7 +605,8 @@ __device__ __forceinline__ void qkv_tile_epilogue(const Params& p, const CUtenso
 //      every adapter that the tile's rows use, the MMAs t_high B^T and t_low B^T accumulate into the
 //      same TMEM tile through the same ring, with a lane mask that leaves the other requests' rows
 //      alone (so a request never meets another one's adapter, not even as a product with zero).
-//      Cost: R / 32 ring slots per adapter of a tile, next to K / 64 of the projection.
+//      Cost per adapter of a tile: one ring slot for ranks up to 32, two per 64 ranks for more, next to K / 64 of the
+//      projection.
 // kCols: output columns per tile.  Modes 0 to 2 have one width, 256; mode 3 takes a narrower one where that fills the
 // machine better.
 template <int kMode, typename G = Grouped, int kCols = BN>

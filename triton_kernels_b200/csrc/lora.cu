@@ -5,7 +5,9 @@
 // (t = high + low to 2^-17 of |t|), so that the tensor cores take it without the rounding a single bf16 would put
 // between the two products.  Both kernels may start while the one in front of them ends: the first waits for everything
 // before it (in every block, before anything is read), only then does it let the second start, and that one waits for
-// t.  In a stream of such calls that took 16.4 us to 13.2 (48 x 5 rows, 1024 -> 4096, 16 adapters) and 26.0 to 24.2 (8 x 1
+// t alone: its x, W, bias, indices and B, which it reads without a wait of its own and partly by the read-only path, are
+// complete because of that order.  So pdl_release() stays behind pdl_wait() in every kernel of this file, and a block that
+// leaves early leaves behind its wait.  In a stream of such calls that took 16.4 us to 13.2 (48 x 5 rows, 1024 -> 4096, 16 adapters) and 26.0 to 24.2 (8 x 1
 // row, 3072 -> 18432).  An adapter index outside [-1, n) leaves its request without an adapter and is recorded
 // in the device status word (site 81).
 #include "lora.cuh"
@@ -89,7 +91,9 @@ __global__ void __launch_bounds__(THREADS, 1) lora_shrink_kernel(const __grid_co
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = tmem_slot;
-  pdl_release();  // behind the TMEM allocation: the projection's blocks take all of an SM's TMEM
+  // behind pdl_wait() above, on which the projection's own reads rely, and behind the TMEM allocation: the projection's
+  // blocks take all of an SM's TMEM
+  pdl_release();
 
   if (warp == 0) {
     int stage = 0;
@@ -318,7 +322,9 @@ __global__ void __launch_bounds__(128) lora_shrink_one_kernel(const ShortParams 
   const int request = blockIdx.x / ranks, j = blockIdx.x - request * ranks;
   const int L = p.req.length, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_wait();
-  pdl_release();  // (its stream of W does not get in front: the loads here are all on their way within the launch)
+  // behind the wait, on which the projection's own reads rely; its stream of W does not get in front: the loads here are
+  // all on their way within the launch
+  pdl_release();
   const int adapter = p.req.of_request(request);
   if (adapter < 0) {
     if (j == 0 && threadIdx.x == 0 && p.req.raw(request) != -1) report_error(p.status, FLUXB_ERR_BAD_ARG, 81);
@@ -371,7 +377,7 @@ __global__ void __launch_bounds__(256) lora_shrink_mma_kernel(const ShortParams 
   const int request = blockIdx.x / p.low.units, j0 = (blockIdx.x - request * p.low.units) * 16;
   const int L = p.req.length, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_wait();
-  pdl_release();
+  pdl_release();  // (behind the wait, as above)
   const int adapter = p.req.of_request(request);
   if (adapter < 0) {
     if (j0 == 0 && threadIdx.x == 0 && p.req.raw(request) != -1) report_error(p.status, FLUXB_ERR_BAD_ARG, 81);
@@ -581,6 +587,8 @@ __global__ void __launch_bounds__(THREADS, 1) lora_rows_kernel(const Params p) {
   const int g = lane >> 2, t4 = lane & 3;
   const int steps = p.piece / (WARPS * 32);  // of 32 columns per warp and piece
   const int col = warp * (p.piece / WARPS) + t4 * 8;
+  // x, like the adapters' indices, the bias and B above, is read without a wait: the low-rank kernel in front has waited for
+  // everything before it in every block by the time this one starts
   const __nv_bfloat16* xr = p.x + g * p.ldx;
   auto load_x = [&](int piece, int s) {
     const int k = piece * p.piece + col + s * 32;
