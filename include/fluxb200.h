@@ -308,7 +308,8 @@ int fluxb_layer_norm_modulation_stats(const void* x, const void* scale, const vo
 /*
  * y = (x - mean) * rstd * (unit + factor[g]) + offset[g], g = row / rows_per_group.  unit = 0 is
  * LayerNorm with a learned scale (one group: rows_per_group = rows), unit = 1 the modulated form.
- * Any width and alignment; x rows x_ld apart, y rows y_ld apart, factor and offset vec_stride
+ * Any width and alignment (for many rows of whole 16-byte pieces with unit = 1 the kernels of
+ * fluxb_layer_norm_modulation are the faster ones); x rows x_ld apart, y rows y_ld apart, factor and offset vec_stride
  * apart from group to group.  factor NULL: ones in place of unit + factor; offset NULL: zeros.
  * mean, rstd: fp32 per row, both or neither.  rows must be a multiple of rows_per_group.
  */

@@ -739,8 +739,8 @@ static BwdPlan bwd_plan(int64_t groups, int64_t rows_per_group, int64_t cols, in
       rows_at_once = 12;
       p.smem = ((size_t)(cols + 31) / 32 * 32 + 24 * (size_t)cols) * 4;
     } else {
-      // pieces per thread: the most that registers hold (two of bf16, four of fp32; three of bf16 spill and are left
-      // to rows of more than 8192), unless fewer leave fewer lanes without a column
+      // pieces per thread: the most that registers hold (two of bf16, four of fp32; three of bf16 spill 64 to 100
+      // bytes a thread and are left to rows of more than 8192), unless fewer leave fewer lanes without a column
       int64_t best = -1;
       for (int k = vn == 8 ? (v > 1024 ? 3 : 2) : 4; k >= 1; --k) {
         const int64_t w = (v + 32 * k - 1) / (32 * k);

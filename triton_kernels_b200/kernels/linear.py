@@ -216,7 +216,7 @@ def linear_lora(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None, lora_a
     low-rank adapter per request, a = adapter[request].  bf16 in/out, fp32 accumulation; forward only:
     where gradients are enabled, an argument that requires one (a weight or bias, too) is refused.
 
-    x [B, ..., K]: the first dim counts the requests (x [B, K] is one row per request).  w [N, K], b
+    K and N are multiples of 8.  x [B, ..., K]: the first dim counts the requests (x [B, K] is one row per request).  w [N, K], b
     [N] or None as in `linear`; lora_a [n, R, K], lora_b [n, N, R] bf16; lora_scale [n] fp32 or None
     (ones); adapter [B] int32 or int64 on x's device, -1 for a request without an adapter.  The
     values of `adapter` are read on the device: one outside [-1, n) counts as -1 and is recorded in
